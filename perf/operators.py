@@ -1,0 +1,461 @@
+"""The measured cases of the layer operators: layer norm and fragment attention, forward and backward.
+
+Layer norm (rows are atoms or edges, the last axis is the hidden width)
+
+    h = (x - mean(x)) / sqrt(var(x) + eps),   y = h w + b
+    g = dy w,   dx = (g - mean(g) - h mean(g h)) / sqrt(var + eps),   dw = sum_rows dy h,   db = sum_rows dy
+
+Fragment attention: a query row i and a key row j meet where they belong to the same fragment; for head a
+
+    s_ij = scale q_i.k_j - slope_a |x_i - x_j| + table[a, bucket(res_j - res_i)]
+    P = softmax_j(s),   o_i = sum_j P_ij v_j        (a query row without keys gives 0)
+    dP_ij = do_i.v_j,   dS = P (dP - sum_j P dP)
+    dq = scale dS k,  dk = scale dS^T q,  dv = P^T do
+    dslope_a = - sum dS |x_i - x_j|,   dtable[a, b] = sum of dS over the pairs of bucket b,
+    dpos = the positions' share of - slope_a dS |x_i - x_j|, summed over heads and over both ends of a pair
+
+The slope and the table are both optional; `bucket` maps the difference of two residue numbers, clipped to +-R.
+"""
+import math
+import random
+
+import numpy as np
+import torch
+
+own = False
+
+EPS = 1e-5
+TYPES = {"float32": torch.float32, "bfloat16": torch.bfloat16, "float16": torch.float16}
+BYTES = {"float32": 4, "bfloat16": 2, "float16": 2}
+PAIRS = 1 << 24  # (query, key, head) triples that the plain forms hold at a time
+
+
+# ---------------------------------------------------------------------------------------------------- the cases
+
+def listed():
+    return [
+        # the norm of one small protein's atoms (175) in an MD step's forward and force pass: latency
+        dict(name="norm_protein", op="norm", rows=175, width=256, dtype="float32", train=True),
+        # the atoms of a batch of 4096 fragments in mixed-precision training
+        dict(name="norm_fragments", op="norm", rows=80000, width=256, dtype="bfloat16", train=True),
+        # edge features of a full chunk of the engine's workspace (1 310 720 edge slots), inference
+        dict(name="norm_edges", op="norm", rows=1310720, width=256, dtype="float32", train=False),
+        # rows of an odd width: nothing is a multiple of a vector
+        dict(name="norm_odd", op="norm", rows=30011, width=509, dtype="float16", train=True),
+        # one whole protein of 175 atoms, inference: latency
+        dict(name="attn_protein", op="attention", layout="whole", sizes="175", heads=8, kv_heads=8, dim=32,
+             dtype="float32", slope=True, buckets=0, reach=0, train=False),
+        # 4096 fragments of a screening batch, energies and forces (gradients of q, k, v and positions)
+        dict(name="attn_fragments", op="attention", layout="fragments", count=4096, draw=11, heads=8, kv_heads=8,
+             dim=32, dtype="float32", slope=True, buckets=0, reach=0, train=True),
+        # one solvated protein (17 882 atoms), inference
+        dict(name="attn_solvated", op="attention", layout="whole", sizes="17882", heads=8, kv_heads=8, dim=32,
+             dtype="bfloat16", slope=True, buckets=0, reach=0, train=False),
+        # one read-out row per conformation, each over all atoms of a solvated protein, shared key heads
+        dict(name="attn_rows", op="attention", layout="rows", sizes="17882 746 17881 1 571 9001 281 175",
+             heads=8, kv_heads=2, dim=64, dtype="bfloat16", slope=True, buckets=0, reach=0, train=False),
+        # 4096 fragments in mixed-precision training, with the table of residue offsets
+        dict(name="bias_fragments", op="attention", layout="fragments", count=4096, draw=12, heads=8, kv_heads=8,
+             dim=32, dtype="bfloat16", slope=True, buckets=65, reach=32, train=True),
+        # four whole proteins of ragged sizes in one training step
+        dict(name="bias_proteins", op="attention", layout="whole", sizes="746 571 281 175", heads=8, kv_heads=8,
+             dim=32, dtype="float32", slope=False, buckets=32, reach=128, train=True),
+        # one long complex in half-precision training, wider heads that share keys two by two
+        dict(name="bias_long", op="attention", layout="whole", sizes="6007", heads=8, kv_heads=4, dim=64,
+             dtype="float16", slope=False, buckets=32, reach=128, train=True),
+        # a solvated protein in mixed-precision training, both terms
+        dict(name="bias_solvated", op="attention", layout="whole", sizes="17882", heads=8, kv_heads=8, dim=32,
+             dtype="bfloat16", slope=True, buckets=65, reach=32, train=True),
+    ]
+
+
+def _log_int(rng, low, high):
+    return max(low, min(high, round(math.exp(rng.uniform(math.log(low), math.log(high + 1))))))
+
+
+def _text(sizes):
+    return " ".join(str(n) for n in sizes)
+
+
+def draw(rng):
+    dtype = rng.choice(sorted(TYPES))
+    if rng.random() < 0.3:
+        width = rng.choice([64, 128, 192, 256, 320, 384, 448, 512, rng.randint(16, 1024)])
+        rows = _log_int(rng, 1, 1310720 * 256 // max(width, 256) // 2)
+        return dict(op="norm", rows=rows, width=width, dtype=dtype, train=rng.random() < 0.7)
+    dim = rng.choice([8, 16, 24, 32, 32, 40, 64, 64, 96, 128])
+    heads = rng.choice([1, 2, 3, 4, 5, 6, 8, 8, 12])
+    while heads * dim > 512:
+        heads = rng.choice([1, 2, 3, 4])
+    kv_heads = rng.choice([n for n in range(1, heads + 1) if heads % n == 0])
+    buckets, reach = rng.choice([(0, 0), (65, 32), (32, 128), (17, 8)])
+    case = dict(op="attention", heads=heads, kv_heads=kv_heads, dim=dim, dtype=dtype, buckets=buckets, reach=reach,
+                slope=buckets == 0 or rng.random() < 0.5, train=rng.random() < 0.6)
+    layout = rng.choice(["fragments", "whole", "long", "rows"])
+    if layout == "fragments":
+        case.update(layout="fragments", count=_log_int(rng, 1, 4096), draw=rng.randrange(1 << 20))
+    elif layout == "whole":
+        case.update(layout="whole", sizes=_text(_log_int(rng, 1, 1500) for _ in range(rng.randint(1, 8))))
+    elif layout == "long":
+        case.update(layout="whole", sizes=_text([_log_int(rng, 1500, 9000)]))
+    else:
+        case.update(layout="rows", sizes=_text(_log_int(rng, 1, 17882) for _ in range(rng.randint(1, 12))))
+    return case
+
+
+def _ranges(case):
+    """(query start, query end, key start, key end) of every fragment."""
+    if case["layout"] == "fragments":
+        pick = random.Random(case["draw"])  # dipeptides of 19 ... 36 atoms, every second fragment a 12-atom cap
+        sizes = [12 if n % 2 else pick.randint(19, 36) if pick.random() < 0.97 else 44 for n in range(case["count"])]
+    else:
+        sizes = [int(n) for n in case["sizes"].split()]
+    end = np.cumsum(np.asarray(sizes, dtype=np.int64))
+    start = end - np.asarray(sizes, dtype=np.int64)
+    if case["layout"] == "rows":
+        one = np.arange(len(sizes), dtype=np.int64)
+        return one, one + 1, start, end
+    return start, end, start, end
+
+
+def _bucket_map(case):
+    """The bucket of every clipped difference -R ... R: one each where there are enough of them, else exact near 0 and
+    logarithmic beyond, the two directions apart."""
+    reach, buckets = case["reach"], case["buckets"]
+    if buckets >= 2 * reach + 1:
+        return np.arange(2 * reach + 1, dtype=np.int32)
+    half = buckets // 2
+    exact = half // 2
+    out = []
+    for diff in range(-reach, reach + 1):
+        far = abs(diff)
+        if far < exact:
+            near = far
+        else:
+            near = exact + int(math.log(far / exact) / math.log(max(reach, 2) / exact) * (half - exact))
+        out.append(min(near, half - 1) + (half if diff > 0 else 0))
+    return np.asarray(out, dtype=np.int32)
+
+
+def work(case):
+    if case["op"] == "norm":
+        n = case["rows"] * case["width"]
+        size = BYTES[case["dtype"]]
+        if case["train"]:
+            return {"bytes": 5 * n * size, "flops": 20 * n}
+        return {"bytes": 2 * n * size, "flops": 8 * n}
+    q0, q1, k0, k1 = _ranges(case)
+    pairs = int(((q1 - q0) * (k1 - k0)).sum())
+    size, heads, dim = BYTES[case["dtype"]], case["heads"], case["dim"]
+    rows_q, rows_k = int(q1[-1]), int(k1[-1])
+    one = (2 * rows_q * heads + 2 * rows_k * case["kv_heads"]) * dim * size
+    extra = rows_k * (12 * case["slope"] + 4 * (case["buckets"] > 0))
+    if not case["train"]:
+        return {"bytes": one + extra, "flops": 4 * pairs * heads * dim}
+    grads = (2 * rows_q * heads + 2 * rows_k * case["kv_heads"]) * dim * size + rows_k * 12 * case["slope"]
+    return {"bytes": one + extra + grads, "flops": 14 * pairs * heads * dim}
+
+
+# ------------------------------------------------------------------------------------------------------- inputs
+
+def _chain(sizes, gen):
+    """Positions [Angstrom] of compact bodies at the density of a protein, and residue numbers along each of them."""
+    n = int(sum(sizes))
+    pos = torch.rand(n, 3, generator=gen, device="cuda")
+    edge = np.repeat([max(s, 1) ** (1 / 3) * 2.15 for s in sizes], sizes).astype(np.float32)
+    pos = pos * torch.as_tensor(edge, device="cuda")[:, None]
+    residue = np.concatenate([np.arange(s) // 12 for s in sizes]).astype(np.int32)
+    return pos, torch.as_tensor(residue, device="cuda")
+
+
+def prepare(case, seed):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    dtype = TYPES[case["dtype"]]
+
+    def normal(*shape, spread=1.0, as_type=dtype):
+        return (torch.randn(*shape, generator=gen, device="cuda") * spread).to(as_type)
+
+    if case["op"] == "norm":
+        rows, width = case["rows"], case["width"]
+        state = dict(case=case, x=normal(rows, width, spread=2.0) + 0.5, w=normal(width, spread=0.2) + 1.0,
+                     b=normal(width, spread=0.2))
+        if case["train"]:
+            state["dy"] = normal(rows, width)
+        return state
+    q0, q1, k0, k1 = _ranges(case)
+    heads, kv_heads, dim = case["heads"], case["kv_heads"], case["dim"]
+    rows_q, rows_k = int(q1[-1]), int(k1[-1])
+    state = dict(case=case, q=normal(rows_q, heads, dim), k=normal(rows_k, kv_heads, dim),
+                 v=normal(rows_k, kv_heads, dim), scale=dim ** -0.5)
+    pos, residue = _chain((k1 - k0).tolist(), gen)
+    apart = case["layout"] == "rows"  # a read-out row is a point of its own
+    if case["slope"]:
+        state["pos"] = pos
+        state["slope"] = torch.tensor([2.0 ** (-1 - 6 * a / heads) for a in range(heads)], device="cuda")
+        if apart:
+            state["query_pos"] = normal(rows_q, 3, spread=5.0, as_type=torch.float32)
+    if case["buckets"]:
+        state["residue"] = residue
+        state["table"] = normal(heads, case["buckets"], spread=0.5, as_type=torch.float32)
+        if apart:
+            state["query_residue"] = torch.randint(0, 64, (rows_q,), generator=gen, device="cuda", dtype=torch.int32)
+    if case["train"]:
+        state["dout"] = normal(rows_q, heads, dim)
+    bucket = _bucket_map(case) if case["buckets"] else None
+    if own:
+        from ai2bmd_amd.attention import FragmentAttention
+        state["plan"] = FragmentAttention(k0, k1, heads, dim, num_kv_heads=kv_heads, query_start=q0, query_end=q1,
+                                          buckets=bucket, device="cuda:0")
+    else:
+        state["bucket"] = None if bucket is None else torch.as_tensor(bucket, device="cuda").long()
+        state["groups"] = _groups(q0, q1, k0, k1, heads)
+    return state
+
+
+# ---------------------------------------------------------------------------------------------- the plain forms
+
+def _groups(q0, q1, k0, k1, heads):
+    """Fragments padded to a common size, as many together as PAIRS allows; a large one goes alone, in runs of rows."""
+    out, at = [], 0
+    while at < len(q0):
+        nq, nk, last = int(q1[at] - q0[at]), int(k1[at] - k0[at]), at + 1
+        if nq * nk * heads > PAIRS:
+            step = max(1, PAIRS // (nk * heads))
+            for row in range(int(q0[at]), int(q1[at]), step):
+                out.append((np.array([row]), np.array([min(row + step, int(q1[at]))]), k0[at:last], k1[at:last]))
+        else:
+            while last < len(q0):
+                wide_q, wide_k = max(nq, int(q1[last] - q0[last])), max(nk, int(k1[last] - k0[last]))
+                if (last + 1 - at) * wide_q * wide_k * heads > PAIRS:
+                    break
+                nq, nk, last = wide_q, wide_k, last + 1
+            out.append((q0[at:last], q1[at:last], k0[at:last], k1[at:last]))
+        at = last
+    made = []
+    for a, b, c, d in out:
+        made.append([t for lo, hi in ((a, b), (c, d)) for t in _padded(lo, hi)])
+    return made
+
+
+def _padded(low, high):
+    rows = low[:, None] + np.arange(int((high - low).max()))[None, :]
+    live = rows < high[:, None]
+    return torch.as_tensor(np.where(live, rows, 0), device="cuda"), torch.as_tensor(live, device="cuda")
+
+
+def _plain_norm(state):
+    case = state["case"]
+    dtype = TYPES[case["dtype"]]
+    x, w, b = state["x"].float(), state["w"].float(), state["b"].float()
+    off = x - x.mean(-1, keepdim=True)
+    rstd = torch.rsqrt((off * off).mean(-1, keepdim=True) + EPS)
+    h = off * rstd
+    y = (h * w + b).to(dtype)
+    if not case["train"]:
+        return y
+    dy = state["dy"].float()
+    g = dy * w
+    dx = (g - g.mean(-1, keepdim=True) - h * (g * h).mean(-1, keepdim=True)) * rstd
+    return {"y": y, "dx": dx.to(dtype), "dw": (dy * h).sum(0).to(dtype), "db": dy.sum(0).to(dtype)}
+
+
+def _plain_attention(state):
+    case = state["case"]
+    dtype, heads, kv_heads, dim = TYPES[case["dtype"]], case["heads"], case["kv_heads"], case["dim"]
+    share, train = heads // kv_heads, case["train"]
+    pos, residue = state.get("pos"), state.get("residue")
+    query_pos, query_residue = state.get("query_pos", pos), state.get("query_residue", residue)
+    q, k, v = state["q"].float(), state["k"].float(), state["v"].float()
+    out = torch.zeros_like(q)
+    if train:
+        dout = state["dout"].float()
+        dq, dk, dv = torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v)
+        if pos is not None:
+            dslope = torch.zeros(heads, dtype=torch.float64, device="cuda")
+            dpos = torch.zeros_like(pos)
+            dquery_pos = torch.zeros_like(query_pos)
+        if residue is not None:
+            dtable = torch.zeros(heads, case["buckets"], dtype=torch.float64, device="cuda")
+    for qi, q_live, ki, k_live in state["groups"]:
+        qg = q[qi].transpose(1, 2)
+        kg = k[ki].transpose(1, 2).repeat_interleave(share, 1)
+        vg = v[ki].transpose(1, 2).repeat_interleave(share, 1)
+        s = (qg @ kg.transpose(2, 3)) * state["scale"]
+        if pos is not None:
+            off = query_pos[qi][:, :, None] - pos[ki][:, None]
+            far = (off * off).sum(-1).sqrt()
+            s = s - state["slope"][:, None, None] * far[:, None]
+        if residue is not None:
+            reach = case["reach"]
+            diff = residue[ki][:, None].long() - query_residue[qi][:, :, None].long()
+            bucket = state["bucket"][diff.clamp(-reach, reach) + reach]
+            s = s + state["table"][:, bucket].transpose(0, 1)
+        both = (q_live[:, :, None] & k_live[:, None])[:, None]
+        s = s.masked_fill(~both, -math.inf)
+        top = s.amax(-1, keepdim=True)
+        top = torch.where(top == -math.inf, torch.zeros_like(top), top)
+        p = (s - top).exp()
+        total = p.sum(-1, keepdim=True)
+        p = p / torch.where(total == 0, torch.ones_like(total), total)
+        out[qi[q_live]] = (p @ vg).transpose(1, 2)[q_live]
+        if not train:
+            continue
+        dog = dout[qi].transpose(1, 2)
+        dp = dog @ vg.transpose(2, 3)
+        ds = p * (dp - (p * dp).sum(-1, keepdim=True))
+        dq[qi[q_live]] = (ds @ kg).transpose(1, 2)[q_live] * state["scale"]
+        count, nk = ki.shape
+        shared = (count, kv_heads, share, nk, dim)
+        dk[ki[k_live]] += (ds.transpose(2, 3) @ qg).view(shared).sum(2).transpose(1, 2)[k_live] * state["scale"]
+        dv[ki[k_live]] += (p.transpose(2, 3) @ dog).view(shared).sum(2).transpose(1, 2)[k_live]
+        if pos is not None:
+            dslope -= (ds * far[:, None]).sum((0, 2, 3)).double()
+            pull = -(ds * state["slope"][:, None, None]).sum(1)
+            pull = (pull / torch.where(far == 0, torch.ones_like(far), far))[..., None] * off
+            dquery_pos[qi[q_live]] += pull.sum(2)[q_live]
+            dpos[ki[k_live]] -= pull.sum(1)[k_live]
+        if residue is not None:
+            spread = ds.transpose(0, 1).reshape(heads, -1)
+            hot = torch.zeros(bucket.numel(), case["buckets"], device="cuda")
+            hot.scatter_(1, bucket.view(-1, 1), 1.0)
+            dtable += (spread @ hot).double()
+    if not train:
+        return out.to(dtype)
+    res = {"out": out.to(dtype), "dq": dq.to(dtype), "dk": dk.to(dtype), "dv": dv.to(dtype)}
+    if pos is not None:
+        res["dslope"] = dslope.float()
+        if "query_pos" in state:
+            res["dpos"], res["dquery_pos"] = dpos, dquery_pos
+        else:
+            res["dpos"] = dpos + dquery_pos
+    if residue is not None:
+        res["dtable"] = dtable.float()
+    return res
+
+
+def _own_norm(state):
+    from ai2bmd_amd.norm import layer_norm, layer_norm_backward
+    y, stats = layer_norm(state["x"], state["w"], state["b"], eps=EPS)
+    if not state["case"]["train"]:
+        return y
+    dx, dw, db = layer_norm_backward(state["dy"], state["x"], stats, state["w"], state["b"])
+    return {"y": y, "dx": dx, "dw": dw, "db": db}
+
+
+def _own_attention(state):
+    terms = {name: state[name] for name in ("pos", "slope", "residue", "table", "query_pos", "query_residue", "scale")
+             if name in state}
+    plan, q, k, v = state["plan"], state["q"], state["k"], state["v"]
+    if not state["case"]["train"]:
+        return plan.forward(q, k, v, **terms)
+    out, saved = plan.forward(q, k, v, save=True, **terms)
+    grads = plan.backward(state["dout"], q, k, v, saved, **terms)
+    res = {"out": out, "dq": grads.dq, "dk": grads.dk, "dv": grads.dv}
+    for name in ("dslope", "dpos", "dquery_pos", "dtable"):
+        if getattr(grads, name) is not None:
+            res[name] = getattr(grads, name)
+    return res
+
+
+def run(state):
+    if state["case"]["op"] == "norm":
+        return _own_norm(state) if own else _plain_norm(state)
+    return _own_attention(state) if own else _plain_attention(state)
+
+
+# ------------------------------------------------------------------------------------- the definitions, in 64 bits
+
+def _exact_norm(case, state):
+    x = state["x"].double().requires_grad_(case["train"])
+    w = state["w"].double().requires_grad_(case["train"])
+    b = state["b"].double().requires_grad_(case["train"])
+    var, mean = torch.var_mean(x, dim=1, correction=0, keepdim=True)
+    y = (x - mean) / torch.sqrt(var + EPS) * w + b
+    if not case["train"]:
+        return y
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), state["dy"].double())
+    return {"y": y.detach(), "dx": dx, "dw": dw, "db": db}
+
+
+def _exact_attention(case, state):
+    """Fragments of one size are taken together, without padding; the gradients are torch's, of the scores' formula."""
+    heads, kv_heads, dim, train = case["heads"], case["kv_heads"], case["dim"], case["train"]
+    slope, table = case["slope"], case["buckets"] > 0
+    q0, q1, k0, k1 = _ranges(case)
+    like = sorted(range(len(q0)), key=lambda f: (q1[f] - q0[f], k1[f] - k0[f]))
+    pieces, at = [], 0
+    while at < len(like):
+        f = like[at]
+        nq, nk = int(q1[f] - q0[f]), int(k1[f] - k0[f])
+        most, last = max(1, PAIRS // max(1, nq * nk * heads)), at + 1
+        while last < len(like) and last - at < most and \
+                (q1[like[last]] - q0[like[last]], k1[like[last]] - k0[like[last]]) == (nq, nk):
+            last += 1
+        some = like[at:last]
+        step = max(1, PAIRS // max(1, nk * heads)) if len(some) == 1 else nq
+        for row in range(0, nq, max(step, 1)):
+            rows = np.arange(row, min(nq, row + step))
+            pieces.append((torch.as_tensor(q0[some][:, None] + rows, device="cuda"),
+                           torch.as_tensor(k0[some][:, None] + np.arange(nk), device="cuda")))
+        at = last
+    rows_q, rows_k = int(q1[-1]), int(k1[-1])
+    full = dict(dtype=torch.float64, device="cuda")
+    res = {"out": torch.zeros(rows_q, heads, dim, **full)}
+    if train:
+        res.update(dq=torch.zeros(rows_q, heads, dim, **full), dk=torch.zeros(rows_k, kv_heads, dim, **full),
+                   dv=torch.zeros(rows_k, kv_heads, dim, **full))
+        if slope:
+            res.update(dslope=torch.zeros(heads, **full), dpos=torch.zeros(rows_k, 3, **full))
+            if "query_pos" in state:
+                res["dquery_pos"] = torch.zeros(rows_q, 3, **full)
+        if table:
+            res["dtable"] = torch.zeros(heads, case["buckets"], **full)
+    lut = torch.as_tensor(_bucket_map(case), device="cuda").long() if table else None
+    for qi, ki in pieces:
+        if ki.shape[1] == 0:
+            continue
+        leaf = {"q": state["q"][qi].double(), "k": state["k"][ki].double(), "v": state["v"][ki].double()}
+        if slope:
+            leaf.update(here=state.get("query_pos", state["pos"])[qi].double(), there=state["pos"][ki].double(),
+                        slope=state["slope"].double())
+        for value in leaf.values():
+            value.requires_grad_(train)
+        split = leaf["q"].reshape(*qi.shape, kv_heads, heads // kv_heads, dim).permute(0, 2, 3, 1, 4)
+        keys = leaf["k"].permute(0, 2, 3, 1).unsqueeze(2)
+        score = (torch.matmul(split, keys) * state["scale"]).reshape(qi.shape[0], heads, qi.shape[1], ki.shape[1])
+        if slope:
+            square = (leaf["here"].unsqueeze(2) - leaf["there"].unsqueeze(1)).pow(2).sum(-1)
+            same = square == 0
+            dist = torch.where(same, 0.0, torch.sqrt(torch.where(same, 1.0, square)))
+            score = score - leaf["slope"].view(1, -1, 1, 1) * dist.unsqueeze(1)
+        if table:
+            here = state.get("query_residue", state["residue"])[qi].long()
+            diff = state["residue"][ki].long().unsqueeze(1) - here.unsqueeze(2)
+            kind = lut[torch.clamp(diff, -case["reach"], case["reach"]) + case["reach"]]
+            score = score + state["table"].double()[:, kind].permute(1, 0, 2, 3)
+        weight = torch.softmax(score, -1)
+        grouped = weight.reshape(qi.shape[0], kv_heads, heads // kv_heads, qi.shape[1], ki.shape[1])
+        mixed = torch.matmul(grouped, leaf["v"].permute(0, 2, 1, 3).unsqueeze(2))
+        mixed = mixed.permute(0, 3, 1, 2, 4).reshape(qi.shape[0], qi.shape[1], heads, dim)
+        res["out"][qi] = mixed.detach()
+        if not train:
+            continue
+        names = list(leaf)
+        grads = torch.autograd.grad(mixed, [leaf[n] for n in names] + [score], state["dout"][qi].double())
+        grad = dict(zip(names, grads))
+        res["dq"][qi] = grad["q"]
+        res["dk"][ki] += grad["k"]
+        res["dv"][ki] += grad["v"]
+        if slope:
+            res["dslope"] += grad["slope"]
+            res["dpos"][ki] += grad["there"]
+            res["dquery_pos" if "query_pos" in state else "dpos"][qi] += grad["here"]
+        if table:
+            for b in range(case["buckets"]):
+                res["dtable"][:, b] += torch.where((kind == b).unsqueeze(1), grads[-1], 0.0).sum((0, 2, 3))
+    return res if train else res["out"]
+
+
+def exact(case, seed):
+    state = prepare(case, seed)
+    return _exact_norm(case, state) if case["op"] == "norm" else _exact_attention(case, state)
