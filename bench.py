@@ -885,7 +885,7 @@ def _cpu_evaluator(hp, sd):
     from oracle.visnet_oracle import ViSNetOracle
 
     o = ViSNetOracle(hp, sd, torch.float32)
-    return "port", "oracle/visnet_oracle.py (fp32 torch + autograd)", o.energy_forces
+    return "port", "oracle/visnet_oracle.py (fp32 torch + autograd)", lambda *batch: o.energy_forces(*batch)[:2]
 
 
 def physical_core_count():
