@@ -52,6 +52,7 @@ class VsnHoptTerms(C.Structure):
 VECNORM = {"none": 0, "rms": 1, "max_min": 2}
 RBF = {"expnorm": 0, "gauss": 1}
 ACTIVATION = {"silu": 0, "swish": 0, "ssp": 1, "tanh": 2, "sigmoid": 3}  # utils.py:93-116 act_class_mapping
+DTYPE = {"float32": 0, "bfloat16": 1, "float16": 2}  # VSN_F32, VSN_BF16, VSN_F16 (include/vsn.h)
 P2P_HANDLE_BYTES = 128  # VSN_P2P_HANDLE_BYTES (include/vsn.h)
 _lib = None
 
@@ -180,6 +181,13 @@ def lib() -> C.CDLL:
     L.vsn_hopt_stats.restype = C.c_int
     L.vsn_partition.argtypes = [i64p, i64p, C.c_int64, C.c_int, C.c_int64, i64p, C.c_int]
     L.vsn_partition.restype = C.c_int
+    i32, i64 = C.c_int, C.c_int64
+    L.vsn_layernorm.argtypes = [i32, i32, i32, vp, i64, vp, vp, i64, i32, C.c_float, vp, i64, vp, vp]
+    L.vsn_layernorm.restype = i32
+    L.vsn_layernorm_workspace.argtypes = [i64, i32]
+    L.vsn_layernorm_workspace.restype = i64
+    L.vsn_layernorm_backward.argtypes = [i32, i32, i32, vp, i64, vp, i64, vp, vp, i64, i32, vp, i64, vp, vp, vp, i64, vp]
+    L.vsn_layernorm_backward.restype = i32
     _lib = L
     return L
 
@@ -196,4 +204,5 @@ EXPORTS = [
     "vsn_p2p_create", "vsn_p2p_export", "vsn_p2p_connect", "vsn_p2p_send_buffer", "vsn_p2p_gather_buffer", "vsn_p2p_set_timeout", "vsn_p2p_allgather", "vsn_p2p_status", "vsn_p2p_destroy",
     "vsn_build_fragments", "vsn_md_create", "vsn_md_destroy", "vsn_md_half1", "vsn_md_half2", "vsn_md_set_noise", "vsn_md_half1_build", "vsn_md_half1_build_relax", "vsn_md_combine_half2", "vsn_md_set_restraints", "vsn_md_restrain", "vsn_md_observe", "vsn_mm_create", "vsn_mm_destroy", "vsn_mm_forces",
     "vsn_hopt_create", "vsn_hopt_destroy", "vsn_hopt_run", "vsn_hopt_stats",
+    "vsn_layernorm", "vsn_layernorm_workspace", "vsn_layernorm_backward",
 ]

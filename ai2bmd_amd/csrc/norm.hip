@@ -1,0 +1,297 @@
+// Layer norm over the last axis, forward and backward with the gradients of weight and bias, as an operator of its own
+// (the ViS-MP layer's torch.nn.LayerNorm, ViSNet/model/visnet_block.py:180,237; the engine's node walks hold the same
+// norm fused and need only its input adjoint).
+//
+//   h = (x - mean) rstd,  rstd = 1 / sqrt(mean((x - mean)^2) + eps),  y = h w + b
+//   g = dy w,  dx = rstd (g - mean(g) - h mean(g h)),  dw = sum_rows dy h,  db = sum_rows dy
+//
+// Bound by memory: x and y once forward; x, dy and dx once backward.  LPR lanes hold one row in registers (NV vectors of
+// 16 bytes each), so the mean is subtracted before the squares are summed and nothing is read twice; narrow rows put
+// 64 / LPR rows into a wave.  A lane keeps its columns for all the rows it visits: weight and bias stay in registers, and
+// so do the column sums of the backward pass, which are joined over the workgroup in LDS and over the workgroups by a
+// second launch, both in a fixed order (no atomics: equal inputs give equal bits).  All sums are float32.
+// Vector loads need only element alignment (gfx950 takes global addresses of any alignment); the row's last, partial
+// vector goes element by element.
+#include "typed.h"
+
+namespace vsn {
+
+template <typename T, int VEC>
+__device__ __forceinline__ void load_row(const T* __restrict__ p, int at, int width, float (&v)[VEC]) {
+  if (at + VEC <= width) {
+    T tmp[VEC];
+    __builtin_memcpy(tmp, p + at, sizeof(tmp));
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v[i] = (float)tmp[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v[i] = at + i < width ? (float)p[at + i] : 0.f;
+  }
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void store_row(T* __restrict__ p, int at, int width, const float (&v)[VEC]) {
+  if (at + VEC <= width) {
+    T tmp[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) tmp[i] = (T)v[i];
+    __builtin_memcpy(p + at, tmp, sizeof(tmp));
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i)
+      if (at + i < width) p[at + i] = (T)v[i];
+  }
+}
+// weight / bias columns of one lane: the rows' type or float32; absent = `fill`
+template <typename T, int VEC>
+__device__ __forceinline__ void load_param(const void* p, int is_f32, int at, int width, float fill, float (&v)[VEC]) {
+#pragma unroll
+  for (int i = 0; i < VEC; ++i)
+    v[i] = at + i >= width ? 0.f : !p ? fill : is_f32 ? ((const float*)p)[at + i] : (float)((const T*)p)[at + i];
+}
+template <int LPR>
+__device__ __forceinline__ float row_sum(float v) {
+#pragma unroll
+  for (int o = LPR / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+
+template <typename T, int VEC, int LPR, int NV>
+__global__ __launch_bounds__(256) void k_layernorm(const T* __restrict__ x, int64_t ldx, const void* __restrict__ w,
+                                                   const void* __restrict__ b, int param_f32, int64_t rows, int width,
+                                                   float inv_width, float eps, T* __restrict__ y, int64_t ldy,
+                                                   float2* __restrict__ stats) {
+  constexpr int RPB = 256 / LPR;  // rows of a workgroup per turn
+  const int lane = threadIdx.x % LPR;
+  float wv[NV][VEC], bv[NV][VEC];
+#pragma unroll
+  for (int n = 0; n < NV; ++n) {
+    load_param<T, VEC>(w, param_f32, (n * LPR + lane) * VEC, width, 1.f, wv[n]);
+    load_param<T, VEC>(b, param_f32, (n * LPR + lane) * VEC, width, 0.f, bv[n]);
+  }
+  for (int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / LPR; row < rows; row += (int64_t)gridDim.x * RPB) {
+    float v[NV][VEC];
+    float s = 0.f;
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      load_row<T, VEC>(x + row * ldx, (n * LPR + lane) * VEC, width, v[n]);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) s += v[n][i];
+    }
+    const float mean = row_sum<LPR>(s) * inv_width;
+    float q = 0.f;
+#pragma unroll
+    for (int n = 0; n < NV; ++n)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        v[n][i] = (n * LPR + lane) * VEC + i < width ? v[n][i] - mean : 0.f;
+        q += v[n][i] * v[n][i];
+      }
+    const float rstd = 1.f / sqrtf(row_sum<LPR>(q) * inv_width + eps);
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) v[n][i] = v[n][i] * rstd * wv[n][i] + bv[n][i];
+      store_row<T, VEC>(y + row * ldy, (n * LPR + lane) * VEC, width, v[n]);
+    }
+    if (stats && lane == 0) stats[row] = make_float2(mean, rstd);
+  }
+}
+
+// partial: [gridDim.x][2][width] column sums of dy h and dy
+template <typename T, int VEC, int LPR, int NV>
+__global__ __launch_bounds__(256) void k_layernorm_bwd(const T* __restrict__ dy, int64_t lddy, const T* __restrict__ x,
+                                                       int64_t ldx, const float2* __restrict__ stats,
+                                                       const void* __restrict__ w, int param_f32, int64_t rows,
+                                                       int width, float inv_width, T* __restrict__ dx, int64_t lddx,
+                                                       float* __restrict__ partial) {
+  constexpr int RPB = 256 / LPR;
+  const int lane = threadIdx.x % LPR;
+  float wv[NV][VEC], aw[NV][VEC], ab[NV][VEC];
+#pragma unroll
+  for (int n = 0; n < NV; ++n) {
+    load_param<T, VEC>(w, param_f32, (n * LPR + lane) * VEC, width, 1.f, wv[n]);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) aw[n][i] = ab[n][i] = 0.f;
+  }
+  for (int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / LPR; row < rows; row += (int64_t)gridDim.x * RPB) {
+    const float2 st = stats[row];
+    float h[NV][VEC], g[NV][VEC];
+    float sg = 0.f, sgh = 0.f;
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      load_row<T, VEC>(x + row * ldx, (n * LPR + lane) * VEC, width, h[n]);
+      load_row<T, VEC>(dy + row * lddy, (n * LPR + lane) * VEC, width, g[n]);
+    }
+#pragma unroll
+    for (int n = 0; n < NV; ++n)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        h[n][i] = (n * LPR + lane) * VEC + i < width ? (h[n][i] - st.x) * st.y : 0.f;
+        aw[n][i] += g[n][i] * h[n][i];
+        ab[n][i] += g[n][i];
+        g[n][i] *= wv[n][i];
+        sg += g[n][i];
+        sgh += g[n][i] * h[n][i];
+      }
+    sg = row_sum<LPR>(sg) * inv_width;
+    sgh = row_sum<LPR>(sgh) * inv_width;
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) g[n][i] = st.y * (g[n][i] - sg - h[n][i] * sgh);
+      store_row<T, VEC>(dx + row * lddx, (n * LPR + lane) * VEC, width, g[n]);
+    }
+  }
+  if (!partial) return;
+  // the RPB row groups of the workgroup hold the same columns: added one after the other, in their order
+  __shared__ float sw[NV * LPR * VEC], sb[NV * LPR * VEC];
+  for (int r = 0; r < RPB; ++r) {
+    if ((int)threadIdx.x / LPR == r)
+#pragma unroll
+      for (int n = 0; n < NV; ++n)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          const int c = (n * VEC + i) * LPR + lane;  // lanes side by side: no bank is hit twice
+          sw[c] = r ? sw[c] + aw[n][i] : aw[n][i];
+          sb[c] = r ? sb[c] + ab[n][i] : ab[n][i];
+        }
+    __syncthreads();
+  }
+  float* out = partial + (size_t)blockIdx.x * 2 * width;
+  for (int c = threadIdx.x; c < width; c += 256) {
+    const int n = c / (LPR * VEC), l = c / VEC % LPR, i = c % VEC;
+    out[c] = sw[(n * VEC + i) * LPR + l];
+    out[width + c] = sb[(n * VEC + i) * LPR + l];
+  }
+}
+
+// dw and db from the workgroups' partial sums: 32 columns x 8 strided rows of partials per workgroup
+template <typename T>
+__global__ __launch_bounds__(256) void k_layernorm_params(const float* __restrict__ partial, int groups, int width,
+                                                          void* __restrict__ dw, void* __restrict__ db,
+                                                          int param_f32) {
+  __shared__ float red[8][33];
+  const int c = blockIdx.x * 32 + threadIdx.x % 32, r = threadIdx.x / 32;
+  const int which = blockIdx.y;
+  float s = 0.f;
+  if (c < width)
+    for (int g = r; g < groups; g += 8) s += partial[((size_t)g * 2 + which) * width + c];
+  red[r][threadIdx.x % 32] = s;
+  __syncthreads();
+  void* out = which ? db : dw;
+  if (r == 0 && c < width && out) {
+#pragma unroll
+    for (int k = 1; k < 8; ++k) s += red[k][threadIdx.x];
+    if (param_f32)
+      ((float*)out)[c] = s;
+    else
+      ((T*)out)[c] = (T)s;
+  }
+}
+
+constexpr int kNormWidth = 4096;
+constexpr int kNormGroups = 1024;
+
+static int norm_groups(int64_t rows, int rows_per_group, int cap) {
+  const int64_t need = (rows + rows_per_group - 1) / rows_per_group;
+  return (int)(need < cap ? need : cap);
+}
+
+struct NormArgs {
+  const void *x, *dy, *w, *b;
+  void *y, *dx, *dw, *db;
+  float *stats, *partial;
+  int64_t ldx, ldy, lddy, lddx, rows;
+  int width, param_f32;
+  float eps;
+  bool backward;
+};
+
+template <typename T, int VEC, int LPR, int NV>
+static void norm_launch(const NormArgs& a, hipStream_t st) {
+  const float inv = 1.0f / (float)a.width;
+  const int rpb = 256 / LPR;
+  if (!a.backward) {
+    if (!a.rows) return;
+    hipLaunchKernelGGL((k_layernorm<T, VEC, LPR, NV>), dim3(norm_groups(a.rows, rpb, 4096)), dim3(256), 0, st,
+                       (const T*)a.x, a.ldx, a.w, a.b, a.param_f32, a.rows, a.width, inv, a.eps, (T*)a.y, a.ldy,
+                       (float2*)a.stats);
+    return;
+  }
+  const int groups = norm_groups(a.rows, rpb, kNormGroups);
+  float* partial = a.dw || a.db ? a.partial : nullptr;
+  if (groups)
+    hipLaunchKernelGGL((k_layernorm_bwd<T, VEC, LPR, NV>), dim3(groups), dim3(256), 0, st, (const T*)a.dy, a.lddy,
+                       (const T*)a.x, a.ldx, (const float2*)a.stats, a.w, a.param_f32, a.rows, a.width, inv, (T*)a.dx,
+                       a.lddx, partial);
+  if (partial || (!groups && (a.dw || a.db)))
+    hipLaunchKernelGGL((k_layernorm_params<T>), dim3((a.width + 31) / 32, 2), dim3(256), 0, st, partial, groups,
+                       a.width, a.dw, a.db, a.param_f32);
+}
+
+template <typename T, int VEC>
+static void norm_pick(const NormArgs& a, hipStream_t st) {
+  const int n = a.width;
+  if (n <= 8 * VEC) return norm_launch<T, VEC, 8, 1>(a, st);
+  if (n <= 16 * VEC) return norm_launch<T, VEC, 16, 1>(a, st);
+  if (n <= 32 * VEC) return norm_launch<T, VEC, 32, 1>(a, st);
+  if (n <= 64 * VEC) return norm_launch<T, VEC, 64, 1>(a, st);
+  if (n <= 128 * VEC) return norm_launch<T, VEC, 64, 2>(a, st);
+  if (n <= 256 * VEC) return norm_launch<T, VEC, 64, 4>(a, st);
+  if (n <= 512 * VEC) return norm_launch<T, VEC, 64, 8>(a, st);
+  if constexpr (VEC == 4) return norm_launch<T, VEC, 64, 16>(a, st);
+}
+
+static int norm_dispatch(int dtype, const NormArgs& a, hipStream_t st) {
+  switch (dtype) {
+    case VSN_F32: norm_pick<float, 4>(a, st); break;
+    case VSN_BF16: norm_pick<__bf16, 8>(a, st); break;
+    default: norm_pick<_Float16, 8>(a, st); break;
+  }
+  return hipGetLastError() == hipSuccess ? 0 : -5;
+}
+
+static bool norm_bad(int dtype, int param_dtype, int64_t rows, int width) {
+  return dtype < VSN_F32 || dtype > VSN_F16 || (param_dtype != dtype && param_dtype != VSN_F32) || rows < 0 ||
+         width < 1 || width > kNormWidth;
+}
+
+}  // namespace vsn
+
+extern "C" int vsn_layernorm(int device_id, int dtype, int param_dtype, const void* dev_x, int64_t ldx,
+                             const void* dev_w, const void* dev_b, int64_t rows, int width, float eps, void* dev_y,
+                             int64_t ldy, float* dev_stats, void* stream) {
+  if (vsn::norm_bad(dtype, param_dtype, rows, width) || !(eps >= 0.f)) return -22;
+  if (rows && (!dev_x || !dev_y || ldx < width || ldy < width)) return -22;
+  vsn::DeviceScope scope(device_id);
+  if (!scope.ok) return -19;
+  vsn::NormArgs a = {};
+  a.x = dev_x, a.w = dev_w, a.b = dev_b, a.y = dev_y, a.stats = dev_stats;
+  a.ldx = ldx, a.ldy = ldy, a.rows = rows, a.width = width, a.param_f32 = param_dtype == VSN_F32, a.eps = eps;
+  return vsn::norm_dispatch(dtype, a, (hipStream_t)stream);
+}
+
+extern "C" int64_t vsn_layernorm_workspace(int64_t rows, int width) {
+  if (rows < 0 || width < 1 || width > vsn::kNormWidth) return -22;
+  // at least 4 rows per workgroup, whatever the lanes per row (norm_launch)
+  const int64_t groups = rows / 4 + 1 < vsn::kNormGroups ? rows / 4 + 1 : vsn::kNormGroups;
+  return groups * 2 * width * (int64_t)sizeof(float);
+}
+
+extern "C" int vsn_layernorm_backward(int device_id, int dtype, int param_dtype, const void* dev_dy, int64_t lddy,
+                                      const void* dev_x, int64_t ldx, const float* dev_stats, const void* dev_w,
+                                      int64_t rows, int width, void* dev_dx, int64_t lddx, void* dev_dw, void* dev_db,
+                                      void* dev_workspace, int64_t workspace_bytes, void* stream) {
+  if (vsn::norm_bad(dtype, param_dtype, rows, width)) return -22;
+  if (rows && (!dev_dy || !dev_x || !dev_stats || !dev_dx || lddy < width || ldx < width || lddx < width)) return -22;
+  if (rows && (dev_dw || dev_db) && (!dev_workspace || workspace_bytes < vsn_layernorm_workspace(rows, width)))
+    return -22;
+  vsn::DeviceScope scope(device_id);
+  if (!scope.ok) return -19;
+  vsn::NormArgs a = {};
+  a.backward = true;
+  a.dy = dev_dy, a.x = dev_x, a.w = dev_w, a.dx = dev_dx, a.dw = dev_dw, a.db = dev_db;
+  a.stats = (float*)dev_stats, a.partial = (float*)dev_workspace;
+  a.lddy = lddy, a.ldx = ldx, a.lddx = lddx, a.rows = rows, a.width = width, a.param_f32 = param_dtype == VSN_F32;
+  return vsn::norm_dispatch(dtype, a, (hipStream_t)stream);
+}

@@ -1,0 +1,133 @@
+"""Layer norm on the MI355X as an operator, forward and backward with the gradients of weight and bias.
+
+The norm of the reference's ViS-MP layer (torch.nn.LayerNorm, ViSNet/model/visnet_block.py:180,237), for rows of atoms or
+edges outside the force engine, which holds the same norm fused and frozen: a layer that is trained needs dx, dw and db.
+Like everything here it is differentiated by hand: the two functions are called explicitly and build no autograd graph.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from . import capi
+
+MAX_WIDTH = 4096
+
+
+def dtype_code(t: torch.Tensor, name: str) -> int:
+    code = capi.DTYPE.get(str(t.dtype).replace("torch.", ""))
+    if code is None:
+        raise ValueError(f"{name}: float32, bfloat16 or float16 expected, not {t.dtype}")
+    return code
+
+
+def on_device(t: torch.Tensor, name: str, device=None) -> None:
+    if not t.is_cuda:
+        raise ValueError(f"{name}: this package is the MI355X path ('cuda:<k>' tensors only), got one on {t.device}")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name} is on {t.device}, expected {device}")
+
+
+def no_graph(*tensors) -> None:
+    """The operators build no autograd graph; a result that silently cut one would train nothing."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError("no autograd graph is built: call under torch.no_grad() and use the backward function")
+
+
+def ptr(t):
+    return C.c_void_p(t.data_ptr() if t is not None else 0)
+
+
+def stream_of(t: torch.Tensor):
+    return C.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+
+
+def _rows(t: torch.Tensor, name: str):
+    """(tensor, rows, elements between rows): the tensor as it is where its rows are evenly spaced, else a copy."""
+    width = t.shape[-1]
+    if t.numel() == 0:
+        return t, t.numel() // max(width, 1), width
+    if t.stride(-1) == 1 or width == 1:
+        lead = [(n, s) for n, s in zip(t.shape[:-1], t.stride()[:-1]) if n != 1]
+        if all(lead[i][1] == lead[i + 1][0] * lead[i + 1][1] for i in range(len(lead) - 1)):
+            step = lead[-1][1] if lead else width
+            if step >= width:
+                return t, t.numel() // width, step
+    return t.contiguous(), t.numel() // width, width
+
+
+def _param(p, x, name: str) -> None:
+    if p is None:
+        return
+    on_device(p, name, x.device)
+    if p.shape != (x.shape[-1],) or not p.is_contiguous():
+        raise ValueError(f"{name}: contiguous [{x.shape[-1]}] expected, got {tuple(p.shape)}")
+    if p.dtype not in (x.dtype, torch.float32):
+        raise ValueError(f"{name}: {x.dtype} or float32 expected, not {p.dtype}")
+
+
+def _check(x, weight, bias) -> int:
+    on_device(x, "x")
+    dtype_code(x, "x")
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_WIDTH:
+        raise ValueError(f"x: a last axis of 1 ... {MAX_WIDTH} expected, got {tuple(x.shape)}")
+    _param(weight, x, "weight")
+    _param(bias, x, "bias")
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise ValueError("weight and bias differ in type")
+    of = weight if weight is not None else bias
+    return dtype_code(of if of is not None else x, "weight")
+
+
+def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, out=None):
+    """y = (x - mean) / sqrt(var + eps) * weight + bias over the last axis -> (y, stats).
+
+    `x` [..., width], float32 / bfloat16 / float16; evenly spaced rows are read in place, other layouts are copied.
+    `weight`, `bias` [width] of x's type or float32 (None: 1 and 0).  `out`: contiguous, of x's shape and type; it may be x.
+    `stats` float32 [rows, 2] (mean, 1 / sqrt(var + eps)) goes to layer_norm_backward.  On the current stream of x's device."""
+    code = _check(x, weight, bias)
+    no_graph(x, weight, bias)
+    if not eps >= 0:
+        raise ValueError("eps: a number >= 0 expected")
+    if out is not None:
+        on_device(out, "out", x.device)
+        if out.shape != x.shape or out.dtype != x.dtype or not out.is_contiguous():
+            raise ValueError("out: contiguous, with x's shape and type expected")
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else out
+    src, rows, ld = _rows(x, "x")
+    stats = torch.empty(rows, 2, dtype=torch.float32, device=x.device)
+    rc = capi.lib().vsn_layernorm(x.device.index, dtype_code(x, "x"), code, ptr(src), ld, ptr(weight), ptr(bias), rows,
+                                  x.shape[-1], eps, ptr(y), x.shape[-1], ptr(stats), stream_of(x))
+    if rc:
+        raise RuntimeError(f"vsn_layernorm failed ({rc})")
+    return y, stats
+
+
+def layer_norm_backward(dy, x, stats, weight=None, bias=None):
+    """Gradients (dx, dweight, dbias) of layer_norm at `x`, with the `stats` it returned, from dy = dL/dy.
+
+    dweight / dbias have the parameters' type and are None where the parameter is.  Sums run in a fixed order."""
+    code = _check(x, weight, bias)
+    no_graph(dy, x, weight, bias)
+    on_device(dy, "dy", x.device)
+    on_device(stats, "stats", x.device)
+    if dy.shape != x.shape or dy.dtype != x.dtype:
+        raise ValueError("dy: x's shape and type expected")
+    width = x.shape[-1]
+    src, rows, ld = _rows(x, "x")
+    if stats.shape != (rows, 2) or stats.dtype != torch.float32 or not stats.is_contiguous():
+        raise ValueError(f"stats: contiguous float32 [{rows}, 2] expected")
+    grad, _, ldg = _rows(dy, "dy")
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dw = torch.empty_like(weight) if weight is not None else None
+    db = torch.empty_like(bias) if bias is not None else None
+    lib = capi.lib()
+    size = lib.vsn_layernorm_workspace(rows, width) if weight is not None or bias is not None else 0
+    work = torch.empty(size // 4, dtype=torch.float32, device=x.device) if size else None
+    rc = lib.vsn_layernorm_backward(x.device.index, dtype_code(x, "x"), code, ptr(grad), ldg, ptr(src), ld, ptr(stats),
+                                    ptr(weight), rows, width, ptr(dx), width, ptr(dw), ptr(db), ptr(work), size,
+                                    stream_of(x))
+    if rc:
+        raise RuntimeError(f"vsn_layernorm_backward failed ({rc})")
+    return dx, dw, db

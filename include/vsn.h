@@ -290,6 +290,28 @@ int vsn_hopt_run(vsn_hopt_handle p, float* dev_frag_pos, void* stream);
  * host_loss_first_last f64[2] (either may be NULL) */
 int vsn_hopt_stats(vsn_hopt_handle p, int32_t* host_iters_evals, double* host_loss_first_last, void* stream);
 
+/* ---- layer operators: what a layer over the rows of a fragment batch is trained and evaluated with ----
+ * Element types of the row arrays; positions, slopes, tables and statistics are float32 throughout. */
+enum { VSN_F32 = 0, VSN_BF16 = 1, VSN_F16 = 2 };
+
+/* Layer norm over the last axis (torch.nn.LayerNorm of the ViS-MP layer, ViSNet/model/visnet_block.py:180,237), as an
+ * operator: y = (x - mean) / sqrt(var + eps) * w + b for `rows` rows of `width` (1 ... 4096) elements.
+ *   ldx, ldy   elements from one row to the next (>= width; any value, no alignment beyond the element's)
+ *   dev_w, dev_b   [width] of `param_dtype` (the rows' dtype, or VSN_F32), or NULL = 1 and 0
+ *   dev_stats  f32 [rows][2] = {mean, 1 / sqrt(var + eps)}: what the backward pass needs; NULL = not wanted
+ * Sums are float32; asynchronous on `stream`; dev_y may be dev_x (same ld), other overlaps are not allowed. */
+int vsn_layernorm(int device_id, int dtype, int param_dtype, const void* dev_x, int64_t ldx, const void* dev_w,
+                  const void* dev_b, int64_t rows, int width, float eps, void* dev_y, int64_t ldy, float* dev_stats,
+                  void* stream);
+/* Its gradients: dx (may be dev_dy, same ld), dw = sum_rows dy h, db = sum_rows dy (param_dtype, overwritten; either may
+ * be NULL).  `dev_workspace` of vsn_layernorm_workspace() bytes belongs to the call until the stream has passed it.
+ * Fixed summation order: equal inputs give equal bits. */
+int64_t vsn_layernorm_workspace(int64_t rows, int width);
+int vsn_layernorm_backward(int device_id, int dtype, int param_dtype, const void* dev_dy, int64_t lddy,
+                           const void* dev_x, int64_t ldx, const float* dev_stats, const void* dev_w, int64_t rows,
+                           int width, void* dev_dx, int64_t lddx, void* dev_dw, void* dev_db, void* dev_workspace,
+                           int64_t workspace_bytes, void* stream);
+
 /* ---- work partitions (Calculators/device_strategy.py:84-127) ---- */
 /* Writes up to max_out triples (device_idx, frag_begin, frag_end); returns count. */
 int vsn_partition(const int64_t* host_start, const int64_t* host_end, int64_t B, int n_devices,
