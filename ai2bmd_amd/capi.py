@@ -49,6 +49,27 @@ class VsnHoptTerms(C.Structure):
     ]
 
 
+class VsnAttnIO(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("scale", C.c_float), ("rows_q", C.c_int64), ("rows_k", C.c_int64),
+        ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p),
+        ("q_row", C.c_int64), ("q_head", C.c_int64), ("k_row", C.c_int64), ("k_head", C.c_int64),
+        ("v_row", C.c_int64), ("v_head", C.c_int64),
+        ("q_pos", C.c_void_p), ("k_pos", C.c_void_p), ("slope", C.c_void_p),
+        ("q_res", C.c_void_p), ("k_res", C.c_void_p), ("table", C.c_void_p),
+        ("out", C.c_void_p), ("out_row", C.c_int64), ("out_head", C.c_int64),
+        ("stats", C.c_void_p),
+    ]
+
+
+class VsnAttnGrads(C.Structure):
+    _fields_ = [
+        ("dout", C.c_void_p), ("dout_row", C.c_int64), ("dout_head", C.c_int64),
+        ("dq", C.c_void_p), ("dk", C.c_void_p), ("dv", C.c_void_p),
+        ("dpos", C.c_void_p), ("dquery_pos", C.c_void_p), ("dslope", C.c_void_p), ("dtable", C.c_void_p),
+    ]
+
+
 VECNORM = {"none": 0, "rms": 1, "max_min": 2}
 RBF = {"expnorm": 0, "gauss": 1}
 ACTIVATION = {"silu": 0, "swish": 0, "ssp": 1, "tanh": 2, "sigmoid": 3}  # utils.py:93-116 act_class_mapping
@@ -188,6 +209,17 @@ def lib() -> C.CDLL:
     L.vsn_layernorm_workspace.restype = i64
     L.vsn_layernorm_backward.argtypes = [i32, i32, i32, vp, i64, vp, i64, vp, vp, i64, i32, vp, i64, vp, vp, vp, i64, vp]
     L.vsn_layernorm_backward.restype = i32
+    i32p = C.POINTER(C.c_int32)
+    L.vsn_attn_create.argtypes = [C.POINTER(vp), i32, i64, i64p, i64p, i64p, i64p, i32, i32, i32, i32, i32p, i32]
+    L.vsn_attn_create.restype = i32
+    L.vsn_attn_destroy.argtypes = [vp]
+    L.vsn_attn_destroy.restype = None
+    L.vsn_attn_workspace.argtypes = [vp, i64, i64, i32]
+    L.vsn_attn_workspace.restype = i64
+    L.vsn_attn_forward.argtypes = [vp, C.POINTER(VsnAttnIO), vp, i64, vp]
+    L.vsn_attn_forward.restype = i32
+    L.vsn_attn_backward.argtypes = [vp, C.POINTER(VsnAttnIO), C.POINTER(VsnAttnGrads), vp, i64, vp]
+    L.vsn_attn_backward.restype = i32
     _lib = L
     return L
 
@@ -205,4 +237,5 @@ EXPORTS = [
     "vsn_build_fragments", "vsn_md_create", "vsn_md_destroy", "vsn_md_half1", "vsn_md_half2", "vsn_md_set_noise", "vsn_md_half1_build", "vsn_md_half1_build_relax", "vsn_md_combine_half2", "vsn_md_set_restraints", "vsn_md_restrain", "vsn_md_observe", "vsn_mm_create", "vsn_mm_destroy", "vsn_mm_forces",
     "vsn_hopt_create", "vsn_hopt_destroy", "vsn_hopt_run", "vsn_hopt_stats",
     "vsn_layernorm", "vsn_layernorm_workspace", "vsn_layernorm_backward",
+    "vsn_attn_create", "vsn_attn_destroy", "vsn_attn_workspace", "vsn_attn_forward", "vsn_attn_backward",
 ]

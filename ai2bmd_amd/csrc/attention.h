@@ -1,0 +1,250 @@
+// Fragment attention: what the forward and the backward kernels share.
+//
+// For a query row i and a key row j of one fragment, head a (key head a / group):
+//   s_ij = scale q_i.k_j - slope_a |x_i - x_j| + table[a][bucket(res_j - res_i)],   P = softmax_j(s),   o_i = sum_j P_ij v_j
+//
+// A wave works on tiles of 32 x 32 scores in the registers of one 32x32 MFMA accumulator: lane = column (lane & 31), the
+// 16 registers = rows acc_row(r).  The tile is computed with the rows' operand from LDS and the columns' operand from
+// registers, so everything that belongs to a column (running maximum and sum, position, residue, gradient scale) is the
+// lane's own, and a column of P or dS is already the B operand of the next product: that product contracts over the
+// tile's rows, whose order inside a contraction is free, and takes its A operand in the same order (load_t).
+// Float32 runs the same tiles on the float32 matrix instruction (8 of 2 rows instead of one of 16).
+#pragma once
+#include "typed.h"
+
+namespace vsn {
+
+constexpr float kLog2e = 1.44269504088896341f;
+constexpr int kTile = 32;         // rows and columns of a tile
+constexpr int kCoopWaves = 4;     // waves that share the tiles of one workgroup (128 columns of one head)
+constexpr int kMaxReach = 1023;   // clipped residue difference: 2 reach + 1 table entries in LDS
+
+// One block of columns (queries in the forward and dq passes, keys in the dk / dv pass) against a run of rows.
+struct AttnWork {
+  int col0, cols;  // first column row, number of columns (<= 32, or <= 128 where the workgroup shares tiles)
+  int row0, row1;  // the rows it meets
+  int slot;        // >= 0: partial result of a split run of keys, joined afterwards
+};
+// Partial results to join: `cols` query rows from col0, slots slot0 ... slot0 + slots - 1
+struct AttnJoin {
+  int col0, cols, slot0, slots;
+};
+
+struct AttnParams {
+  const AttnWork* work;
+  int count;              // work items
+  int workers, part0;     // backward: workers per head of this launch, first partial sum of this launch
+  int parts;              // partial sums per head over all launches
+  int heads, kv_heads, dim;
+  int reach, n_rel, n_buckets;
+  const int* lut;         // [n_rel] bucket of a clipped difference
+  const void *q, *k, *v, *dout;
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head, do_row, do_head;
+  const float *q_pos, *k_pos, *slope;
+  const int *q_res, *k_res;
+  const float* table;     // [heads][n_buckets]
+  float scale;
+  int64_t rows_q, rows_k; // rows of the arrays (statistics and partial sums are laid out by them)
+  void* out;
+  int64_t out_row, out_head;
+  float2* stats;          // [heads][rows_q] {maximum, sum of exponentials}
+  float* part_o;          // split keys: [slot][heads][32][dim] unnormalised output
+  float2* part_ml;        // [slot][heads][32]
+  const AttnJoin* join;
+  // backward
+  float* delta;           // [heads][rows_q]
+  void *dq, *dk, *dv;     // contiguous
+  float* part_pos_q;      // [heads][rows_q][3] or null
+  float* part_pos_k;      // [kv_heads][rows_k][3] or null
+  float* part_slope;      // [heads][4 parts] or null
+  float* part_hist;       // [heads][n_rel][parts] or null
+  float *dpos, *dq_pos, *dslope, *dtable;
+  int64_t used_q, used_k; // rows that belong to fragments
+};
+
+template <typename T>
+struct Mma;
+template <>
+struct Mma<__bf16> {
+  static __device__ __forceinline__ f32x16 run(bf16x8 a, bf16x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+};
+template <>
+struct Mma<_Float16> {
+  static __device__ __forceinline__ f32x16 run(f16x8 a, f16x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+};
+template <>
+struct Mma<float> {
+  static __device__ __forceinline__ f32x16 run(f32x8 a, f32x8 b, f32x16 c) {
+#pragma unroll
+    for (int t = 0; t < 8; ++t) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[t], b[t], c, 0, 0, 0);
+    return c;
+  }
+};
+
+// row of accumulator register r in the lane's half
+__device__ __forceinline__ int acc_row(int r, int hi) { return 8 * (r >> 2) + 4 * hi + (r & 3); }
+
+__device__ __forceinline__ f32x16 acc_zero() {
+  f32x16 z;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) z[r] = 0.f;
+  return z;
+}
+
+template <typename T, int DP>
+struct TileShape {
+  static constexpr int LD = DP + 16 / (int)sizeof(T);            // 16 bytes of padding per row: 16-byte reads of 8 rows
+                                                                 // in a row fall on different banks
+  static constexpr int EPC = 16 / (int)sizeof(T);                // elements per 16-byte chunk
+  static constexpr int CPR = DP / EPC;                           // chunks per row
+  static constexpr int CHUNKS = kTile * CPR;                     // chunks per tile
+  static constexpr size_t BYTES = sizeof(T) * kTile * LD;
+};
+
+// Copies two tiles (32 rows of two arrays) into LDS by way of registers, so the loads of the next tiles can be in flight
+// while the present ones are computed with.  Rows and columns beyond the end are zeros.
+template <typename T, int DP, int THREADS>
+struct TilePair {
+  typedef TileShape<T, DP> S;
+  static constexpr int N = (2 * S::CHUNKS + THREADS - 1) / THREADS;
+  uint4 reg[N];
+  __device__ __forceinline__ void load(const T* a, int64_t a_row, const T* b, int64_t b_row, int rows, int dim, int tid) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int c = tid + i * THREADS;
+      const bool second = c >= S::CHUNKS;
+      const int rest = second ? c - S::CHUNKS : c;
+      const int row = rest / S::CPR, at = rest % S::CPR * S::EPC;
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (row < rows && at < dim && c < 2 * S::CHUNKS)
+        v = *(const uint4*)((second ? b + row * b_row : a + row * a_row) + at);
+      reg[i] = v;
+    }
+  }
+  __device__ __forceinline__ void store(T* a, T* b, int tid) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int c = tid + i * THREADS;
+      if (c < 2 * S::CHUNKS) {
+        const int rest = c >= S::CHUNKS ? c - S::CHUNKS : c;
+        *(uint4*)((c >= S::CHUNKS ? b : a) + rest / S::CPR * S::LD + rest % S::CPR * S::EPC) = reg[i];
+      }
+    }
+  }
+};
+
+// Orders LDS writes of some lanes before reads of others: a barrier where the workgroup shares the tiles, and an order
+// for the compiler where they are the wave's own (a wave's LDS accesses are carried out in program order).
+template <bool COOP>
+__device__ __forceinline__ void tile_sync() {
+  if constexpr (COOP) {
+    __syncthreads();
+  } else {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  }
+}
+
+// A operand "row of the tile": lane's row (lane & 31), elements c 16 + hi 8 ... + 7
+template <typename T, int DP>
+__device__ __forceinline__ typename vec8<T>::type load_n(const T* tile, int c, int col, int hi) {
+  return *(const typename vec8<T>::type*)(tile + col * TileShape<T, DP>::LD + c * 16 + hi * 8);
+}
+
+// A operand "column of the tile": lane's column d0 + (lane & 31), rows acc_row(8 c + 0 ... 7) - the order in which a lane
+// holds its scores.  16-bit types: two transposing LDS reads of 4 rows x 16 columns per 16 lanes (lane 4 e + j / 4 of a
+// group supplies row e, four columns from 4 (j & 3); lane j receives column j).
+template <typename T, int DP>
+__device__ __forceinline__ typename vec8<T>::type load_t(const T* tile, int c, int d0, int lane, int hi) {
+  typename vec8<T>::type f;
+  constexpr int LD = TileShape<T, DP>::LD;
+  if constexpr (sizeof(T) == 4) {
+    const float* p = tile + d0 + (lane & 31);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = p[acc_row(8 * c + i, hi) * LD];
+  } else {
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+    const int j = lane & 15;
+    const T* p = tile + (16 * c + 4 * hi + (j >> 2)) * LD + d0 + (lane & 16) + 4 * (j & 3);
+    s16x4 part[2];
+    part[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
+    part[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 8 * LD));
+    __builtin_memcpy(&f, part, 16);
+  }
+  return f;
+}
+
+// eight elements of a global row as a B operand (column operand), zeros beyond the end
+template <typename T>
+__device__ __forceinline__ typename vec8<T>::type load_col(const T* row, int at, int dim, bool live) {
+  typename vec8<T>::type f;
+  if (live && at < dim) {
+    f = *(const typename vec8<T>::type*)(row + at);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = (T)0.f;
+  }
+  return f;
+}
+
+template <typename T>
+__device__ __forceinline__ typename vec8<T>::type pack8(const float* p) {
+  typename vec8<T>::type f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = (T)p[i];
+  return f;
+}
+
+// four consecutive elements of an output row
+template <typename T>
+__device__ __forceinline__ void store4(T* p, float a, float b, float c, float d) {
+  T v[4] = {(T)a, (T)b, (T)c, (T)d};
+  if constexpr (sizeof(T) == 4)
+    *(float4*)p = *(float4*)v;
+  else
+    *(uint2*)p = *(uint2*)v;
+}
+
+// |a - b| from the difference's components, and its reciprocal; 0 and a huge finite number where the points coincide
+// (the difference itself is 0 there, so the direction is 0).  One reciprocal root instead of a root and a division.
+__device__ __forceinline__ float pair_dist(float dx, float dy, float dz, float& inv) {
+  const float d2 = dx * dx + dy * dy + dz * dz;
+  inv = __builtin_amdgcn_rsqf(__builtin_amdgcn_fmed3f(d2, 1e-37f, 3e38f));
+  return d2 * inv;
+}
+
+// index of the clipped difference of two residue numbers; the difference saturates
+__device__ __forceinline__ int rel_index(int key_res, int query_res, int reach) {
+  const int d = __builtin_elementwise_sub_sat(key_res, query_res);
+  return (d < -reach ? -reach : d > reach ? reach : d) + reach;
+}
+
+__device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, 64); }
+
+// wave-private (or shared) LDS of one work item
+template <typename T, int DP>
+struct AttnLds {
+  static constexpr size_t TILES = 2 * TileShape<T, DP>::BYTES;
+  static constexpr size_t META = kTile * (sizeof(float4) * 2 + sizeof(int));  // positions, statistics, residues
+  T *a, *b;
+  float4 *pos, *stat;
+  int* res;
+  float* tab;  // [n_rel] this head's table, expanded
+  __device__ __forceinline__ explicit AttnLds(char* p) {
+    a = (T*)p;
+    b = (T*)(p + TileShape<T, DP>::BYTES);
+    pos = (float4*)(p + TILES);
+    stat = pos + kTile;
+    res = (int*)(stat + kTile);
+    tab = (float*)(res + kTile);
+  }
+  static size_t bytes(int n_rel) { return (TILES + META + sizeof(float) * n_rel + 15) & ~(size_t)15; }
+};
+
+}  // namespace vsn

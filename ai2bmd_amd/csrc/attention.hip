@@ -1,0 +1,320 @@
+// Fragment attention: the plan (work lists of both passes, made once per fragment layout) and the entry points.
+#include <algorithm>
+#include <vector>
+
+#include "attention.h"
+#include "attention_host.h"
+
+struct vsn_attn {
+  struct Side {
+    vsn::AttnWork *lone_work = nullptr, *coop_work = nullptr;
+    vsn::AttnJoin* join = nullptr;
+    int lone = 0, coop = 0, joins = 0, slots = 0;
+    vsn::AttnPlanView view() const { return {lone_work, coop_work, lone, coop, join, joins}; }
+  };
+  int device = 0, heads = 0, kv_heads = 0, dim = 0, reach = 0, n_rel = 0, n_buckets = 0;
+  int64_t used_q = 0, used_k = 0;
+  Side fwd, by_query, by_key;
+  int* lut = nullptr;
+};
+
+namespace vsn {
+namespace {
+
+// A workgroup of four waves reads each tile of rows once for 128 columns, a lone wave once for 32.  Sharing pays where
+// there are workgroups enough for every compute unit; with fewer, 32 columns per wave spread over four times as many
+// compute units.
+constexpr int kCoopCols = kTile * kCoopWaves;
+constexpr int64_t kCoopMin = 256;
+// A run of keys is split where the items alone leave most of the 1024 SIMDs without a wave and a piece still keeps
+// enough tiles to be worth joining.
+constexpr int64_t kSplitBelow = 1024, kSplitWaves = 2048;
+constexpr int kSplitTiles = 16;
+
+struct Lists {
+  std::vector<AttnWork> lone, coop;
+  std::vector<AttnJoin> join;
+  int slots = 0;
+};
+
+Lists make_lists(int64_t n, const int64_t* col_start, const int64_t* col_end, const int64_t* row_start,
+                 const int64_t* row_end, int heads, bool split) {
+  Lists out;
+  int64_t groups = 0;
+  for (int64_t f = 0; f < n; ++f) {
+    const int64_t cols = col_end[f] - col_start[f];
+    if (cols > 2 * kTile) groups += (cols + kCoopCols - 1) / kCoopCols * heads;
+  }
+  const bool share = groups >= kCoopMin;
+  int64_t tiles = 0;
+  for (int64_t f = 0; f < n; ++f) {
+    const int64_t cols = col_end[f] - col_start[f], rows = row_end[f] - row_start[f];
+    const bool coop = share && cols > 2 * kTile;
+    const int64_t step = coop ? kCoopCols : kTile;
+    for (int64_t c = 0; c < cols; c += step) {
+      AttnWork w = {};
+      w.col0 = (int)(col_start[f] + c);
+      w.cols = (int)std::min<int64_t>(step, cols - c);
+      w.row0 = (int)row_start[f];
+      w.row1 = (int)row_end[f];
+      w.slot = -1;
+      (coop ? out.coop : out.lone).push_back(w);
+      if (!coop) tiles += (rows + kTile - 1) / kTile;
+    }
+  }
+  const int64_t waves = (int64_t)out.lone.size() * heads;
+  if (split && waves && waves < kSplitBelow && out.coop.empty()) {
+    std::vector<AttnWork> pieces;
+    for (const AttnWork& w : out.lone) {
+      const int64_t have = ((int64_t)w.row1 - w.row0 + kTile - 1) / kTile;
+      const int64_t per = std::max<int64_t>({2, (tiles * heads + kSplitWaves - 1) / kSplitWaves,
+                                             (have + kMaxSlots - 1) / kMaxSlots});
+      const int64_t parts = (have + per - 1) / per;
+      if (have < kSplitTiles || parts < 2) {
+        pieces.push_back(w);
+        continue;
+      }
+      out.join.push_back({w.col0, w.cols, out.slots, (int)parts});
+      for (int64_t i = 0; i < parts; ++i) {
+        AttnWork piece = w;
+        piece.row0 = (int)(w.row0 + i * per * kTile);
+        piece.row1 = (int)std::min<int64_t>(w.row1, w.row0 + (i + 1) * per * kTile);
+        piece.slot = out.slots++;
+        pieces.push_back(piece);
+      }
+    }
+    out.lone.swap(pieces);
+  }
+  return out;
+}
+
+template <typename E>
+bool upload(const std::vector<E>& v, E** dev) {
+  if (v.empty()) return true;
+  return hipMalloc((void**)dev, v.size() * sizeof(E)) == hipSuccess &&
+         hipMemcpy(*dev, v.data(), v.size() * sizeof(E), hipMemcpyHostToDevice) == hipSuccess;
+}
+
+bool upload_side(const Lists& l, vsn_attn::Side& s) {
+  s.lone = (int)l.lone.size(), s.coop = (int)l.coop.size(), s.joins = (int)l.join.size(), s.slots = l.slots;
+  return upload(l.lone, &s.lone_work) && upload(l.coop, &s.coop_work) && upload(l.join, &s.join);
+}
+
+void free_side(vsn_attn::Side& s) {
+  hipFree(s.lone_work);
+  hipFree(s.coop_work);
+  hipFree(s.join);
+}
+
+bool ranges_ok(int64_t n, const int64_t* start, const int64_t* end) {
+  if (!start || !end) return false;
+  for (int64_t f = 0; f < n; ++f)
+    if (end[f] < start[f] || start[f] != (f ? end[f - 1] : 0)) return false;
+  return end[n - 1] <= (int64_t)1 << 30;
+}
+
+// Workers per head of the dq pass: each adds up the slope's and the table's gradient over its items and leaves one
+// partial sum, so their number is bounded, and more tightly where a partial sum is a large table.
+int workers(int items, int heads, int n_rel, int most) {
+  int64_t cap = std::max(1, most / heads);
+  if (n_rel) cap = std::min<int64_t>(cap, std::max<int64_t>(32, ((int64_t)1 << 24) / ((int64_t)n_rel * heads)));
+  return (int)std::min<int64_t>(items, cap);
+}
+
+struct Workspace {
+  int64_t size = 0;
+  int64_t take(int64_t bytes) {
+    const int64_t at = size;
+    size += (bytes + 255) & ~(int64_t)255;
+    return at;
+  }
+};
+
+struct BackwardSpace {
+  int64_t delta, pos_q, pos_k, slope, hist, size;
+  int lone, coop, parts;
+};
+
+BackwardSpace backward_space(const vsn_attn& a, int64_t rows_q, int64_t rows_k) {
+  BackwardSpace s;
+  s.lone = workers(a.by_query.lone, a.heads, a.n_rel, 8192);
+  s.coop = workers(a.by_query.coop, a.heads, a.n_rel, 2048);
+  s.parts = s.lone + s.coop;
+  Workspace w;
+  s.delta = w.take(rows_q * a.heads * 4);
+  s.pos_q = w.take(rows_q * a.heads * 12);
+  s.pos_k = w.take(rows_k * a.kv_heads * 12);
+  s.slope = w.take((int64_t)s.parts * a.heads * kCoopWaves * 4);
+  s.hist = w.take((int64_t)s.parts * a.heads * a.n_rel * 4);
+  s.size = w.size;
+  return s;
+}
+
+int64_t forward_space(const vsn_attn& a, int64_t* ml) {
+  Workspace w;
+  const int64_t rows = (int64_t)a.fwd.slots * a.heads * kTile;
+  w.take(rows * a.dim * 4);
+  const int64_t at = w.take(rows * 8);
+  if (ml) *ml = at;
+  return w.size;
+}
+
+bool lines_up(const void* p, int64_t row, int64_t head, int heads, int dim, int size) {
+  const int64_t step = 16 / size;
+  return p && (uintptr_t)p % 16 == 0 && row % step == 0 && head % step == 0 && row >= 0 && head >= 0 &&
+         (heads == 1 || head >= dim);
+}
+
+// rows and heads of an output that do not run into one another
+bool apart(int64_t rows, int64_t row, int heads, int64_t head, int dim) {
+  if (rows > 1 && row < dim) return false;
+  if (heads > 1 && head < dim) return false;
+  return rows <= 1 || heads <= 1 || row >= (heads - 1) * head + dim || head >= (rows - 1) * row + dim;
+}
+
+bool io_ok(const vsn_attn& a, const vsn_attn_io& io) {
+  if (io.dtype < VSN_F32 || io.dtype > VSN_F16) return false;
+  const int size = io.dtype == VSN_F32 ? 4 : 2;
+  if (io.rows_q < a.used_q || io.rows_k < a.used_k || io.rows_q > (int64_t)1 << 30 || io.rows_k > (int64_t)1 << 30)
+    return false;
+  if (a.used_q && !lines_up(io.q, io.q_row, io.q_head, a.heads, a.dim, size)) return false;
+  if (a.used_k && (!lines_up(io.k, io.k_row, io.k_head, a.kv_heads, a.dim, size) ||
+                   !lines_up(io.v, io.v_row, io.v_head, a.kv_heads, a.dim, size)))
+    return false;
+  if (io.slope && ((a.used_q && !io.q_pos) || (a.used_k && !io.k_pos))) return false;
+  if (io.table && (!a.n_rel || (a.used_q && !io.q_res) || (a.used_k && !io.k_res))) return false;
+  return true;
+}
+
+AttnParams params(const vsn_attn& a, const vsn_attn_io& io) {
+  AttnParams p = {};
+  p.heads = a.heads, p.kv_heads = a.kv_heads, p.dim = a.dim;
+  p.reach = a.reach, p.n_rel = a.n_rel, p.n_buckets = a.n_buckets, p.lut = a.lut;
+  p.q = io.q, p.k = io.k, p.v = io.v;
+  p.q_row = io.q_row, p.q_head = io.q_head, p.k_row = io.k_row, p.k_head = io.k_head, p.v_row = io.v_row,
+  p.v_head = io.v_head;
+  p.q_pos = io.q_pos, p.k_pos = io.k_pos, p.slope = io.slope;
+  p.q_res = io.q_res, p.k_res = io.k_res, p.table = io.table;
+  p.scale = io.scale;
+  p.rows_q = io.rows_q, p.rows_k = io.rows_k;
+  p.out = io.out, p.out_row = io.out_row, p.out_head = io.out_head;
+  p.stats = (float2*)io.stats;
+  p.used_q = a.used_q, p.used_k = a.used_k;
+  return p;
+}
+
+}  // namespace
+}  // namespace vsn
+
+extern "C" int vsn_attn_create(vsn_attn_handle* out, int device_id, int64_t n, const int64_t* host_start,
+                               const int64_t* host_end, const int64_t* host_query_start, const int64_t* host_query_end,
+                               int heads, int kv_heads, int head_dim, int reach, const int32_t* host_buckets,
+                               int n_buckets) {
+  using namespace vsn;
+  if (!out) return -22;
+  *out = nullptr;
+  if (n <= 0 || n > (int64_t)1 << 30 || !ranges_ok(n, host_start, host_end)) return -22;
+  if ((host_query_start != nullptr) != (host_query_end != nullptr)) return -22;
+  if (host_query_start && !ranges_ok(n, host_query_start, host_query_end)) return -22;
+  if (heads < 1 || heads > 1024 || kv_heads < 1 || heads % kv_heads || head_dim < 8 || head_dim > 128 || head_dim % 8)
+    return -22;
+  if (n_buckets < 0 || (n_buckets && !host_buckets) || reach < 0 || reach > kMaxReach) return -22;
+  if (n_buckets > 4096) return -22;
+  if (n_buckets)
+    for (int i = 0; i < 2 * reach + 1; ++i)
+      if (host_buckets[i] < 0 || host_buckets[i] >= n_buckets) return -22;
+  DeviceScope scope(device_id);
+  if (!scope.ok) return -19;
+  const int64_t* qs = host_query_start ? host_query_start : host_start;
+  const int64_t* qe = host_query_start ? host_query_end : host_end;
+  vsn_attn* a = nullptr;
+  bool ok = false;
+  try {
+    a = new vsn_attn();
+    a->device = device_id, a->heads = heads, a->kv_heads = kv_heads, a->dim = head_dim;
+    a->used_q = qe[n - 1], a->used_k = host_end[n - 1];
+    std::vector<int> lut;
+    if (n_buckets) {
+      a->reach = reach, a->n_rel = 2 * reach + 1, a->n_buckets = n_buckets;
+      lut.assign(host_buckets, host_buckets + a->n_rel);
+    }
+    ok = upload_side(make_lists(n, qs, qe, host_start, host_end, heads, true), a->fwd) &&
+         upload_side(make_lists(n, qs, qe, host_start, host_end, heads, false), a->by_query) &&
+         upload_side(make_lists(n, host_start, host_end, qs, qe, kv_heads, false), a->by_key) &&
+         upload(lut, &a->lut);
+  } catch (...) {  // out of host memory
+    ok = false;
+  }
+  if (!ok) {
+    vsn_attn_destroy(a);
+    return -12;
+  }
+  *out = a;
+  return 0;
+}
+
+extern "C" void vsn_attn_destroy(vsn_attn_handle a) {
+  if (!a) return;
+  vsn::DeviceScope scope(a->device);
+  vsn::free_side(a->fwd);
+  vsn::free_side(a->by_query);
+  vsn::free_side(a->by_key);
+  hipFree(a->lut);
+  delete a;
+}
+
+extern "C" int64_t vsn_attn_workspace(vsn_attn_handle a, int64_t rows_q, int64_t rows_k, int backward) {
+  if (!a || rows_q < a->used_q || rows_k < a->used_k) return -22;
+  return backward ? vsn::backward_space(*a, rows_q, rows_k).size : vsn::forward_space(*a, nullptr);
+}
+
+extern "C" int vsn_attn_forward(vsn_attn_handle a, const vsn_attn_io* io, void* dev_workspace, int64_t workspace_bytes,
+                                void* stream) {
+  using namespace vsn;
+  if (!a || !io || !io_ok(*a, *io)) return -22;
+  if (a->used_q && (!lines_up(io->out, io->out_row, io->out_head, a->heads, a->dim, io->dtype == VSN_F32 ? 4 : 2) ||
+                    !apart(io->rows_q, io->out_row, a->heads, io->out_head, a->dim)))
+    return -22;
+  int64_t ml = 0;
+  const int64_t need = forward_space(*a, &ml);
+  if (need && (!dev_workspace || (uintptr_t)dev_workspace % 16 || workspace_bytes < need)) return -22;
+  DeviceScope scope(a->device);
+  if (!scope.ok) return -19;
+  AttnParams p = params(*a, *io);
+  p.part_o = (float*)dev_workspace;
+  p.part_ml = (float2*)((char*)dev_workspace + ml);
+  return attn_forward(io->dtype, a->fwd.view(), p, (hipStream_t)stream);
+}
+
+extern "C" int vsn_attn_backward(vsn_attn_handle a, const vsn_attn_io* io, const vsn_attn_grads* g,
+                                 void* dev_workspace, int64_t workspace_bytes, void* stream) {
+  using namespace vsn;
+  if (!a || !io || !g || !io_ok(*a, *io)) return -22;
+  const int size = io->dtype == VSN_F32 ? 4 : 2;
+  if (a->used_q && (!io->stats || !lines_up(g->dout, g->dout_row, g->dout_head, a->heads, a->dim, size) || !g->dq))
+    return -22;
+  if (a->used_k && (!g->dk || !g->dv)) return -22;
+  if ((uintptr_t)g->dq % 16 || (uintptr_t)g->dk % 16 || (uintptr_t)g->dv % 16) return -22;
+  if ((g->dpos || g->dquery_pos || g->dslope) && !io->slope) return -22;
+  if (g->dquery_pos && !g->dpos) return -22;
+  if (g->dpos && !g->dquery_pos && (a->used_q != a->used_k || io->rows_q != io->rows_k)) return -22;
+  if (g->dtable && !io->table) return -22;
+  const BackwardSpace s = backward_space(*a, io->rows_q, io->rows_k);
+  if (s.size && (!dev_workspace || (uintptr_t)dev_workspace % 16 || workspace_bytes < s.size)) return -22;
+  DeviceScope scope(a->device);
+  if (!scope.ok) return -19;
+  char* base = (char*)dev_workspace;
+  AttnParams p = params(*a, *io);
+  p.dout = g->dout, p.do_row = g->dout_row, p.do_head = g->dout_head;
+  p.delta = (float*)(base + s.delta);
+  p.dq = g->dq, p.dk = g->dk, p.dv = g->dv;
+  p.parts = s.parts;
+  if (g->dpos) {
+    p.part_pos_q = (float*)(base + s.pos_q);
+    p.part_pos_k = (float*)(base + s.pos_k);
+  }
+  if (g->dslope) p.part_slope = (float*)(base + s.slope);
+  if (g->dtable) p.part_hist = (float*)(base + s.hist);
+  p.dpos = g->dpos, p.dq_pos = g->dquery_pos, p.dslope = g->dslope, p.dtable = g->dtable;
+  return attn_backward(io->dtype, a->by_query.view(), a->by_key.view(), p, s.lone, s.coop, (hipStream_t)stream);
+}

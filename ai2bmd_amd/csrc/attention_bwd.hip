@@ -1,0 +1,524 @@
+// Fragment attention, backward (attention.h has the tile; formulas of the forward pass there).
+//
+//   P = exp(s - m) / l,  dP_ij = do_i.v_j,  D_i = sum_j P_ij dP_ij,  dS = P (dP - D)
+//   dq_i = scale sum_j dS k_j      dk_j = scale sum_i dS q_i      dv_j = sum_i P do_i
+//   dslope_a = - sum dS r          dtable[a][b] = sum over the pairs of bucket b
+//   dx_i -= slope dS (x_i - x_j) / r,  dx_j -= the opposite; summed over heads
+//
+// Two passes that both recompute the scores, each with its sums in registers and nothing to add atomically: queries in
+// lanes for dq, D, the slopes, the table and the queries' share of the positions; keys in lanes for dk, dv and the keys'
+// share.  Seven products instead of five, against a pass that would have to add dq (or dk, dv) across workgroups in an
+// order of its own.  The maximum and the sum are kept apart (not as one logarithm), so P keeps its precision however
+// large the scores are.  D is summed from the scores before anything is rounded (do_i.o_i would carry the rounding of P
+// in the forward product into every float32 gradient): a walk over the keys of its own ahead of the dq pass, except where
+// one tile holds all keys of a fragment, as it does for most fragments, and everything is still in registers.
+// P and dS are rounded to the rows' type where they enter a product.  float16 has few exponents for that: P goes in
+// times 2^14, and dS times a power of two per column that follows the largest one seen so far.
+// All sums are in a fixed order; the table's are kept per wave in LDS.
+#include "attention.h"
+#include "attention_host.h"
+
+namespace vsn {
+
+// a column's power of two for float16 gradients: keeps max |dS| scale below 2^15
+struct ColumnScale {
+  float f = 0x1p100f;
+  // the factor by which what was summed so far has to be multiplied, 1 where the scale stays
+  __device__ __forceinline__ float follow(float largest) {
+    if (largest * f <= 0x1p15f || !(largest < INFINITY)) return 1.f;
+    const float next = ldexpf(1.f, 14 - ilogbf(largest));
+    const float change = next / f;
+    f = next;
+    return change;
+  }
+};
+
+template <typename T, int DP, bool COOP>
+__global__ __launch_bounds__(256) void k_attn_bwd_q(AttnParams p, size_t lds_per_wave) {
+  extern __shared__ __attribute__((aligned(16))) char lds_raw[];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int col = lane & 31, hi = lane >> 5;
+  const int tid = COOP ? threadIdx.x : lane;
+  constexpr int THREADS = COOP ? 64 * kCoopWaves : 64;
+  constexpr bool HALF = sizeof(T) == 2 && !__is_same(T, __bf16);
+  const int64_t id = COOP ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * (blockDim.x >> 6) + wave;
+  if (id >= (int64_t)p.workers * p.heads) return;
+  const int head = (int)(id % p.heads), worker = (int)(id / p.heads);
+  char* base = lds_raw + (COOP ? 0 : wave * lds_per_wave);
+  const AttnLds<T, DP> lds(base);
+  float* hist_all = lds.tab + p.n_rel;  // one histogram per wave
+  float* hist = hist_all + (COOP ? wave * p.n_rel : 0);
+  const bool count = p.part_hist != nullptr;
+
+  const int kv = head / (p.heads / p.kv_heads);
+  const T* kp = (const T*)p.k + kv * p.k_head;
+  const T* vp = (const T*)p.v + kv * p.v_head;
+  const float slope = p.slope ? p.slope[head] : 0.f;
+  if (p.table)
+    for (int i = tid; i < p.n_rel; i += THREADS) lds.tab[i] = p.table[(int64_t)head * p.n_buckets + p.lut[i]];
+  if (count)
+    for (int i = lane; i < p.n_rel; i += 64) hist[i] = 0.f;
+  float dslope = 0.f, low = 0.f, high = 0.f;  // low, high: the two clipped ends of the table, per lane
+
+  for (int item = worker; item < p.count; item += p.workers) {
+    const AttnWork w = p.work[item];
+    const int mine = (COOP ? wave * kTile : 0) + col;
+    const bool live = mine < w.cols;
+    const bool busy = (COOP ? wave * kTile : 0) < w.cols;
+    const bool whole = (COOP ? wave * kTile : 0) + kTile <= w.cols;
+    const int64_t row = (int64_t)w.col0 + (live ? mine : 0);
+
+    typename vec8<T>::type qf[DP / 16], df[DP / 16];
+    const T* qp = (const T*)p.q + row * p.q_row + head * p.q_head;
+    const T* dp_ = (const T*)p.dout + row * p.do_row + head * p.do_head;
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) {
+      qf[c] = load_col<T>(qp, c * 16 + hi * 8, p.dim, live);
+      df[c] = load_col<T>(dp_, c * 16 + hi * 8, p.dim, live);
+    }
+    const float2 ml = p.stats[head * p.rows_q + row];
+    const float ref = ml.x == -INFINITY ? 0.f : ml.x;
+    const float inv_l = ml.y == 0.f ? 0.f : 1.f / ml.y;
+    float px = 0, py = 0, pz = 0, gx = 0, gy = 0, gz = 0;
+    if (p.slope) px = p.q_pos[3 * row], py = p.q_pos[3 * row + 1], pz = p.q_pos[3 * row + 2];
+    const int res = p.table ? p.q_res[row] : 0;
+
+    f32x16 dq[DP / 32];
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) dq[d] = acc_zero();
+    ColumnScale cs;
+
+    TilePair<T, DP, THREADS> tiles;
+    constexpr bool AHEAD = TilePair<T, DP, THREADS>::N <= 8;
+    if (AHEAD && w.row0 < w.row1)
+      tiles.load(kp + w.row0 * p.k_row, p.k_row, vp + w.row0 * p.v_row, p.v_row, w.row1 - w.row0, p.dim, tid);
+    float delta = 0.f;
+    const bool once = w.row1 - w.row0 <= kTile;
+    bool sum_delta = true;  // the walk for D (with `once`: that tile itself)
+    for (int k0 = w.row0; k0 < w.row1;) {
+      const int n = w.row1 - k0 < kTile ? w.row1 - k0 : kTile;
+      if (!AHEAD) tiles.load(kp + k0 * p.k_row, p.k_row, vp + k0 * p.v_row, p.v_row, n, p.dim, tid);
+      tile_sync<COOP>();
+      tiles.store(lds.a, lds.b, tid);
+      if (tid < kTile) {
+        const int64_t kr = k0 + (tid < n ? tid : 0);
+        if (p.slope) lds.pos[tid] = make_float4(p.k_pos[3 * kr], p.k_pos[3 * kr + 1], p.k_pos[3 * kr + 2], 0.f);
+        if (p.table) lds.res[tid] = p.k_res[kr];
+      }
+      tile_sync<COOP>();
+      const bool first = sum_delta;
+      k0 += kTile;
+      if (first && !once && k0 >= w.row1) k0 = w.row0, sum_delta = false;
+      if (AHEAD && k0 < w.row1)
+        tiles.load(kp + k0 * p.k_row, p.k_row, vp + k0 * p.v_row, p.v_row, w.row1 - k0, p.dim, tid);
+      if (!busy) continue;
+
+      f32x16 acc = acc_zero(), dp = acc_zero();
+#pragma unroll
+      for (int c = 0; c < DP / 16; ++c)
+        if (c * 16 < p.dim) {
+          acc = Mma<T>::run(load_n<T, DP>(lds.a, c, col, hi), qf[c], acc);
+          dp = Mma<T>::run(load_n<T, DP>(lds.b, c, col, hi), df[c], dp);
+        }
+      float s[16];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = acc[r] * p.scale;
+      if (p.slope) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float4 k = lds.pos[acc_row(r, hi)];
+          float inv;
+          s[r] -= slope * pair_dist(px - k.x, py - k.y, pz - k.z, inv);
+        }
+      }
+      if (p.table) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] += lds.tab[rel_index(lds.res[acc_row(r, hi)], res, p.reach)];
+      }
+      if (n < kTile || !whole) {
+        const int limit = live ? n : 0;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = acc_row(r, hi) < limit ? s[r] : -INFINITY;
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f((s[r] - ref) * kLog2e) * inv_l;
+      if (first) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) delta += s[r] * dp[r];
+        if (once || !sum_delta) delta += other_half(delta);
+        if (!once) continue;
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] *= dp[r] - delta;  // dS from here on
+
+      if (p.slope) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float4 k = lds.pos[acc_row(r, hi)];
+          const float dx = px - k.x, dy = py - k.y, dz = pz - k.z;
+          float inv;
+          const float far = pair_dist(dx, dy, dz, inv);
+          dslope -= s[r] * far;
+          const float pull = s[r] * inv;
+          gx += pull * dx, gy += pull * dy, gz += pull * dz;
+        }
+      }
+      if (count) {
+        // runs of keys of one residue are added up in the lane first; the clipped ends stay in the lane altogether
+        float run = 0.f;
+        int at = rel_index(lds.res[acc_row(0, hi)], res, p.reach);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          run += s[r];
+          const int then = r < 15 ? rel_index(lds.res[acc_row(r < 15 ? r + 1 : 15, hi)], res, p.reach) : -1;
+          if (then != at) {
+            if (at == 0)
+              low += run;
+            else if (at == 2 * p.reach)
+              high += run;
+            else
+              __hip_atomic_fetch_add(hist + at, run, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+            run = 0.f;
+          }
+          at = then;
+        }
+      }
+      if constexpr (HALF) {
+        float largest = 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) largest = fmaxf(largest, fabsf(s[r]));
+        const float change = cs.follow(fmaxf(largest, other_half(largest)));
+        if (__any(change != 1.f)) {
+#pragma unroll
+          for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) dq[d][r] *= change;
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] *= cs.f;
+      }
+      const typename vec8<T>::type s0 = pack8<T>(s), s1 = pack8<T>(s + 8);
+#pragma unroll
+      for (int d = 0; d < DP / 32; ++d) {
+        if (d * 32 >= p.dim) continue;
+        dq[d] = Mma<T>::run(load_t<T, DP>(lds.a, 0, d * 32, lane, hi), s0, dq[d]);
+        dq[d] = Mma<T>::run(load_t<T, DP>(lds.a, 1, d * 32, lane, hi), s1, dq[d]);
+      }
+    }
+
+    if (p.part_pos_q) {
+      gx += other_half(gx), gy += other_half(gy), gz += other_half(gz);
+      if (live && hi == 0) {
+        float* g = p.part_pos_q + (head * p.rows_q + row) * 3;
+        g[0] = -slope * gx, g[1] = -slope * gy, g[2] = -slope * gz;
+      }
+    }
+    if (live && hi == 0) p.delta[head * p.rows_q + row] = delta;
+    if (live) {
+      const float f = HALF ? p.scale / cs.f : p.scale;
+      T* o = (T*)p.dq + (row * p.heads + head) * p.dim;
+#pragma unroll
+      for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int e = d * 32 + 8 * g + 4 * hi;
+          if (e < p.dim) store4<T>(o + e, dq[d][4 * g] * f, dq[d][4 * g + 1] * f, dq[d][4 * g + 2] * f, dq[d][4 * g + 3] * f);
+        }
+    }
+  }
+
+  const int64_t part = p.part0 + worker;
+  if (p.part_slope) {
+    dslope = wave_sum(dslope);
+    if (lane == 0) {
+      float* out = p.part_slope + (head * (int64_t)p.parts + part) * kCoopWaves;
+      if (COOP) {
+        out[wave] = dslope;
+      } else {
+        out[0] = dslope;
+        out[1] = out[2] = out[3] = 0.f;
+      }
+    }
+  }
+  if (count) {
+    low = wave_sum(low);
+    high = wave_sum(high);
+    if (lane == 0) {
+      hist[0] += low;
+      hist[2 * p.reach] += high;
+    }
+    tile_sync<COOP>();
+    for (int i = tid; i < p.n_rel; i += THREADS) {
+      float t = hist_all[i];
+      if (COOP)
+        for (int k = 1; k < kCoopWaves; ++k) t += hist_all[k * p.n_rel + i];
+      p.part_hist[((int64_t)head * p.n_rel + i) * p.parts + part] = t;
+    }
+  }
+}
+
+template <typename T, int DP, bool COOP>
+__global__ __launch_bounds__(256) void k_attn_bwd_k(AttnParams p, size_t lds_per_wave) {
+  extern __shared__ __attribute__((aligned(16))) char lds_raw[];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int col = lane & 31, hi = lane >> 5;
+  const int tid = COOP ? threadIdx.x : lane;
+  constexpr int THREADS = COOP ? 64 * kCoopWaves : 64;
+  constexpr bool HALF = sizeof(T) == 2 && !__is_same(T, __bf16);
+  const int64_t id = COOP ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * (blockDim.x >> 6) + wave;
+  if (id >= (int64_t)p.count * p.kv_heads) return;
+  const int kv = (int)(id % p.kv_heads), share = p.heads / p.kv_heads;
+  const AttnWork w = p.work[id / p.kv_heads];
+  const AttnLds<T, DP> lds(lds_raw + (COOP ? 0 : wave * lds_per_wave));
+
+  const int mine = (COOP ? wave * kTile : 0) + col;
+  const bool live = mine < w.cols;
+  const bool busy = (COOP ? wave * kTile : 0) < w.cols;
+  const bool whole = (COOP ? wave * kTile : 0) + kTile <= w.cols;
+  const int64_t row = (int64_t)w.col0 + (live ? mine : 0);
+
+  typename vec8<T>::type kf[DP / 16], vf[DP / 16];
+  const T* kp = (const T*)p.k + row * p.k_row + kv * p.k_head;
+  const T* vp = (const T*)p.v + row * p.v_row + kv * p.v_head;
+#pragma unroll
+  for (int c = 0; c < DP / 16; ++c) {
+    kf[c] = load_col<T>(kp, c * 16 + hi * 8, p.dim, live);
+    vf[c] = load_col<T>(vp, c * 16 + hi * 8, p.dim, live);
+  }
+  float px = 0, py = 0, pz = 0, gx = 0, gy = 0, gz = 0;
+  if (p.slope) px = p.k_pos[3 * row], py = p.k_pos[3 * row + 1], pz = p.k_pos[3 * row + 2];
+  const int res = p.table ? p.k_res[row] : 0;
+
+  f32x16 dk[DP / 32], dv[DP / 32];
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d) dk[d] = acc_zero(), dv[d] = acc_zero();
+  ColumnScale cs;
+  constexpr float PUP = HALF ? 0x1p14f : 1.f;
+
+  for (int sub = 0; sub < share; ++sub) {
+    const int head = kv * share + sub;
+    const T* qp = (const T*)p.q + head * p.q_head;
+    const T* dp_ = (const T*)p.dout + head * p.do_head;
+    const float slope = p.slope ? p.slope[head] : 0.f;
+    if (p.table) {
+      tile_sync<COOP>();
+      for (int i = tid; i < p.n_rel; i += THREADS) lds.tab[i] = p.table[(int64_t)head * p.n_buckets + p.lut[i]];
+    }
+    TilePair<T, DP, THREADS> tiles;
+    constexpr bool AHEAD = TilePair<T, DP, THREADS>::N <= 8;
+    if (AHEAD && w.row0 < w.row1)
+      tiles.load(qp + w.row0 * p.q_row, p.q_row, dp_ + w.row0 * p.do_row, p.do_row, w.row1 - w.row0, p.dim, tid);
+    for (int q0 = w.row0; q0 < w.row1; q0 += kTile) {
+      const int n = w.row1 - q0 < kTile ? w.row1 - q0 : kTile;
+      if (!AHEAD) tiles.load(qp + q0 * p.q_row, p.q_row, dp_ + q0 * p.do_row, p.do_row, n, p.dim, tid);
+      tile_sync<COOP>();
+      tiles.store(lds.a, lds.b, tid);
+      if (tid < kTile) {
+        const int64_t qr = q0 + (tid < n ? tid : 0);
+        if (p.slope) lds.pos[tid] = make_float4(p.q_pos[3 * qr], p.q_pos[3 * qr + 1], p.q_pos[3 * qr + 2], 0.f);
+        if (p.table) lds.res[tid] = p.q_res[qr];
+        const float2 ml = p.stats[head * p.rows_q + qr];
+        lds.stat[tid] = make_float4(ml.x == -INFINITY ? 0.f : ml.x, ml.y == 0.f ? 0.f : 1.f / ml.y,
+                                    p.delta[head * p.rows_q + qr], 0.f);
+      }
+      tile_sync<COOP>();
+      const int next = q0 + kTile;
+      if (AHEAD && next < w.row1)
+        tiles.load(qp + next * p.q_row, p.q_row, dp_ + next * p.do_row, p.do_row, w.row1 - next, p.dim, tid);
+      if (!busy) continue;
+
+      f32x16 acc = acc_zero(), dp = acc_zero();
+#pragma unroll
+      for (int c = 0; c < DP / 16; ++c)
+        if (c * 16 < p.dim) {
+          acc = Mma<T>::run(load_n<T, DP>(lds.a, c, col, hi), kf[c], acc);
+          dp = Mma<T>::run(load_n<T, DP>(lds.b, c, col, hi), vf[c], dp);
+        }
+      float s[16];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = acc[r] * p.scale;
+      if (p.slope) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float4 q = lds.pos[acc_row(r, hi)];
+          float inv;
+          s[r] -= slope * pair_dist(q.x - px, q.y - py, q.z - pz, inv);
+        }
+      }
+      if (p.table) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] += lds.tab[rel_index(res, lds.res[acc_row(r, hi)], p.reach)];
+      }
+      if (n < kTile || !whole) {
+        const int limit = live ? n : 0;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = acc_row(r, hi) < limit ? s[r] : -INFINITY;
+      }
+      float pr[16];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float4 st = lds.stat[acc_row(r, hi)];
+        const float e = __builtin_amdgcn_exp2f((s[r] - st.x) * kLog2e) * st.y;
+        s[r] = e * (dp[r] - st.z);  // dS from here on
+        pr[r] = e * PUP;
+      }
+      if (p.part_pos_k) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float4 q = lds.pos[acc_row(r, hi)];
+          const float dx = q.x - px, dy = q.y - py, dz = q.z - pz;
+          float inv;
+          pair_dist(dx, dy, dz, inv);
+          const float pull = slope * s[r] * inv;
+          gx += pull * dx, gy += pull * dy, gz += pull * dz;
+        }
+      }
+      if constexpr (HALF) {
+        float largest = 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) largest = fmaxf(largest, fabsf(s[r]));
+        const float change = cs.follow(fmaxf(largest, other_half(largest)));
+        if (__any(change != 1.f)) {
+#pragma unroll
+          for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) dk[d][r] *= change;
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] *= cs.f;
+      }
+      const typename vec8<T>::type s0 = pack8<T>(s), s1 = pack8<T>(s + 8), p0 = pack8<T>(pr), p1 = pack8<T>(pr + 8);
+#pragma unroll
+      for (int d = 0; d < DP / 32; ++d) {
+        if (d * 32 >= p.dim) continue;
+        dv[d] = Mma<T>::run(load_t<T, DP>(lds.b, 0, d * 32, lane, hi), p0, dv[d]);
+        dv[d] = Mma<T>::run(load_t<T, DP>(lds.b, 1, d * 32, lane, hi), p1, dv[d]);
+        dk[d] = Mma<T>::run(load_t<T, DP>(lds.a, 0, d * 32, lane, hi), s0, dk[d]);
+        dk[d] = Mma<T>::run(load_t<T, DP>(lds.a, 1, d * 32, lane, hi), s1, dk[d]);
+      }
+    }
+  }
+
+  if (p.part_pos_k) {
+    gx += other_half(gx), gy += other_half(gy), gz += other_half(gz);
+    if (live && hi == 0) {
+      float* g = p.part_pos_k + (kv * p.rows_k + row) * 3;
+      g[0] = gx, g[1] = gy, g[2] = gz;
+    }
+  }
+  if (!live) return;
+  const float f = HALF ? p.scale / cs.f : p.scale;
+  constexpr float PDOWN = 1.f / PUP;
+  T* ok = (T*)p.dk + (row * p.kv_heads + kv) * p.dim;
+  T* ov = (T*)p.dv + (row * p.kv_heads + kv) * p.dim;
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int e = d * 32 + 8 * g + 4 * hi;
+      if (e >= p.dim) continue;
+      store4<T>(ok + e, dk[d][4 * g] * f, dk[d][4 * g + 1] * f, dk[d][4 * g + 2] * f, dk[d][4 * g + 3] * f);
+      store4<T>(ov + e, dv[d][4 * g] * PDOWN, dv[d][4 * g + 1] * PDOWN, dv[d][4 * g + 2] * PDOWN, dv[d][4 * g + 3] * PDOWN);
+    }
+}
+
+// Joins the partial sums in a fixed order: positions over heads (workgroups 0 ... n_pos - 1, one thread per component),
+// then one workgroup per head for its slope and one per (head, bucket) for the table, both summed in float64.
+__global__ __launch_bounds__(256) void k_attn_bwd_join(AttnParams p, int n_pos, int n_slope) {
+  const int b = blockIdx.x, tid = threadIdx.x;
+  if (b < n_pos) {
+    const int64_t at = (int64_t)b * 256 + tid;
+    if (at < p.used_k * 3 && p.dpos) {
+      float t = 0.f;
+      for (int h = 0; h < p.kv_heads; ++h) t += p.part_pos_k[h * p.rows_k * 3 + at];
+      if (!p.dq_pos)
+        for (int h = 0; h < p.heads; ++h) t += p.part_pos_q[h * p.rows_q * 3 + at];
+      p.dpos[at] = t;
+    }
+    if (at < p.used_q * 3 && p.dq_pos) {
+      float t = 0.f;
+      for (int h = 0; h < p.heads; ++h) t += p.part_pos_q[h * p.rows_q * 3 + at];
+      p.dq_pos[at] = t;
+    }
+    return;
+  }
+  __shared__ double red[4];
+  double t = 0.0;
+  float* out;
+  if (b < n_pos + n_slope) {
+    const int head = b - n_pos;
+    for (int i = tid; i < p.parts * kCoopWaves; i += 256) t += p.part_slope[(int64_t)head * p.parts * kCoopWaves + i];
+    out = p.dslope + head;
+  } else {
+    const int at = b - n_pos - n_slope, head = at / p.n_buckets, bucket = at % p.n_buckets;
+    for (int rel = 0; rel < p.n_rel; ++rel)
+      if (p.lut[rel] == bucket)
+        for (int i = tid; i < p.parts; i += 256) t += p.part_hist[((int64_t)head * p.n_rel + rel) * p.parts + i];
+    out = p.dtable + at;
+  }
+  for (int o = 32; o > 0; o >>= 1) t += __shfl_xor(t, o, 64);
+  if ((tid & 63) == 0) red[tid >> 6] = t;
+  __syncthreads();
+  if (tid == 0) *out = (float)(red[0] + red[1] + red[2] + red[3]);
+}
+
+template <typename T, int DP>
+static int bwd_launch(const AttnPlanView& by_query, const AttnPlanView& by_key, AttnParams p, int lone_workers,
+                      int coop_workers, hipStream_t st) {
+  const int n_rel = p.table ? p.n_rel : 0;
+  const size_t tab = AttnLds<T, DP>::bytes(n_rel);
+  const size_t lone_q = AttnLds<T, DP>::bytes(n_rel + (p.part_hist ? p.n_rel : 0));
+  const size_t coop_q = AttnLds<T, DP>::bytes(n_rel + (p.part_hist ? kCoopWaves * p.n_rel : 0));
+  if (by_query.lone) {
+    p.work = by_query.lone_work, p.count = by_query.lone, p.workers = lone_workers, p.part0 = 0;
+    const int64_t total = (int64_t)lone_workers * p.heads;
+    const int waves = lone_waves(total, lone_q);
+    if (!allow_lds((const void*)k_attn_bwd_q<T, DP, false>, waves * lone_q)) return -5;
+    hipLaunchKernelGGL((k_attn_bwd_q<T, DP, false>), dim3((unsigned)((total + waves - 1) / waves)), dim3(64 * waves),
+                       waves * lone_q, st, p, lone_q);
+  }
+  if (by_query.coop) {
+    p.work = by_query.coop_work, p.count = by_query.coop, p.workers = coop_workers, p.part0 = lone_workers;
+    if (!allow_lds((const void*)k_attn_bwd_q<T, DP, true>, coop_q)) return -5;
+    hipLaunchKernelGGL((k_attn_bwd_q<T, DP, true>), dim3((unsigned)((int64_t)coop_workers * p.heads)),
+                       dim3(64 * kCoopWaves), coop_q, st, p, coop_q);
+  }
+  if (by_key.lone) {
+    p.work = by_key.lone_work, p.count = by_key.lone;
+    const int64_t total = (int64_t)by_key.lone * p.kv_heads;
+    const int waves = lone_waves(total, tab);
+    if (!allow_lds((const void*)k_attn_bwd_k<T, DP, false>, waves * tab)) return -5;
+    hipLaunchKernelGGL((k_attn_bwd_k<T, DP, false>), dim3((unsigned)((total + waves - 1) / waves)), dim3(64 * waves),
+                       waves * tab, st, p, tab);
+  }
+  if (by_key.coop) {
+    p.work = by_key.coop_work, p.count = by_key.coop;
+    if (!allow_lds((const void*)k_attn_bwd_k<T, DP, true>, tab)) return -5;
+    hipLaunchKernelGGL((k_attn_bwd_k<T, DP, true>), dim3((unsigned)((int64_t)by_key.coop * p.kv_heads)),
+                       dim3(64 * kCoopWaves), tab, st, p, tab);
+  }
+  const int64_t rows = p.used_k > p.used_q ? p.used_k : p.used_q;
+  const int n_pos = p.dpos || p.dq_pos ? (int)((rows * 3 + 255) / 256) : 0;
+  const int n_slope = p.dslope ? p.heads : 0, n_table = p.dtable ? p.heads * p.n_buckets : 0;
+  if (n_pos + n_slope + n_table)
+    hipLaunchKernelGGL(k_attn_bwd_join, dim3(n_pos + n_slope + n_table), dim3(256), 0, st, p, n_pos, n_slope);
+  return hipGetLastError() == hipSuccess ? 0 : -5;
+}
+
+template <typename T>
+static int bwd_dim(const AttnPlanView& a, const AttnPlanView& b, const AttnParams& p, int lw, int cw, hipStream_t st) {
+  if (p.dim <= 32) return bwd_launch<T, 32>(a, b, p, lw, cw, st);
+  if (p.dim <= 64) return bwd_launch<T, 64>(a, b, p, lw, cw, st);
+  return bwd_launch<T, 128>(a, b, p, lw, cw, st);
+}
+
+int attn_backward(int dtype, const AttnPlanView& by_query, const AttnPlanView& by_key, const AttnParams& p,
+                  int lone_workers, int coop_workers, hipStream_t st) {
+  switch (dtype) {
+    case VSN_F32: return bwd_dim<float>(by_query, by_key, p, lone_workers, coop_workers, st);
+    case VSN_BF16: return bwd_dim<__bf16>(by_query, by_key, p, lone_workers, coop_workers, st);
+    default: return bwd_dim<_Float16>(by_query, by_key, p, lone_workers, coop_workers, st);
+  }
+}
+
+}  // namespace vsn

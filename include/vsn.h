@@ -312,6 +312,59 @@ int vsn_layernorm_backward(int device_id, int dtype, int param_dtype, const void
                            int width, void* dev_dx, int64_t lddx, void* dev_dw, void* dev_db, void* dev_workspace,
                            int64_t workspace_bytes, void* stream);
 
+/* Fragment attention: softmax attention among ALL atoms of a fragment (the engine's ViS-MP attention,
+ * ViSNet/model/visnet_block.py:276-312, runs over <= 32 neighbours and has no softmax), its scores biased by distance and
+ * by residue offset.  For query row i and key row j of one fragment, head a, key head a / (heads / kv_heads):
+ *   s_ij = scale q_i.k_j - slope[a] |x_i - x_j| + table[a][bucket(res_j - res_i)],  P = softmax_j(s),  o_i = sum_j P_ij v_j
+ * A row whose fragment has no keys, or whose scores are all -inf, gives 0 and no gradient.
+ *
+ *   vsn_attn_create   the plan of a batch layout: fragment f's keys are rows host_start[f] ... host_end[f] - 1, its
+ *     queries the same rows, or those of host_query_start / host_query_end (both NULL: the same), e.g. one read-out row
+ *     per fragment.  Ranges contiguous and ascending from 0, as in vsn_forces; empty ones are allowed.  head_dim: a
+ *     multiple of 8, 8 ... 128; kv_heads divides heads.  n_buckets > 0: host_buckets[2 reach + 1] gives the bucket of
+ *     each difference clipped to -reach ... reach (reach <= 1023).  A plan holds no results and may be used from any
+ *     stream, by several calls at once.
+ *   vsn_attn_io   `q` [rows_q][heads][head_dim], `k`, `v` [rows_k][kv_heads][head_dim], `out` as q: last axis dense, the
+ *     strides (elements) of rows and heads multiples of 16 bytes, addresses too.  rows_* may exceed the plan's: rows
+ *     behind the last fragment are neither read nor written.  q_pos / k_pos f32 [rows][3] and slope f32 [heads]: all
+ *     or none.  q_res / k_res i32 [rows] and table f32 [heads][n_buckets]: all or none.  stats f32
+ *     [heads][rows_q][2] (maximum, sum of exponentials) is all that a backward call needs of the forward one (NULL in a
+ *     forward call: not wanted); `out` is not read by a backward call.
+ *   vsn_attn_grads   dout as out; dq, dk, dv dense.  dpos f32 [rows_k][3]: of both ends of a pair where dquery_pos is
+ *     NULL (queries = keys), else of the keys' positions, and dquery_pos f32 [rows_q][3] of the queries'.  dpos, dslope
+ *     f32 [heads], dtable f32 [heads][n_buckets] are overwritten and may be NULL.  Fixed summation order.
+ * Asynchronous on `stream`; the workspace (vsn_attn_workspace bytes, 16-byte aligned) belongs to the call until the
+ * stream has passed it. */
+typedef struct vsn_attn* vsn_attn_handle;
+typedef struct vsn_attn_io {
+  int32_t dtype; /* VSN_F32 | VSN_BF16 | VSN_F16: q, k, v, out and the gradients of q, k, v, out */
+  float scale;
+  int64_t rows_q, rows_k;
+  const void *q, *k, *v;
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head;
+  const float *q_pos, *k_pos, *slope;
+  const int32_t *q_res, *k_res;
+  const float* table;
+  void* out;
+  int64_t out_row, out_head;
+  float* stats;
+} vsn_attn_io;
+typedef struct vsn_attn_grads {
+  const void* dout;
+  int64_t dout_row, dout_head;
+  void *dq, *dk, *dv;
+  float *dpos, *dquery_pos, *dslope, *dtable;
+} vsn_attn_grads;
+int vsn_attn_create(vsn_attn_handle* out, int device_id, int64_t n_fragments, const int64_t* host_start,
+                    const int64_t* host_end, const int64_t* host_query_start, const int64_t* host_query_end, int heads,
+                    int kv_heads, int head_dim, int reach, const int32_t* host_buckets, int n_buckets);
+void vsn_attn_destroy(vsn_attn_handle a);
+int64_t vsn_attn_workspace(vsn_attn_handle a, int64_t rows_q, int64_t rows_k, int backward);
+int vsn_attn_forward(vsn_attn_handle a, const vsn_attn_io* io, void* dev_workspace, int64_t workspace_bytes,
+                     void* stream);
+int vsn_attn_backward(vsn_attn_handle a, const vsn_attn_io* io, const vsn_attn_grads* grads, void* dev_workspace,
+                      int64_t workspace_bytes, void* stream);
+
 /* ---- work partitions (Calculators/device_strategy.py:84-127) ---- */
 /* Writes up to max_out triples (device_idx, frag_begin, frag_end); returns count. */
 int vsn_partition(const int64_t* host_start, const int64_t* host_end, int64_t B, int n_devices,

@@ -44,3 +44,71 @@ def test_layer_norm_refuses_host_tensors():
         layer_norm(x)
     with pytest.raises(ValueError, match="cuda"):
         layer_norm_backward(x, x, torch.zeros(4, 2))
+
+
+def i64(*v):
+    return (C.c_int64 * len(v))(*v)
+
+
+def test_attention_entry_points_refuse(lib_built):
+    from ai2bmd_amd import capi
+    L = capi.lib()
+    h = C.c_void_p()
+    s, e = i64(0, 5), i64(5, 9)
+    lut = (C.c_int32 * 5)(0, 1, 2, 1, 0)
+    good = [C.byref(h), 0, 2, s, e, None, None, 8, 8, 32, 2, lut, 3]
+
+    def create(**change):
+        a = list(good)
+        for k, v in change.items():
+            a[int(k[1:])] = v
+        return L.vsn_attn_create(*a)
+
+    assert create(_0=None) == -22
+    assert create(_2=0) == create(_2=-1) == -22                                       # no fragments
+    assert create(_3=None) == create(_3=i64(0, 6)) == create(_3=i64(1, 5)) == -22      # gaps, a start that is not 0
+    assert create(_4=i64(5, 4)) == create(_4=i64(5, 1 << 40)) == -22                   # backwards, too many rows
+    assert create(_5=s) == create(_5=i64(0, 3), _6=i64(2, 4)) == -22                   # half of the query ranges, a gap
+    assert create(_7=0) == create(_8=3) == create(_8=0) == -22                         # heads
+    assert create(_9=4) == create(_9=36) == create(_9=136) == -22                      # head_dim
+    assert create(_10=1024) == create(_10=-1) == create(_11=None) == -22               # reach, map
+    assert create(_12=2) == create(_12=4097) == create(_12=-1) == -22                  # a bucket beyond the table
+    assert create(_11=(C.c_int32 * 5)(0, 1, -1, 1, 0)) == -22
+    assert not h.value
+    assert L.vsn_attn_workspace(None, 1, 1, 0) == -22
+    io, g = capi.VsnAttnIO(), capi.VsnAttnGrads()
+    assert L.vsn_attn_forward(None, C.byref(io), None, 0, None) == -22
+    assert L.vsn_attn_backward(None, C.byref(io), C.byref(g), None, 0, None) == -22
+    L.vsn_attn_destroy(None)
+    if not torch.cuda.is_available():
+        assert create() == -19
+
+
+def test_attention_plan_refuses_in_python():
+    from ai2bmd_amd.attention import FragmentAttention
+    with pytest.raises(RuntimeError, match="cuda"):
+        FragmentAttention([0], [4], 2, 8, device="cpu")
+    for bad in (dict(start=[1], end=[4]), dict(start=[0, 5], end=[4, 6]), dict(start=[], end=[]), dict(start=[0], end=[[4]]),
+                dict(heads=3, num_kv_heads=2), dict(dim=12), dict(dim=136), dict(dim=0), dict(buckets=[0, 1]), dict(buckets=[0, -1, 0]),
+                dict(buckets=[0] * 2049), dict(buckets=[0, 1, 2], num_buckets=2), dict(buckets=[0], num_buckets=5000), dict(query_start=[0]),
+                dict(query_start=[0, 1], query_end=[1, 2])):
+        a = dict(start=[0], end=[4], heads=2, dim=8)
+        a.update(bad)
+        with pytest.raises(ValueError):
+            FragmentAttention(a.pop("start"), a.pop("end"), a.pop("heads"), a.pop("dim"), **a)
+
+
+def test_relative_buckets():
+    from ai2bmd_amd.attention import relative_buckets
+    assert relative_buckets(9, 4).tolist() == list(range(9))
+    assert relative_buckets(3, 0).tolist() == [0]
+    b = relative_buckets(32, 128)
+    assert len(b) == 257 and b[128] == 0 and b.min() == 0 and b.max() == 31
+    assert b[128 - 7:128][::-1].tolist() == [1, 2, 3, 4, 5, 6, 7] and b[129:136].tolist() == [17, 18, 19, 20, 21, 22, 23]
+    back, ahead = b[:128][::-1], b[129:]
+    assert (ahead == back + 16).all() and (back[1:] >= back[:-1]).all()
+    # the border of bucket 8 + n lies at 8 * 16^(n / 8): 16 ^ (1 / 2) = 4 gives 32 for n = 4, 8 * 16^(1 / 8) = 11.3 for n = 1
+    assert back[31 - 1] == 11 and back[32 - 1] == 12 and back[11 - 1] == 8 and back[12 - 1] == 9 and back[128 - 1] == 15
+    for bad in ((31, 128), (2, 128), (0, 4), (32, 1024), (32, -1)):
+        with pytest.raises(ValueError):
+            relative_buckets(*bad)
