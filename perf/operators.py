@@ -204,8 +204,9 @@ def prepare(case, seed):
     bucket = _bucket_map(case) if case["buckets"] else None
     if own:
         from ai2bmd_amd.attention import FragmentAttention
-        state["plan"] = FragmentAttention(k0, k1, heads, dim, num_kv_heads=kv_heads, query_start=q0, query_end=q1,
-                                          buckets=bucket, device="cuda:0")
+        ranges = dict(query_start=q0, query_end=q1) if apart else {}
+        state["plan"] = FragmentAttention(k0, k1, heads, dim, num_kv_heads=kv_heads, buckets=bucket, device="cuda:0",
+                                          **ranges)
     else:
         state["bucket"] = None if bucket is None else torch.as_tensor(bucket, device="cuda").long()
         state["groups"] = _groups(q0, q1, k0, k1, heads)
