@@ -64,9 +64,9 @@ def build(force: bool = False, verbose: bool = False) -> str:
         return LIB
     hipcc = _hipcc()
 
-    def unit_digest(src):  # one translation unit: its source, every header, its flags
+    def unit_digest(src):  # one translation unit: its source, every header (attention*.h: of its own units), its flags
         h = hashlib.sha256()
-        for f in [src] + HEADERS:
+        for f in [src] + [x for x in HEADERS if not x.startswith("attention") or src.startswith("attention")]:
             with open(os.path.join(CSRC, f), "rb") as fh:
                 h.update(fh.read())
         h.update(" ".join(FLAGS + PER_FILE_FLAGS.get(src, [])).encode())

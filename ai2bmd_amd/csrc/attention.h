@@ -8,7 +8,11 @@
 // registers, so everything that belongs to a column (running maximum and sum, position, residue, gradient scale) is the
 // lane's own, and a column of P or dS is already the B operand of the next product: that product contracts over the
 // tile's rows, whose order inside a contraction is free, and takes its A operand in the same order (load_t).
-// Float32 runs the same tiles on the float32 matrix instruction (8 of 2 rows instead of one of 16).
+// Float32 runs the same tiles on the float32 matrix instruction (8 of 2 rows instead of one of 16), each tile's product
+// in an accumulator of its own that is then added to the sum: a chain of one addition per two rows would lose half of a
+// decimal digit over a protein of some thousand atoms.
+// Scores are in units of log 2 (scale, slopes and table are multiplied by log2 e beforehand), so the exponential needs no
+// product of its own, and no rounding of one.
 #pragma once
 #include "typed.h"
 
@@ -47,12 +51,12 @@ struct AttnParams {
   int64_t rows_q, rows_k; // rows of the arrays (statistics and partial sums are laid out by them)
   void* out;
   int64_t out_row, out_head;
-  float2* stats;          // [heads][rows_q] {maximum, sum of exponentials}
+  float2* stats;          // [heads][rows_q] {maximum in units of log 2, sum of exponentials}
   float* part_o;          // split keys: [slot][heads][32][dim] unnormalised output
   float2* part_ml;        // [slot][heads][32]
   const AttnJoin* join;
   // backward
-  float* delta;           // [heads][rows_q]
+  float2* delta;          // [heads][rows_q] {D, 1 / sum of exponentials}
   void *dq, *dk, *dv;     // contiguous
   float* part_pos_q;      // [heads][rows_q][3] or null
   float* part_pos_k;      // [kv_heads][rows_k][3] or null
@@ -225,7 +229,54 @@ __device__ __forceinline__ int rel_index(int key_res, int query_res, int reach) 
   return (d < -reach ? -reach : d > reach ? reach : d) + reach;
 }
 
+// a table entry in units of log 2; the lowest float32 stays a finite value (a mask of it must not turn into -inf)
+__device__ __forceinline__ float table_log2(float t) {
+  const float v = t * kLog2e;
+  return fabsf(t) < INFINITY ? __builtin_amdgcn_fmed3f(v, -3.4028235e38f, 3.4028235e38f) : v;
+}
+
+// c += a * b over one tile of 32 rows
+template <typename T>
+__device__ __forceinline__ void tile_mma(f32x16& c, typename vec8<T>::type a0, typename vec8<T>::type b0,
+                                         typename vec8<T>::type a1, typename vec8<T>::type b1) {
+  if constexpr (sizeof(T) == 4) {
+    f32x16 t = acc_zero();
+    t = Mma<T>::run(a0, b0, t);
+    t = Mma<T>::run(a1, b1, t);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) c[r] += t[r];
+  } else {
+    c = Mma<T>::run(a0, b0, c);
+    c = Mma<T>::run(a1, b1, c);
+  }
+}
+
 __device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, 64); }
+
+// the 16 values of a tile's column half, added up pairwise
+__device__ __forceinline__ float tile_sum(const float* v) {
+  float t[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) t[i] = v[i] + v[i + 8];
+  return ((t[0] + t[4]) + (t[2] + t[6])) + ((t[1] + t[5]) + (t[3] + t[7]));
+}
+
+// A sum over many tiles that carries its rounding error along (two-sum): sums over whole proteins whose terms cancel -
+// sum_j dS_ij is 0 - keep the precision of their tiles.
+struct LongSum {
+  float s = 0.f, c = 0.f;
+  __device__ __forceinline__ void add(float x) {
+    const float t = s + x, b = t - s;
+    c += (s - (t - b)) + (x - b);
+    s = t;
+  }
+  __device__ __forceinline__ void scale(float f) { s *= f, c *= f; }
+  __device__ __forceinline__ float both_halves() const {
+    const float hi = s + other_half(s), lo = c + other_half(c);
+    return hi + lo;
+  }
+  __device__ __forceinline__ float value() const { return s + c; }
+};
 
 // wave-private (or shared) LDS of one work item
 template <typename T, int DP>

@@ -141,7 +141,7 @@ BackwardSpace backward_space(const vsn_attn& a, int64_t rows_q, int64_t rows_k) 
   s.coop = workers(a.by_query.coop, a.heads, a.n_rel, 2048);
   s.parts = s.lone + s.coop;
   Workspace w;
-  s.delta = w.take(rows_q * a.heads * 4);
+  s.delta = w.take(rows_q * a.heads * 8);
   s.pos_q = w.take(rows_q * a.heads * 12);
   s.pos_k = w.take(rows_k * a.kv_heads * 12);
   s.slope = w.take((int64_t)s.parts * a.heads * kCoopWaves * 4);
@@ -306,7 +306,7 @@ extern "C" int vsn_attn_backward(vsn_attn_handle a, const vsn_attn_io* io, const
   char* base = (char*)dev_workspace;
   AttnParams p = params(*a, *io);
   p.dout = g->dout, p.do_row = g->dout_row, p.do_head = g->dout_head;
-  p.delta = (float*)(base + s.delta);
+  p.delta = (float2*)(base + s.delta);
   p.dq = g->dq, p.dk = g->dk, p.dv = g->dv;
   p.parts = s.parts;
   if (g->dpos) {

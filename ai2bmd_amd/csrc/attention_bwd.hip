@@ -1,6 +1,6 @@
 // Fragment attention, backward (attention.h has the tile; formulas of the forward pass there).
 //
-//   P = exp(s - m) / l,  dP_ij = do_i.v_j,  D_i = sum_j P_ij dP_ij,  dS = P (dP - D)
+//   P = 2^(s - m) / l (s in units of log 2),  dP_ij = do_i.v_j,  D_i = sum_j P_ij dP_ij,  dS = P (dP - D)
 //   dq_i = scale sum_j dS k_j      dk_j = scale sum_i dS q_i      dv_j = sum_i P do_i
 //   dslope_a = - sum dS r          dtable[a][b] = sum over the pairs of bucket b
 //   dx_i -= slope dS (x_i - x_j) / r,  dx_j -= the opposite; summed over heads
@@ -53,12 +53,12 @@ __global__ __launch_bounds__(256) void k_attn_bwd_q(AttnParams p, size_t lds_per
   const int kv = head / (p.heads / p.kv_heads);
   const T* kp = (const T*)p.k + kv * p.k_head;
   const T* vp = (const T*)p.v + kv * p.v_head;
-  const float slope = p.slope ? p.slope[head] : 0.f;
+  const float slope = p.slope ? p.slope[head] : 0.f, slope2 = slope * kLog2e, scale = p.scale * kLog2e;
   if (p.table)
-    for (int i = tid; i < p.n_rel; i += THREADS) lds.tab[i] = p.table[(int64_t)head * p.n_buckets + p.lut[i]];
+    for (int i = tid; i < p.n_rel; i += THREADS) lds.tab[i] = table_log2(p.table[(int64_t)head * p.n_buckets + p.lut[i]]);
   if (count)
     for (int i = lane; i < p.n_rel; i += 64) hist[i] = 0.f;
-  float dslope = 0.f, low = 0.f, high = 0.f;  // low, high: the two clipped ends of the table, per lane
+  LongSum dslope, low, high;  // low, high: the two clipped ends of the table
 
   for (int item = worker; item < p.count; item += p.workers) {
     const AttnWork w = p.work[item];
@@ -78,8 +78,8 @@ __global__ __launch_bounds__(256) void k_attn_bwd_q(AttnParams p, size_t lds_per
     }
     const float2 ml = p.stats[head * p.rows_q + row];
     const float ref = ml.x == -INFINITY ? 0.f : ml.x;
-    const float inv_l = ml.y == 0.f ? 0.f : 1.f / ml.y;
-    float px = 0, py = 0, pz = 0, gx = 0, gy = 0, gz = 0;
+    float px = 0, py = 0, pz = 0;
+    LongSum gx, gy, gz;
     if (p.slope) px = p.q_pos[3 * row], py = p.q_pos[3 * row + 1], pz = p.q_pos[3 * row + 2];
     const int res = p.table ? p.q_res[row] : 0;
 
@@ -92,7 +92,8 @@ __global__ __launch_bounds__(256) void k_attn_bwd_q(AttnParams p, size_t lds_per
     constexpr bool AHEAD = TilePair<T, DP, THREADS>::N <= 8;
     if (AHEAD && w.row0 < w.row1)
       tiles.load(kp + w.row0 * p.k_row, p.k_row, vp + w.row0 * p.v_row, p.v_row, w.row1 - w.row0, p.dim, tid);
-    float delta = 0.f;
+    float delta = 0.f, inv_l = 0.f;
+    LongSum sum_e, sum_edp;
     const bool once = w.row1 - w.row0 <= kTile;
     bool sum_delta = true;  // the walk for D (with `once`: that tile itself)
     for (int k0 = w.row0; k0 < w.row1;) {
@@ -122,13 +123,13 @@ __global__ __launch_bounds__(256) void k_attn_bwd_q(AttnParams p, size_t lds_per
         }
       float s[16];
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = acc[r] * p.scale;
+      for (int r = 0; r < 16; ++r) s[r] = acc[r] * scale;
       if (p.slope) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const float4 k = lds.pos[acc_row(r, hi)];
           float inv;
-          s[r] -= slope * pair_dist(px - k.x, py - k.y, pz - k.z, inv);
+          s[r] -= slope2 * pair_dist(px - k.x, py - k.y, pz - k.z, inv);
         }
       }
       if (p.table) {
@@ -141,31 +142,42 @@ __global__ __launch_bounds__(256) void k_attn_bwd_q(AttnParams p, size_t lds_per
         for (int r = 0; r < 16; ++r) s[r] = acc_row(r, hi) < limit ? s[r] : -INFINITY;
       }
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f((s[r] - ref) * kLog2e) * inv_l;
+      for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(s[r] - ref);
       if (first) {
+        // the sum of exponentials once more, from the very values that D is summed from: then sum_j dS_ij is 0
+        float t[16];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) delta += s[r] * dp[r];
-        if (once || !sum_delta) delta += other_half(delta);
+        for (int r = 0; r < 16; ++r) t[r] = s[r] * dp[r];
+        sum_e.add(tile_sum(s));
+        sum_edp.add(tile_sum(t));
+        if (once || !sum_delta) {
+          const float l = sum_e.both_halves();
+          inv_l = l == 0.f ? 0.f : 1.f / l;
+          delta = sum_edp.both_halves() * inv_l;
+        }
         if (!once) continue;
       }
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] *= dp[r] - delta;  // dS from here on
+      for (int r = 0; r < 16; ++r) s[r] *= inv_l * (dp[r] - delta);  // dS from here on
 
       if (p.slope) {
+        float ts = 0.f, tx = 0.f, ty = 0.f, tz = 0.f;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const float4 k = lds.pos[acc_row(r, hi)];
           const float dx = px - k.x, dy = py - k.y, dz = pz - k.z;
           float inv;
           const float far = pair_dist(dx, dy, dz, inv);
-          dslope -= s[r] * far;
+          ts -= s[r] * far;
           const float pull = s[r] * inv;
-          gx += pull * dx, gy += pull * dy, gz += pull * dz;
+          tx += pull * dx, ty += pull * dy, tz += pull * dz;
         }
+        dslope.add(ts);
+        gx.add(tx), gy.add(ty), gz.add(tz);
       }
       if (count) {
         // runs of keys of one residue are added up in the lane first; the clipped ends stay in the lane altogether
-        float run = 0.f;
+        float run = 0.f, first_end = 0.f, last_end = 0.f;
         int at = rel_index(lds.res[acc_row(0, hi)], res, p.reach);
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
@@ -173,15 +185,17 @@ __global__ __launch_bounds__(256) void k_attn_bwd_q(AttnParams p, size_t lds_per
           const int then = r < 15 ? rel_index(lds.res[acc_row(r < 15 ? r + 1 : 15, hi)], res, p.reach) : -1;
           if (then != at) {
             if (at == 0)
-              low += run;
+              first_end += run;
             else if (at == 2 * p.reach)
-              high += run;
+              last_end += run;
             else
               __hip_atomic_fetch_add(hist + at, run, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
             run = 0.f;
           }
           at = then;
         }
+        low.add(first_end);
+        high.add(last_end);
       }
       if constexpr (HALF) {
         float largest = 0.f;
@@ -201,19 +215,18 @@ __global__ __launch_bounds__(256) void k_attn_bwd_q(AttnParams p, size_t lds_per
 #pragma unroll
       for (int d = 0; d < DP / 32; ++d) {
         if (d * 32 >= p.dim) continue;
-        dq[d] = Mma<T>::run(load_t<T, DP>(lds.a, 0, d * 32, lane, hi), s0, dq[d]);
-        dq[d] = Mma<T>::run(load_t<T, DP>(lds.a, 1, d * 32, lane, hi), s1, dq[d]);
+        tile_mma<T>(dq[d], load_t<T, DP>(lds.a, 0, d * 32, lane, hi), s0, load_t<T, DP>(lds.a, 1, d * 32, lane, hi), s1);
       }
     }
 
     if (p.part_pos_q) {
-      gx += other_half(gx), gy += other_half(gy), gz += other_half(gz);
+      const float x = gx.both_halves(), y = gy.both_halves(), z = gz.both_halves();
       if (live && hi == 0) {
         float* g = p.part_pos_q + (head * p.rows_q + row) * 3;
-        g[0] = -slope * gx, g[1] = -slope * gy, g[2] = -slope * gz;
+        g[0] = -slope * x, g[1] = -slope * y, g[2] = -slope * z;
       }
     }
-    if (live && hi == 0) p.delta[head * p.rows_q + row] = delta;
+    if (live && hi == 0) p.delta[head * p.rows_q + row] = make_float2(delta, inv_l);
     if (live) {
       const float f = HALF ? p.scale / cs.f : p.scale;
       T* o = (T*)p.dq + (row * p.heads + head) * p.dim;
@@ -229,23 +242,22 @@ __global__ __launch_bounds__(256) void k_attn_bwd_q(AttnParams p, size_t lds_per
 
   const int64_t part = p.part0 + worker;
   if (p.part_slope) {
-    dslope = wave_sum(dslope);
+    const float sum = wave_sum(dslope.value());
     if (lane == 0) {
       float* out = p.part_slope + (head * (int64_t)p.parts + part) * kCoopWaves;
       if (COOP) {
-        out[wave] = dslope;
+        out[wave] = sum;
       } else {
-        out[0] = dslope;
+        out[0] = sum;
         out[1] = out[2] = out[3] = 0.f;
       }
     }
   }
   if (count) {
-    low = wave_sum(low);
-    high = wave_sum(high);
+    const float first_end = wave_sum(low.value()), last_end = wave_sum(high.value());
     if (lane == 0) {
-      hist[0] += low;
-      hist[2 * p.reach] += high;
+      hist[0] += first_end;
+      hist[2 * p.reach] += last_end;
     }
     tile_sync<COOP>();
     for (int i = tid; i < p.n_rel; i += THREADS) {
@@ -285,7 +297,8 @@ __global__ __launch_bounds__(256) void k_attn_bwd_k(AttnParams p, size_t lds_per
     kf[c] = load_col<T>(kp, c * 16 + hi * 8, p.dim, live);
     vf[c] = load_col<T>(vp, c * 16 + hi * 8, p.dim, live);
   }
-  float px = 0, py = 0, pz = 0, gx = 0, gy = 0, gz = 0;
+  float px = 0, py = 0, pz = 0;
+  LongSum gx, gy, gz;
   if (p.slope) px = p.k_pos[3 * row], py = p.k_pos[3 * row + 1], pz = p.k_pos[3 * row + 2];
   const int res = p.table ? p.k_res[row] : 0;
 
@@ -293,16 +306,17 @@ __global__ __launch_bounds__(256) void k_attn_bwd_k(AttnParams p, size_t lds_per
 #pragma unroll
   for (int d = 0; d < DP / 32; ++d) dk[d] = acc_zero(), dv[d] = acc_zero();
   ColumnScale cs;
+  const float scale = p.scale * kLog2e;
   constexpr float PUP = HALF ? 0x1p14f : 1.f;
 
   for (int sub = 0; sub < share; ++sub) {
     const int head = kv * share + sub;
     const T* qp = (const T*)p.q + head * p.q_head;
     const T* dp_ = (const T*)p.dout + head * p.do_head;
-    const float slope = p.slope ? p.slope[head] : 0.f;
+    const float slope = p.slope ? p.slope[head] : 0.f, slope2 = slope * kLog2e;
     if (p.table) {
       tile_sync<COOP>();
-      for (int i = tid; i < p.n_rel; i += THREADS) lds.tab[i] = p.table[(int64_t)head * p.n_buckets + p.lut[i]];
+      for (int i = tid; i < p.n_rel; i += THREADS) lds.tab[i] = table_log2(p.table[(int64_t)head * p.n_buckets + p.lut[i]]);
     }
     TilePair<T, DP, THREADS> tiles;
     constexpr bool AHEAD = TilePair<T, DP, THREADS>::N <= 8;
@@ -317,9 +331,9 @@ __global__ __launch_bounds__(256) void k_attn_bwd_k(AttnParams p, size_t lds_per
         const int64_t qr = q0 + (tid < n ? tid : 0);
         if (p.slope) lds.pos[tid] = make_float4(p.q_pos[3 * qr], p.q_pos[3 * qr + 1], p.q_pos[3 * qr + 2], 0.f);
         if (p.table) lds.res[tid] = p.q_res[qr];
-        const float2 ml = p.stats[head * p.rows_q + qr];
-        lds.stat[tid] = make_float4(ml.x == -INFINITY ? 0.f : ml.x, ml.y == 0.f ? 0.f : 1.f / ml.y,
-                                    p.delta[head * p.rows_q + qr], 0.f);
+        const float top = p.stats[head * p.rows_q + qr].x;
+        const float2 d = p.delta[head * p.rows_q + qr];
+        lds.stat[tid] = make_float4(top == -INFINITY ? 0.f : top, d.y, d.x, 0.f);
       }
       tile_sync<COOP>();
       const int next = q0 + kTile;
@@ -336,13 +350,13 @@ __global__ __launch_bounds__(256) void k_attn_bwd_k(AttnParams p, size_t lds_per
         }
       float s[16];
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = acc[r] * p.scale;
+      for (int r = 0; r < 16; ++r) s[r] = acc[r] * scale;
       if (p.slope) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const float4 q = lds.pos[acc_row(r, hi)];
           float inv;
-          s[r] -= slope * pair_dist(q.x - px, q.y - py, q.z - pz, inv);
+          s[r] -= slope2 * pair_dist(q.x - px, q.y - py, q.z - pz, inv);
         }
       }
       if (p.table) {
@@ -358,11 +372,12 @@ __global__ __launch_bounds__(256) void k_attn_bwd_k(AttnParams p, size_t lds_per
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const float4 st = lds.stat[acc_row(r, hi)];
-        const float e = __builtin_amdgcn_exp2f((s[r] - st.x) * kLog2e) * st.y;
+        const float e = __builtin_amdgcn_exp2f(s[r] - st.x) * st.y;
         s[r] = e * (dp[r] - st.z);  // dS from here on
         pr[r] = e * PUP;
       }
       if (p.part_pos_k) {
+        float tx = 0.f, ty = 0.f, tz = 0.f;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const float4 q = lds.pos[acc_row(r, hi)];
@@ -370,8 +385,9 @@ __global__ __launch_bounds__(256) void k_attn_bwd_k(AttnParams p, size_t lds_per
           float inv;
           pair_dist(dx, dy, dz, inv);
           const float pull = slope * s[r] * inv;
-          gx += pull * dx, gy += pull * dy, gz += pull * dz;
+          tx += pull * dx, ty += pull * dy, tz += pull * dz;
         }
+        gx.add(tx), gy.add(ty), gz.add(tz);
       }
       if constexpr (HALF) {
         float largest = 0.f;
@@ -391,19 +407,17 @@ __global__ __launch_bounds__(256) void k_attn_bwd_k(AttnParams p, size_t lds_per
 #pragma unroll
       for (int d = 0; d < DP / 32; ++d) {
         if (d * 32 >= p.dim) continue;
-        dv[d] = Mma<T>::run(load_t<T, DP>(lds.b, 0, d * 32, lane, hi), p0, dv[d]);
-        dv[d] = Mma<T>::run(load_t<T, DP>(lds.b, 1, d * 32, lane, hi), p1, dv[d]);
-        dk[d] = Mma<T>::run(load_t<T, DP>(lds.a, 0, d * 32, lane, hi), s0, dk[d]);
-        dk[d] = Mma<T>::run(load_t<T, DP>(lds.a, 1, d * 32, lane, hi), s1, dk[d]);
+        tile_mma<T>(dv[d], load_t<T, DP>(lds.b, 0, d * 32, lane, hi), p0, load_t<T, DP>(lds.b, 1, d * 32, lane, hi), p1);
+        tile_mma<T>(dk[d], load_t<T, DP>(lds.a, 0, d * 32, lane, hi), s0, load_t<T, DP>(lds.a, 1, d * 32, lane, hi), s1);
       }
     }
   }
 
   if (p.part_pos_k) {
-    gx += other_half(gx), gy += other_half(gy), gz += other_half(gz);
+    const float x = gx.both_halves(), y = gy.both_halves(), z = gz.both_halves();
     if (live && hi == 0) {
       float* g = p.part_pos_k + (kv * p.rows_k + row) * 3;
-      g[0] = gx, g[1] = gy, g[2] = gz;
+      g[0] = x, g[1] = y, g[2] = z;
     }
   }
   if (!live) return;

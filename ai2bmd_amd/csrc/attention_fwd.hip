@@ -34,21 +34,23 @@ __global__ __launch_bounds__(256) void k_attn_fwd(AttnParams p, size_t lds_per_w
   const T* qp = (const T*)p.q + row * p.q_row + head * p.q_head;
 #pragma unroll
   for (int c = 0; c < DP / 16; ++c) qf[c] = load_col<T>(qp, c * 16 + hi * 8, p.dim, live);
+  const float scale = p.scale * kLog2e;
   float px = 0, py = 0, pz = 0, slope = 0;
   if (p.slope) {
-    slope = p.slope[head];
+    slope = p.slope[head] * kLog2e;
     px = p.q_pos[3 * row], py = p.q_pos[3 * row + 1], pz = p.q_pos[3 * row + 2];
   }
   int res = 0;
   if (p.table) {
     res = p.q_res[row];
-    for (int i = tid; i < p.n_rel; i += THREADS) lds.tab[i] = p.table[(int64_t)head * p.n_buckets + p.lut[i]];
+    for (int i = tid; i < p.n_rel; i += THREADS) lds.tab[i] = table_log2(p.table[(int64_t)head * p.n_buckets + p.lut[i]]);
   }
 
   f32x16 o[DP / 32];
 #pragma unroll
   for (int d = 0; d < DP / 32; ++d) o[d] = acc_zero();
-  float m = -INFINITY, l = 0.f;  // l: this half's share
+  float m = -INFINITY;
+  LongSum l;  // this half's share
 
   TilePair<T, DP, THREADS> tiles;
   constexpr bool AHEAD = TilePair<T, DP, THREADS>::N <= 8;
@@ -76,7 +78,7 @@ __global__ __launch_bounds__(256) void k_attn_fwd(AttnParams p, size_t lds_per_w
       if (c * 16 < p.dim) acc = Mma<T>::run(load_n<T, DP>(lds.a, c, col, hi), qf[c], acc);
     float s[16];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = acc[r] * p.scale;
+    for (int r = 0; r < 16; ++r) s[r] = acc[r] * scale;
     if (p.slope) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
@@ -100,15 +102,12 @@ __global__ __launch_bounds__(256) void k_attn_fwd(AttnParams p, size_t lds_per_w
     top = fmaxf(m, fmaxf(top, other_half(top)));
     // a row whose scores are all -inf so far keeps the maximum -inf and adds nothing
     const float ref = top == -INFINITY ? 0.f : top;
-    const float fade = __builtin_amdgcn_exp2f((m - ref) * kLog2e);
+    const float fade = __builtin_amdgcn_exp2f(m - ref);
     m = top;
-    l *= fade;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      // (difference first: the scores may be as large as the type allows, their difference decides)
-      s[r] = __builtin_amdgcn_exp2f((s[r] - ref) * kLog2e);
-      l += s[r];
-    }
+    for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(s[r] - ref);
+    l.scale(fade);
+    l.add(tile_sum(s));
     if (__any(fade != 1.f)) {
 #pragma unroll
       for (int d = 0; d < DP / 32; ++d)
@@ -119,16 +118,15 @@ __global__ __launch_bounds__(256) void k_attn_fwd(AttnParams p, size_t lds_per_w
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d) {
       if (d * 32 >= p.dim) continue;
-      o[d] = Mma<T>::run(load_t<T, DP>(lds.b, 0, d * 32, lane, hi), p0, o[d]);
-      o[d] = Mma<T>::run(load_t<T, DP>(lds.b, 1, d * 32, lane, hi), p1, o[d]);
+      tile_mma<T>(o[d], load_t<T, DP>(lds.b, 0, d * 32, lane, hi), p0, load_t<T, DP>(lds.b, 1, d * 32, lane, hi), p1);
     }
   }
 
-  l += other_half(l);
+  const float total = l.both_halves();
   if (!live) return;
   if (w.slot >= 0) {
     const int64_t at = ((int64_t)w.slot * p.heads + head) * kTile + col;
-    if (hi == 0) p.part_ml[at] = make_float2(m, l);
+    if (hi == 0) p.part_ml[at] = make_float2(m, total);
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
@@ -138,8 +136,8 @@ __global__ __launch_bounds__(256) void k_attn_fwd(AttnParams p, size_t lds_per_w
       }
     return;
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  if (hi == 0 && p.stats) p.stats[head * p.rows_q + row] = make_float2(m, l);
+  const float inv = total == 0.f ? 0.f : 1.f / total;
+  if (hi == 0 && p.stats) p.stats[head * p.rows_q + row] = make_float2(m, total);
   T* op = (T*)p.out + row * p.out_row + head * p.out_head;
 #pragma unroll
   for (int d = 0; d < DP / 32; ++d)
@@ -171,7 +169,7 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnParams p) {
   float l = 0.f;
   for (int s = tid; s < j.slots; s += 256) {
     const float2 ml = p.part_ml[((int64_t)(j.slot0 + s) * p.heads + head) * kTile + col];
-    weight[s] = __builtin_amdgcn_exp2f((ml.x - ref) * kLog2e);
+    weight[s] = __builtin_amdgcn_exp2f(ml.x - ref);
     l += weight[s] * ml.y;
   }
   l = wave_sum(l);

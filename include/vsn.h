@@ -328,7 +328,7 @@ int vsn_layernorm_backward(int device_id, int dtype, int param_dtype, const void
  *     strides (elements) of rows and heads multiples of 16 bytes, addresses too.  rows_* may exceed the plan's: rows
  *     behind the last fragment are neither read nor written.  q_pos / k_pos f32 [rows][3] and slope f32 [heads]: all
  *     or none.  q_res / k_res i32 [rows] and table f32 [heads][n_buckets]: all or none.  stats f32
- *     [heads][rows_q][2] (maximum, sum of exponentials) is all that a backward call needs of the forward one (NULL in a
+ *     [heads][rows_q][2] (maximum in units of log 2, sum of exponentials) is all that a backward call needs of the forward one (NULL in a
  *     forward call: not wanted); `out` is not read by a backward call.
  *   vsn_attn_grads   dout as out; dq, dk, dv dense.  dpos f32 [rows_k][3]: of both ends of a pair where dquery_pos is
  *     NULL (queries = keys), else of the keys' positions, and dquery_pos f32 [rows_q][3] of the queries'.  dpos, dslope
