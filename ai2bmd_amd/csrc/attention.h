@@ -63,7 +63,6 @@ struct AttnParams {
   float* part_slope;      // [heads][4 parts] or null
   float* part_hist;       // [heads][n_rel][parts] or null
   float *dpos, *dq_pos, *dslope, *dtable;
-  int64_t used_q, used_k; // rows that belong to fragments
 };
 
 template <typename T>

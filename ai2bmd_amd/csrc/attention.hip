@@ -7,10 +7,10 @@
 
 struct vsn_attn {
   struct Side {
-    vsn::AttnWork *lone_work = nullptr, *coop_work = nullptr;
+    vsn::AttnWork *small_work = nullptr, *lone_work = nullptr, *coop_work = nullptr;
     vsn::AttnJoin* join = nullptr;
-    int lone = 0, coop = 0, joins = 0, slots = 0;
-    vsn::AttnPlanView view() const { return {lone_work, coop_work, lone, coop, join, joins}; }
+    int small = 0, lone = 0, coop = 0, joins = 0, slots = 0;
+    vsn::AttnPlanView view() const { return {small_work, lone_work, coop_work, small, lone, coop, join, joins}; }
   };
   int device = 0, heads = 0, kv_heads = 0, dim = 0, reach = 0, n_rel = 0, n_buckets = 0;
   int64_t used_q = 0, used_k = 0;
@@ -31,14 +31,16 @@ constexpr int64_t kCoopMin = 256;
 constexpr int64_t kSplitBelow = 1024, kSplitWaves = 2048;
 constexpr int kSplitTiles = 16;
 
+constexpr int kSmallSums = 4096;  // floats of table and slope sums per wave
+
 struct Lists {
-  std::vector<AttnWork> lone, coop;
+  std::vector<AttnWork> small, lone, coop;
   std::vector<AttnJoin> join;
   int slots = 0;
 };
 
 Lists make_lists(int64_t n, const int64_t* col_start, const int64_t* col_end, const int64_t* row_start,
-                 const int64_t* row_end, int heads, bool split) {
+                 const int64_t* row_end, int heads, bool small, bool split) {
   Lists out;
   int64_t groups = 0;
   for (int64_t f = 0; f < n; ++f) {
@@ -49,6 +51,14 @@ Lists make_lists(int64_t n, const int64_t* col_start, const int64_t* col_end, co
   int64_t tiles = 0;
   for (int64_t f = 0; f < n; ++f) {
     const int64_t cols = col_end[f] - col_start[f], rows = row_end[f] - row_start[f];
+    if (small && cols <= kTile && rows <= kTile) {
+      if (cols + rows) {
+        AttnWork w = {};
+        w.col0 = (int)col_start[f], w.cols = (int)cols, w.row0 = (int)row_start[f], w.row1 = (int)row_end[f], w.slot = -1;
+        out.small.push_back(w);
+      }
+      continue;
+    }
     const bool coop = share && cols > 2 * kTile;
     const int64_t step = coop ? kCoopCols : kTile;
     for (int64_t c = 0; c < cols; c += step) {
@@ -96,11 +106,12 @@ bool upload(const std::vector<E>& v, E** dev) {
 }
 
 bool upload_side(const Lists& l, vsn_attn::Side& s) {
-  s.lone = (int)l.lone.size(), s.coop = (int)l.coop.size(), s.joins = (int)l.join.size(), s.slots = l.slots;
-  return upload(l.lone, &s.lone_work) && upload(l.coop, &s.coop_work) && upload(l.join, &s.join);
+  s.small = (int)l.small.size(), s.lone = (int)l.lone.size(), s.coop = (int)l.coop.size(), s.joins = (int)l.join.size(), s.slots = l.slots;
+  return upload(l.small, &s.small_work) && upload(l.lone, &s.lone_work) && upload(l.coop, &s.coop_work) && upload(l.join, &s.join);
 }
 
 void free_side(vsn_attn::Side& s) {
+  hipFree(s.small_work);
   hipFree(s.lone_work);
   hipFree(s.coop_work);
   hipFree(s.join);
@@ -132,14 +143,16 @@ struct Workspace {
 
 struct BackwardSpace {
   int64_t delta, pos_q, pos_k, slope, hist, size;
-  int lone, coop, parts;
+  AttnWorkers workers;
+  int parts;
 };
 
 BackwardSpace backward_space(const vsn_attn& a, int64_t rows_q, int64_t rows_k) {
   BackwardSpace s;
-  s.lone = workers(a.by_query.lone, a.heads, a.n_rel, 8192);
-  s.coop = workers(a.by_query.coop, a.heads, a.n_rel, 2048);
-  s.parts = s.lone + s.coop;
+  s.workers.lone = workers(a.by_query.lone, a.heads, a.n_rel, 8192);
+  s.workers.coop = workers(a.by_query.coop, a.heads, a.n_rel, 2048);
+  s.workers.small = workers(a.by_query.small, 1, a.n_rel * a.heads, 4096);
+  s.parts = s.workers.lone + s.workers.coop + s.workers.small;
   Workspace w;
   s.delta = w.take(rows_q * a.heads * 8);
   s.pos_q = w.take(rows_q * a.heads * 12);
@@ -199,7 +212,6 @@ AttnParams params(const vsn_attn& a, const vsn_attn_io& io) {
   p.rows_q = io.rows_q, p.rows_k = io.rows_k;
   p.out = io.out, p.out_row = io.out_row, p.out_head = io.out_head;
   p.stats = (float2*)io.stats;
-  p.used_q = a.used_q, p.used_k = a.used_k;
   return p;
 }
 
@@ -238,9 +250,11 @@ extern "C" int vsn_attn_create(vsn_attn_handle* out, int device_id, int64_t n, c
       a->reach = reach, a->n_rel = 2 * reach + 1, a->n_buckets = n_buckets;
       lut.assign(host_buckets, host_buckets + a->n_rel);
     }
-    ok = upload_side(make_lists(n, qs, qe, host_start, host_end, heads, true), a->fwd) &&
-         upload_side(make_lists(n, qs, qe, host_start, host_end, heads, false), a->by_query) &&
-         upload_side(make_lists(n, host_start, host_end, qs, qe, kv_heads, false), a->by_key) &&
+    // one-tile fragments go by a kernel of their own where a wave's per-head sums fit its share of LDS
+    const bool small = (int64_t)heads * (a->n_rel + 64) <= kSmallSums;
+    ok = upload_side(make_lists(n, qs, qe, host_start, host_end, heads, small, true), a->fwd) &&
+         upload_side(make_lists(n, qs, qe, host_start, host_end, heads, small, false), a->by_query) &&
+         upload_side(make_lists(n, host_start, host_end, qs, qe, kv_heads, small, false), a->by_key) &&
          upload(lut, &a->lut);
   } catch (...) {  // out of host memory
     ok = false;
@@ -316,5 +330,5 @@ extern "C" int vsn_attn_backward(vsn_attn_handle a, const vsn_attn_io* io, const
   if (g->dslope) p.part_slope = (float*)(base + s.slope);
   if (g->dtable) p.part_hist = (float*)(base + s.hist);
   p.dpos = g->dpos, p.dq_pos = g->dquery_pos, p.dslope = g->dslope, p.dtable = g->dtable;
-  return attn_backward(io->dtype, a->by_query.view(), a->by_key.view(), p, s.lone, s.coop, (hipStream_t)stream);
+  return attn_backward(io->dtype, a->by_query.view(), a->by_key.view(), p, s.workers, (hipStream_t)stream);
 }

@@ -436,37 +436,51 @@ __global__ __launch_bounds__(256) void k_attn_bwd_k(AttnParams p, size_t lds_per
     }
 }
 
-// Joins the partial sums in a fixed order: positions over heads (workgroups 0 ... n_pos - 1, one thread per component),
-// then one workgroup per head for its slope and one per (head, bucket) for the table, both summed in float64.
-__global__ __launch_bounds__(256) void k_attn_bwd_join(AttnParams p, int n_pos, int n_slope) {
-  const int b = blockIdx.x, tid = threadIdx.x;
-  if (b < n_pos) {
-    const int64_t at = (int64_t)b * 256 + tid;
-    if (at < p.used_k * 3 && p.dpos) {
-      float t = 0.f;
-      for (int h = 0; h < p.kv_heads; ++h) t += p.part_pos_k[h * p.rows_k * 3 + at];
-      if (!p.dq_pos)
-        for (int h = 0; h < p.heads; ++h) t += p.part_pos_q[h * p.rows_q * 3 + at];
-      p.dpos[at] = t;
+// Joins the partial sums in a fixed order: positions over heads (a workgroup per work item of the segments), then one
+// workgroup per head for its slope and one per (head, bucket) for the table, both summed in float64.
+struct AttnPosSegment {
+  const AttnWork* work;
+  int count;
+  int of_rows;           // the item's rows (1) or its columns (0)
+  int parts_q, parts_k;  // partial sums of each side that make up the result
+  float* out;
+};
+struct AttnPosJoin {
+  AttnPosSegment seg[6];
+  int n;
+};
+
+__global__ __launch_bounds__(256) void k_attn_bwd_join(AttnParams p, AttnPosJoin join, int n_slope) {
+  int b = blockIdx.x;
+  const int tid = threadIdx.x;
+  for (int i = 0; i < join.n; ++i) {
+    const AttnPosSegment g = join.seg[i];
+    if (b < g.count) {
+      const AttnWork w = g.work[b];
+      const int64_t first = g.of_rows ? w.row0 : w.col0, n = g.of_rows ? w.row1 - w.row0 : w.cols;
+      for (int64_t at = first * 3 + tid; at < (first + n) * 3; at += 256) {
+        float t = 0.f;
+        for (int h = 0; h < g.parts_k; ++h) t += p.part_pos_k[h * p.rows_k * 3 + at];
+        for (int h = 0; h < g.parts_q; ++h) t += p.part_pos_q[h * p.rows_q * 3 + at];
+        g.out[at] = t;
+      }
+      return;
     }
-    if (at < p.used_q * 3 && p.dq_pos) {
-      float t = 0.f;
-      for (int h = 0; h < p.heads; ++h) t += p.part_pos_q[h * p.rows_q * 3 + at];
-      p.dq_pos[at] = t;
-    }
-    return;
+    b -= g.count;
   }
   __shared__ double red[4];
+  __shared__ int lut[2 * kMaxReach + 1];
   double t = 0.0;
   float* out;
-  if (b < n_pos + n_slope) {
-    const int head = b - n_pos;
-    for (int i = tid; i < p.parts * kCoopWaves; i += 256) t += p.part_slope[(int64_t)head * p.parts * kCoopWaves + i];
-    out = p.dslope + head;
+  if (b < n_slope) {
+    for (int i = tid; i < p.parts * kCoopWaves; i += 256) t += p.part_slope[(int64_t)b * p.parts * kCoopWaves + i];
+    out = p.dslope + b;
   } else {
-    const int at = b - n_pos - n_slope, head = at / p.n_buckets, bucket = at % p.n_buckets;
+    const int at = b - n_slope, head = at / p.n_buckets, bucket = at % p.n_buckets;
+    for (int i = tid; i < p.n_rel; i += 256) lut[i] = p.lut[i];
+    __syncthreads();
     for (int rel = 0; rel < p.n_rel; ++rel)
-      if (p.lut[rel] == bucket)
+      if (lut[rel] == bucket)
         for (int i = tid; i < p.parts; i += 256) t += p.part_hist[((int64_t)head * p.n_rel + rel) * p.parts + i];
     out = p.dtable + at;
   }
@@ -511,11 +525,32 @@ static int bwd_launch(const AttnPlanView& by_query, const AttnPlanView& by_key, 
     hipLaunchKernelGGL((k_attn_bwd_k<T, DP, true>), dim3((unsigned)((int64_t)by_key.coop * p.kv_heads)),
                        dim3(64 * kCoopWaves), tab, st, p, tab);
   }
-  const int64_t rows = p.used_k > p.used_q ? p.used_k : p.used_q;
-  const int n_pos = p.dpos || p.dq_pos ? (int)((rows * 3 + 255) / 256) : 0;
+  return 0;
+}
+
+static int join_launch(const AttnPlanView& by_query, const AttnPlanView& by_key, const AttnParams& p, int groups,
+                       hipStream_t st) {
+  AttnPosJoin join = {};
+  int64_t blocks = 0;
+  auto add = [&](const AttnWork* work, int count, int of_rows, int parts_q, int parts_k, float* out) {
+    if (!count) return;
+    join.seg[join.n++] = {work, count, of_rows, parts_q, parts_k, out};
+    blocks += count;
+  };
+  if (p.dpos) {
+    const bool self = !p.dq_pos;
+    add(by_key.lone_work, by_key.lone, 0, self ? p.heads : 0, p.kv_heads, p.dpos);
+    add(by_key.coop_work, by_key.coop, 0, self ? p.heads : 0, p.kv_heads, p.dpos);
+    if (groups > 1) add(by_query.small_work, by_query.small, 1, self ? groups : 0, groups, p.dpos);
+    if (!self) {
+      add(by_query.lone_work, by_query.lone, 0, p.heads, 0, p.dq_pos);
+      add(by_query.coop_work, by_query.coop, 0, p.heads, 0, p.dq_pos);
+      if (groups > 1) add(by_query.small_work, by_query.small, 0, groups, 0, p.dq_pos);
+    }
+  }
   const int n_slope = p.dslope ? p.heads : 0, n_table = p.dtable ? p.heads * p.n_buckets : 0;
-  if (n_pos + n_slope + n_table)
-    hipLaunchKernelGGL(k_attn_bwd_join, dim3(n_pos + n_slope + n_table), dim3(256), 0, st, p, n_pos, n_slope);
+  blocks += n_slope + n_table;
+  if (blocks) hipLaunchKernelGGL(k_attn_bwd_join, dim3((unsigned)blocks), dim3(256), 0, st, p, join, n_slope);
   return hipGetLastError() == hipSuccess ? 0 : -5;
 }
 
@@ -527,12 +562,21 @@ static int bwd_dim(const AttnPlanView& a, const AttnPlanView& b, const AttnParam
 }
 
 int attn_backward(int dtype, const AttnPlanView& by_query, const AttnPlanView& by_key, const AttnParams& p,
-                  int lone_workers, int coop_workers, hipStream_t st) {
+                  const AttnWorkers& n, hipStream_t st) {
+  int rc = 0;
   switch (dtype) {
-    case VSN_F32: return bwd_dim<float>(by_query, by_key, p, lone_workers, coop_workers, st);
-    case VSN_BF16: return bwd_dim<__bf16>(by_query, by_key, p, lone_workers, coop_workers, st);
-    default: return bwd_dim<_Float16>(by_query, by_key, p, lone_workers, coop_workers, st);
+    case VSN_F32: rc = bwd_dim<float>(by_query, by_key, p, n.lone, n.coop, st); break;
+    case VSN_BF16: rc = bwd_dim<__bf16>(by_query, by_key, p, n.lone, n.coop, st); break;
+    default: rc = bwd_dim<_Float16>(by_query, by_key, p, n.lone, n.coop, st); break;
   }
+  const int groups = small_groups(by_query.small, p.kv_heads);
+  if (!rc && by_query.small) {
+    AttnParams small = p;
+    small.work = by_query.small_work, small.count = by_query.small;
+    small.workers = n.small, small.part0 = n.lone + n.coop;
+    rc = attn_small(dtype, small, groups, true, st);
+  }
+  return rc ? rc : join_launch(by_query, by_key, p, groups, st);
 }
 
 }  // namespace vsn

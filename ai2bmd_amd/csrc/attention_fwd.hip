@@ -231,6 +231,12 @@ static int fwd_dim(const AttnPlanView& plan, const AttnParams& p, hipStream_t st
 }
 
 int attn_forward(int dtype, const AttnPlanView& plan, const AttnParams& p, hipStream_t st) {
+  if (plan.small) {
+    AttnParams small = p;
+    small.work = plan.small_work, small.count = plan.small;
+    const int rc = attn_small(dtype, small, small_groups(plan.small, p.kv_heads), false, st);
+    if (rc) return rc;
+  }
   switch (dtype) {
     case VSN_F32: return fwd_dim<float>(plan, p, st);
     case VSN_BF16: return fwd_dim<__bf16>(plan, p, st);

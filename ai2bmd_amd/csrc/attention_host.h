@@ -7,10 +7,11 @@ namespace vsn {
 constexpr int kMaxSlots = 1024;          // partial results of one query block
 constexpr size_t kLdsPerCu = 160 * 1024;
 
-// the work lists of one pass: `lone` items are a wave each with tiles of its own, `coop` items a workgroup of four
+// the work lists of one pass: `small` items are fragments of one tile, `lone` items a wave each with tiles of its own,
+// `coop` items a workgroup of four
 struct AttnPlanView {
-  const AttnWork *lone_work, *coop_work;
-  int lone, coop;
+  const AttnWork *small_work, *lone_work, *coop_work;
+  int small, lone, coop;
   const AttnJoin* join;
   int joins;
 };
@@ -28,9 +29,19 @@ inline bool allow_lds(const void* kernel, size_t bytes) {
          hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) == hipSuccess;
 }
 
+// Waves per small fragment: one that walks all heads, so distances are computed once and positions' gradients need no
+// joining - or, where the fragments alone would leave half of the 1024 SIMDs idle, one per key head.
+inline int small_groups(int items, int kv_heads) { return items >= 512 ? 1 : kv_heads; }
+
+// workers of the backward passes that add up slope and table gradients, per list
+struct AttnWorkers {
+  int lone, coop, small;
+};
+
+int attn_small(int dtype, const AttnParams& p, int groups, bool backward, hipStream_t st);
 int attn_forward(int dtype, const AttnPlanView& plan, const AttnParams& p, hipStream_t st);
-// dq pass (with delta, dslope, dtable and the queries' share of dpos), then the dk / dv pass, then the joins
+// dq pass (with delta, dslope, dtable and the queries' share of dpos), dk / dv pass, small fragments, then the joins
 int attn_backward(int dtype, const AttnPlanView& by_query, const AttnPlanView& by_key, const AttnParams& p,
-                  int lone_workers, int coop_workers, hipStream_t st);
+                  const AttnWorkers& n, hipStream_t st);
 
 }  // namespace vsn
