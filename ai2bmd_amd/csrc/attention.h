@@ -65,6 +65,30 @@ struct AttnParams {
   float *dpos, *dq_pos, *dslope, *dtable;
 };
 
+// A value that is the same for all lanes, in a scalar register (an integer division leaves it in a vector register, and
+// with it every address computed from it).
+__device__ __forceinline__ int uniform(uint32_t v) { return __builtin_amdgcn_readfirstlane((int)v); }
+// Keeps what is computed from `v` inside the loop that uses it.  The compiler otherwise holds every address and comparison
+// that does not change over the loop in a register of its own: a hundred of them, which is a wave or two per SIMD.
+template <typename V>
+__device__ __forceinline__ void compute_here(V& v) {
+  asm volatile("" : "+v"(v));
+}
+__device__ __forceinline__ int here(int v) {
+  compute_here(v);
+  return v;
+}
+
+// A work item in scalar registers: it is the same for all lanes, which the compiler cannot know of a value that it has to
+// load behind the stores of the item before.
+__device__ __forceinline__ AttnWork load_work(const AttnWork* work, int64_t at) {
+  AttnWork w = work[at];
+  w.col0 = __builtin_amdgcn_readfirstlane(w.col0), w.cols = __builtin_amdgcn_readfirstlane(w.cols);
+  w.row0 = __builtin_amdgcn_readfirstlane(w.row0), w.row1 = __builtin_amdgcn_readfirstlane(w.row1);
+  w.slot = __builtin_amdgcn_readfirstlane(w.slot);
+  return w;
+}
+
 template <typename T>
 struct Mma;
 template <>
@@ -120,21 +144,21 @@ struct TilePair {
     for (int i = 0; i < N; ++i) {
       const int c = tid + i * THREADS;
       const bool second = c >= S::CHUNKS;
-      const int rest = second ? c - S::CHUNKS : c;
+      const int rest = c >= 2 * S::CHUNKS ? 0 : second ? c - S::CHUNKS : c;
       const int row = rest / S::CPR, at = rest % S::CPR * S::EPC;
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (row < rows && at < dim && c < 2 * S::CHUNKS)
-        v = *(const uint4*)((second ? b + row * b_row : a + row * a_row) + at);
-      reg[i] = v;
+      // (loads without a branch, from a row and a column that are there; what is beyond the end is zeroed on the way to LDS)
+      const int r = row < rows ? row : 0, e = at < dim ? at : 0;
+      reg[i] = *(const uint4*)((second ? b + r * b_row : a + r * a_row) + e);
     }
   }
-  __device__ __forceinline__ void store(T* a, T* b, int tid) const {
+  __device__ __forceinline__ void store(T* a, T* b, int rows, int dim, int tid) const {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int c = tid + i * THREADS;
       if (c < 2 * S::CHUNKS) {
         const int rest = c >= S::CHUNKS ? c - S::CHUNKS : c;
-        *(uint4*)((c >= S::CHUNKS ? b : a) + rest / S::CPR * S::LD + rest % S::CPR * S::EPC) = reg[i];
+        const int row = rest / S::CPR, at = rest % S::CPR * S::EPC;
+        *(uint4*)((c >= S::CHUNKS ? b : a) + row * S::LD + at) = row < rows && at < dim ? reg[i] : make_uint4(0, 0, 0, 0);
       }
     }
   }
@@ -276,6 +300,14 @@ struct LongSum {
   }
   __device__ __forceinline__ float value() const { return s + c; }
 };
+
+// Waves per SIMD that the tile kernels are compiled for.  16-bit rows of up to 32 columns fit three without spilling
+// (17 882 atoms: dq pass 10.2 -> 8.1 ms, dk / dv pass 5.6 -> 4.3 ms, forward 2.8 -> 2.6 ms; four spill and lose it again);
+// wider or float32 rows are left to the compiler.
+template <typename T, int DP>
+constexpr int tile_waves() {
+  return sizeof(T) == 2 && DP <= 32 ? 3 : 1;
+}
 
 // wave-private (or shared) LDS of one work item
 template <typename T, int DP>

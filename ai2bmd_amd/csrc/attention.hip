@@ -31,7 +31,7 @@ constexpr int64_t kCoopMin = 256;
 constexpr int64_t kSplitBelow = 1024, kSplitWaves = 2048;
 constexpr int kSplitTiles = 16;
 
-constexpr int kSmallSums = 4096;  // floats of table and slope sums per wave
+constexpr int kSmallSums = 4096;  // floats of table sums per wave
 
 struct Lists {
   std::vector<AttnWork> small, lone, coop;
@@ -51,12 +51,10 @@ Lists make_lists(int64_t n, const int64_t* col_start, const int64_t* col_end, co
   int64_t tiles = 0;
   for (int64_t f = 0; f < n; ++f) {
     const int64_t cols = col_end[f] - col_start[f], rows = row_end[f] - row_start[f];
-    if (small && cols <= kTile && rows <= kTile) {
-      if (cols + rows) {
-        AttnWork w = {};
-        w.col0 = (int)col_start[f], w.cols = (int)cols, w.row0 = (int)row_start[f], w.row1 = (int)row_end[f], w.slot = -1;
-        out.small.push_back(w);
-      }
+    if (small && cols && rows && cols <= kTile && rows <= kTile) {
+      AttnWork w = {};
+      w.col0 = (int)col_start[f], w.cols = (int)cols, w.row0 = (int)row_start[f], w.row1 = (int)row_end[f], w.slot = -1;
+      out.small.push_back(w);
       continue;
     }
     const bool coop = share && cols > 2 * kTile;
@@ -251,7 +249,7 @@ extern "C" int vsn_attn_create(vsn_attn_handle* out, int device_id, int64_t n, c
       lut.assign(host_buckets, host_buckets + a->n_rel);
     }
     // one-tile fragments go by a kernel of their own where a wave's per-head sums fit its share of LDS
-    const bool small = (int64_t)heads * (a->n_rel + 64) <= kSmallSums;
+    const bool small = heads <= 64 && (int64_t)heads * a->n_rel <= kSmallSums;
     ok = upload_side(make_lists(n, qs, qe, host_start, host_end, heads, small, true), a->fwd) &&
          upload_side(make_lists(n, qs, qe, host_start, host_end, heads, small, false), a->by_query) &&
          upload_side(make_lists(n, host_start, host_end, qs, qe, kv_heads, small, false), a->by_key) &&

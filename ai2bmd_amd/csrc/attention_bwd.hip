@@ -34,23 +34,23 @@ struct ColumnScale {
 };
 
 template <typename T, int DP, bool COOP>
-__global__ __launch_bounds__(256) void k_attn_bwd_q(AttnParams p, size_t lds_per_wave) {
+__global__ __launch_bounds__(256, (tile_waves<T, DP>())) void k_attn_bwd_q(AttnParams p, size_t lds_per_wave) {
   extern __shared__ __attribute__((aligned(16))) char lds_raw[];
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, lane_of_wave = lane;
   const int col = lane & 31, hi = lane >> 5;
   const int tid = COOP ? threadIdx.x : lane;
   constexpr int THREADS = COOP ? 64 * kCoopWaves : 64;
   constexpr bool HALF = sizeof(T) == 2 && !__is_same(T, __bf16);
-  const int64_t id = COOP ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * (blockDim.x >> 6) + wave;
-  if (id >= (int64_t)p.workers * p.heads) return;
-  const int head = (int)(id % p.heads), worker = (int)(id / p.heads);
+  const uint32_t id = COOP ? blockIdx.x : blockIdx.x * (blockDim.x >> 6) + wave;
+  if (id >= (uint32_t)p.workers * p.heads) return;
+  const int head = uniform(id % p.heads), worker = uniform(id / p.heads);
   char* base = lds_raw + (COOP ? 0 : wave * lds_per_wave);
   const AttnLds<T, DP> lds(base);
   float* hist_all = lds.tab + p.n_rel;  // one histogram per wave
   float* hist = hist_all + (COOP ? wave * p.n_rel : 0);
   const bool count = p.part_hist != nullptr;
 
-  const int kv = head / (p.heads / p.kv_heads);
+  const int kv = uniform(head / (p.heads / p.kv_heads));
   const T* kp = (const T*)p.k + kv * p.k_head;
   const T* vp = (const T*)p.v + kv * p.v_head;
   const float slope = p.slope ? p.slope[head] : 0.f, slope2 = slope * kLog2e, scale = p.scale * kLog2e;
@@ -61,7 +61,7 @@ __global__ __launch_bounds__(256) void k_attn_bwd_q(AttnParams p, size_t lds_per
   LongSum dslope, low, high;  // low, high: the two clipped ends of the table
 
   for (int item = worker; item < p.count; item += p.workers) {
-    const AttnWork w = p.work[item];
+    const AttnWork w = load_work(p.work, item);
     const int mine = (COOP ? wave * kTile : 0) + col;
     const bool live = mine < w.cols;
     const bool busy = (COOP ? wave * kTile : 0) < w.cols;
@@ -100,7 +100,7 @@ __global__ __launch_bounds__(256) void k_attn_bwd_q(AttnParams p, size_t lds_per
       const int n = w.row1 - k0 < kTile ? w.row1 - k0 : kTile;
       if (!AHEAD) tiles.load(kp + k0 * p.k_row, p.k_row, vp + k0 * p.v_row, p.v_row, n, p.dim, tid);
       tile_sync<COOP>();
-      tiles.store(lds.a, lds.b, tid);
+      tiles.store(lds.a, lds.b, n, p.dim, tid);
       if (tid < kTile) {
         const int64_t kr = k0 + (tid < n ? tid : 0);
         if (p.slope) lds.pos[tid] = make_float4(p.k_pos[3 * kr], p.k_pos[3 * kr + 1], p.k_pos[3 * kr + 2], 0.f);
@@ -114,6 +114,7 @@ __global__ __launch_bounds__(256) void k_attn_bwd_q(AttnParams p, size_t lds_per
         tiles.load(kp + k0 * p.k_row, p.k_row, vp + k0 * p.v_row, p.v_row, w.row1 - k0, p.dim, tid);
       if (!busy) continue;
 
+      const int lane = here(lane_of_wave), col = lane & 31, hi = lane >> 5;
       f32x16 acc = acc_zero(), dp = acc_zero();
 #pragma unroll
       for (int c = 0; c < DP / 16; ++c)
@@ -270,17 +271,17 @@ __global__ __launch_bounds__(256) void k_attn_bwd_q(AttnParams p, size_t lds_per
 }
 
 template <typename T, int DP, bool COOP>
-__global__ __launch_bounds__(256) void k_attn_bwd_k(AttnParams p, size_t lds_per_wave) {
+__global__ __launch_bounds__(256, (tile_waves<T, DP>())) void k_attn_bwd_k(AttnParams p, size_t lds_per_wave) {
   extern __shared__ __attribute__((aligned(16))) char lds_raw[];
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, lane_of_wave = lane;
   const int col = lane & 31, hi = lane >> 5;
   const int tid = COOP ? threadIdx.x : lane;
   constexpr int THREADS = COOP ? 64 * kCoopWaves : 64;
   constexpr bool HALF = sizeof(T) == 2 && !__is_same(T, __bf16);
-  const int64_t id = COOP ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * (blockDim.x >> 6) + wave;
-  if (id >= (int64_t)p.count * p.kv_heads) return;
-  const int kv = (int)(id % p.kv_heads), share = p.heads / p.kv_heads;
-  const AttnWork w = p.work[id / p.kv_heads];
+  const uint32_t id = COOP ? blockIdx.x : blockIdx.x * (blockDim.x >> 6) + wave;
+  if (id >= (uint32_t)p.count * p.kv_heads) return;
+  const int kv = uniform(id % p.kv_heads), share = uniform(p.heads / p.kv_heads);
+  const AttnWork w = load_work(p.work, uniform(id / p.kv_heads));
   const AttnLds<T, DP> lds(lds_raw + (COOP ? 0 : wave * lds_per_wave));
 
   const int mine = (COOP ? wave * kTile : 0) + col;
@@ -326,7 +327,7 @@ __global__ __launch_bounds__(256) void k_attn_bwd_k(AttnParams p, size_t lds_per
       const int n = w.row1 - q0 < kTile ? w.row1 - q0 : kTile;
       if (!AHEAD) tiles.load(qp + q0 * p.q_row, p.q_row, dp_ + q0 * p.do_row, p.do_row, n, p.dim, tid);
       tile_sync<COOP>();
-      tiles.store(lds.a, lds.b, tid);
+      tiles.store(lds.a, lds.b, n, p.dim, tid);
       if (tid < kTile) {
         const int64_t qr = q0 + (tid < n ? tid : 0);
         if (p.slope) lds.pos[tid] = make_float4(p.q_pos[3 * qr], p.q_pos[3 * qr + 1], p.q_pos[3 * qr + 2], 0.f);
@@ -341,6 +342,7 @@ __global__ __launch_bounds__(256) void k_attn_bwd_k(AttnParams p, size_t lds_per
         tiles.load(qp + next * p.q_row, p.q_row, dp_ + next * p.do_row, p.do_row, w.row1 - next, p.dim, tid);
       if (!busy) continue;
 
+      const int lane = here(lane_of_wave), col = lane & 31, hi = lane >> 5;
       f32x16 acc = acc_zero(), dp = acc_zero();
 #pragma unroll
       for (int c = 0; c < DP / 16; ++c)
@@ -473,15 +475,31 @@ __global__ __launch_bounds__(256) void k_attn_bwd_join(AttnParams p, AttnPosJoin
   double t = 0.0;
   float* out;
   if (b < n_slope) {
-    for (int i = tid; i < p.parts * kCoopWaves; i += 256) t += p.part_slope[(int64_t)b * p.parts * kCoopWaves + i];
+    const float4* part = (const float4*)(p.part_slope + (int64_t)b * p.parts * kCoopWaves);
+    for (int i = tid; i < p.parts; i += 4 * 256) {
+      float4 u[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) u[k] = i + k * 256 < p.parts ? part[i + k * 256] : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) t += ((double)u[k].x + u[k].y) + ((double)u[k].z + u[k].w);
+    }
     out = p.dslope + b;
   } else {
     const int at = b - n_slope, head = at / p.n_buckets, bucket = at % p.n_buckets;
     for (int i = tid; i < p.n_rel; i += 256) lut[i] = p.lut[i];
     __syncthreads();
-    for (int rel = 0; rel < p.n_rel; ++rel)
-      if (lut[rel] == bucket)
-        for (int i = tid; i < p.parts; i += 256) t += p.part_hist[((int64_t)head * p.n_rel + rel) * p.parts + i];
+    // as many lanes along the partial sums as there are, the others along the differences
+    const int along = p.parts > 128 ? 256 : p.parts > 64 ? 128 : 64, step = 256 / along;
+    for (int rel = tid / along; rel < p.n_rel; rel += step)
+      if (lut[rel] == bucket) {
+        const float* part = p.part_hist + ((int64_t)head * p.n_rel + rel) * p.parts;
+        float u[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int i = tid % along; i < p.parts; i += 4 * along)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (i + k * along < p.parts) u[k] += part[i + k * along];
+        t += ((double)u[0] + u[1]) + ((double)u[2] + u[3]);
+      }
     out = p.dtable + at;
   }
   for (int o = 32; o > 0; o >>= 1) t += __shfl_xor(t, o, 64);

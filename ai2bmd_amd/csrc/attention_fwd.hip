@@ -9,16 +9,16 @@
 namespace vsn {
 
 template <typename T, int DP, bool COOP>
-__global__ __launch_bounds__(256) void k_attn_fwd(AttnParams p, size_t lds_per_wave) {
+__global__ __launch_bounds__(256, (tile_waves<T, DP>())) void k_attn_fwd(AttnParams p, size_t lds_per_wave) {
   extern __shared__ __attribute__((aligned(16))) char lds_raw[];
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, lane_of_wave = lane;
   const int col = lane & 31, hi = lane >> 5;
   const int tid = COOP ? threadIdx.x : lane;
   constexpr int THREADS = COOP ? 64 * kCoopWaves : 64;
-  const int64_t id = COOP ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * (blockDim.x >> 6) + wave;
-  if (id >= (int64_t)p.count * p.heads) return;
-  const int head = (int)(id % p.heads);
-  const AttnWork w = p.work[id / p.heads];
+  const uint32_t id = COOP ? blockIdx.x : blockIdx.x * (blockDim.x >> 6) + wave;
+  if (id >= (uint32_t)p.count * p.heads) return;
+  const int head = uniform(id % p.heads);
+  const AttnWork w = load_work(p.work, uniform(id / p.heads));
   const AttnLds<T, DP> lds(lds_raw + (COOP ? 0 : wave * lds_per_wave));
 
   const int mine = (COOP ? wave * kTile : 0) + col;
@@ -26,7 +26,7 @@ __global__ __launch_bounds__(256) void k_attn_fwd(AttnParams p, size_t lds_per_w
   const bool busy = (COOP ? wave * kTile : 0) < w.cols;  // wave-uniform
   const bool whole = (COOP ? wave * kTile : 0) + kTile <= w.cols;
   const int64_t row = (int64_t)w.col0 + (live ? mine : 0);
-  const int kv = head / (p.heads / p.kv_heads);
+  const int kv = uniform(head / (p.heads / p.kv_heads));
   const T* kp = (const T*)p.k + kv * p.k_head;
   const T* vp = (const T*)p.v + kv * p.v_head;
 
@@ -60,7 +60,7 @@ __global__ __launch_bounds__(256) void k_attn_fwd(AttnParams p, size_t lds_per_w
     const int n = w.row1 - k0 < kTile ? w.row1 - k0 : kTile;
     if (!AHEAD) tiles.load(kp + k0 * p.k_row, p.k_row, vp + k0 * p.v_row, p.v_row, n, p.dim, tid);
     tile_sync<COOP>();
-    tiles.store(lds.a, lds.b, tid);
+    tiles.store(lds.a, lds.b, n, p.dim, tid);
     if (tid < kTile) {
       const int64_t kr = k0 + (tid < n ? tid : 0);
       if (p.slope) lds.pos[tid] = make_float4(p.k_pos[3 * kr], p.k_pos[3 * kr + 1], p.k_pos[3 * kr + 2], 0.f);
@@ -72,6 +72,7 @@ __global__ __launch_bounds__(256) void k_attn_fwd(AttnParams p, size_t lds_per_w
       tiles.load(kp + next * p.k_row, p.k_row, vp + next * p.v_row, p.v_row, w.row1 - next, p.dim, tid);
     if (!busy) continue;
 
+    const int lane = here(lane_of_wave), col = lane & 31, hi = lane >> 5;
     f32x16 acc = acc_zero();
 #pragma unroll
     for (int c = 0; c < DP / 16; ++c)

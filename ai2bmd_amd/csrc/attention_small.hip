@@ -13,31 +13,41 @@
 
 namespace vsn {
 
+// Waves per SIMD that the backward kernel is compiled for (registers are what limits them).
+template <typename T, int DP>
+constexpr int small_waves() {
+  return DP > 64 || (DP > 32 && sizeof(T) == 4) ? 1 : 2;
+}
+
 constexpr int kPullLd = 33;  // floats per row of the transposed pulls: column reads fall on different banks
 
 template <typename T, int DP>
 struct SmallLds {
   static constexpr size_t A = TileShape<T, DP>::BYTES, B = TileShape<T, 32>::BYTES;
   static constexpr size_t PULL = sizeof(float) * kTile * kPullLd;
-  static constexpr size_t SCRATCH = A + B > PULL ? A + B : PULL;  // tiles during the heads, pulls after them
-  T *a, *b;
-  float* pull;
+  T *dout, *q, *k;  // rows to be read transposed (the forward pass has v in `dout`)
+  T* score;         // [query][key]: P, then dS
+  float* pull;      // after the heads, in the tiles' place
   float4 *kpos, *qpos;
   int* kres;
-  float *hist, *slope;  // [heads][n_rel], [heads][64]
-  __device__ __forceinline__ SmallLds(char* p, int heads, int n_rel) {
-    a = (T*)p;
-    b = (T*)(p + A);
+  float* hist;  // [heads][n_rel]
+  __device__ __forceinline__ SmallLds(char* p, bool backward) {
+    dout = (T*)p;
+    q = (T*)(p + A);
+    k = (T*)(p + 2 * A);
+    score = (T*)(p + 3 * A);
     pull = (float*)p;
-    kpos = (float4*)(p + ((SCRATCH + 15) & ~(size_t)15));
+    kpos = (float4*)(p + scratch(backward));
     qpos = kpos + kTile;
     kres = (int*)(qpos + kTile);
     hist = (float*)(kres + kTile);
-    slope = hist + heads * n_rel;
+  }
+  static constexpr __host__ __device__ size_t scratch(bool backward) {
+    return ((backward ? (3 * A + B > PULL ? 3 * A + B : PULL) : A) + 15) & ~(size_t)15;
   }
   static size_t bytes(int heads, int n_rel, bool backward) {
-    const size_t fixed = ((SCRATCH + 15) & ~(size_t)15) + 2 * kTile * sizeof(float4) + kTile * sizeof(int);
-    return (fixed + (backward ? sizeof(float) * heads * (n_rel + 64) : 0) + 15) & ~(size_t)15;
+    return (scratch(backward) + 2 * kTile * sizeof(float4) + kTile * sizeof(int) +
+            (backward ? sizeof(float) * heads * n_rel : 0) + 15) & ~(size_t)15;
   }
 };
 
@@ -48,6 +58,26 @@ __device__ __forceinline__ void put_rows(T* tile, const typename vec8<T>::type (
   for (int c = 0; c < DP / 16; ++c)
     *(typename vec8<T>::type*)(tile + col * TileShape<T, DP>::LD + c * 16 + hi * 8) = f[c];
 }
+// A lane's row, loaded without a branch: the row is one of the fragment's in any case, a column beyond the end is
+// another one of it.  Both are zeroed where the row is used (keep_rows), so that nothing waits for a load ahead of that.
+// `base` is the wave's (its fragment's first row), `lane` the lane's offset in elements.
+template <typename T, int DP>
+__device__ __forceinline__ void load_rows(typename vec8<T>::type (&f)[DP / 16], const T* base, uint32_t lane, int dim,
+                                          int hi) {
+#pragma unroll
+  for (int c = 0; c < DP / 16; ++c)
+    f[c] = *(const typename vec8<T>::type*)(base + (lane + (c * 16 + hi * 8 < dim ? c * 16 + hi * 8 : 0)));
+}
+template <typename T, int DP>
+__device__ __forceinline__ void keep_rows(typename vec8<T>::type (&f)[DP / 16], int dim, int hi, bool live) {
+#pragma unroll
+  for (int c = 0; c < DP / 16; ++c) {
+    typename vec8<T>::type zero;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) zero[i] = (T)0.f;
+    f[c] = live && c * 16 + hi * 8 < dim ? f[c] : zero;
+  }
+}
 // the lane's 16 values as its row of [column][row]
 template <typename T>
 __device__ __forceinline__ void put_scores(T* tile, const float* v, int col, int hi) {
@@ -56,44 +86,52 @@ __device__ __forceinline__ void put_scores(T* tile, const float* v, int col, int
     store4<T>(tile + col * TileShape<T, 32>::LD + 8 * g + 4 * hi, v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
 }
 
-// distances (units of the input) and reciprocals, table indices, from LDS
+// distances and table indices of the lane's 16 pairs
 struct SmallGeometry {
-  float far[16], inv[16];
-  int at[16];
+  float far[16];
+  uint32_t pair[8];  // two table indices each
+  // (unpacked where it is used: 16 indices kept over the heads would cost a wave per SIMD)
+  __device__ __forceinline__ void here() {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) compute_here(pair[i]);
+  }
+  __device__ __forceinline__ int at(int r) const { return r & 1 ? pair[r >> 1] >> 16 : pair[r >> 1] & 0xffff; }
 };
 
-template <typename T, int DP, bool BACKWARD>
+template <typename T, int DP>
 __device__ __forceinline__ void small_geometry(const AttnParams& p, const AttnWork& w, const SmallLds<T, DP>& lds,
                                                SmallGeometry& g, int nk, int64_t q_row, int lane, int col, int hi) {
   tile_sync<false>();
   if (lane < kTile) {
     const int64_t kr = (int64_t)w.row0 + (col < nk ? col : 0);
     if (p.slope) {
-      lds.kpos[col] = nk ? make_float4(p.k_pos[3 * kr], p.k_pos[3 * kr + 1], p.k_pos[3 * kr + 2], 0.f)
-                         : make_float4(0.f, 0.f, 0.f, 0.f);
-      if (w.cols) lds.qpos[col] = make_float4(p.q_pos[3 * q_row], p.q_pos[3 * q_row + 1], p.q_pos[3 * q_row + 2], 0.f);
+      lds.kpos[col] = make_float4(p.k_pos[3 * kr], p.k_pos[3 * kr + 1], p.k_pos[3 * kr + 2], 0.f);
+      lds.qpos[col] = make_float4(p.q_pos[3 * q_row], p.q_pos[3 * q_row + 1], p.q_pos[3 * q_row + 2], 0.f);
     }
-    if (p.table) lds.kres[col] = nk ? p.k_res[kr] : 0;
+    if (p.table) lds.kres[col] = p.k_res[kr];
   }
   tile_sync<false>();
   if (p.slope) {
-    const float4 q = w.cols ? lds.qpos[col] : make_float4(0.f, 0.f, 0.f, 0.f);
+    const float4 q = lds.qpos[col];
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       const float4 k = lds.kpos[acc_row(r, hi)];
-      g.far[r] = pair_dist(q.x - k.x, q.y - k.y, q.z - k.z, g.inv[r]);
+      float inv;
+      g.far[r] = pair_dist(q.x - k.x, q.y - k.y, q.z - k.z, inv);
     }
   }
   if (p.table) {
-    const int res = w.cols ? p.q_res[q_row] : 0;
+    const int res = p.q_res[q_row];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) g.at[r] = rel_index(lds.kres[acc_row(r, hi)], res, p.reach);
+    for (int r = 0; r < 16; r += 2)
+      g.pair[r >> 1] = rel_index(lds.kres[acc_row(r, hi)], res, p.reach) |
+                       rel_index(lds.kres[acc_row(r + 1, hi)], res, p.reach) << 16;
   }
 }
 
 // the scores of one head, masked, from the product q.k
 template <typename T>
-__device__ __forceinline__ void small_scores(const AttnParams& p, const SmallGeometry& g, const f32x16& acc, float scale,
+__device__ __forceinline__ void small_scores(const AttnParams& p, SmallGeometry& g, const f32x16& acc, float scale,
                                              float slope2, const float* tab, int limit, int hi, float* s) {
 #pragma unroll
   for (int r = 0; r < 16; ++r) s[r] = acc[r] * scale;
@@ -102,9 +140,14 @@ __device__ __forceinline__ void small_scores(const AttnParams& p, const SmallGeo
     for (int r = 0; r < 16; ++r) s[r] -= slope2 * g.far[r];
   }
   if (p.table) {
+    g.here();
+    float b[16];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] += tab[g.at[r]];
+    for (int r = 0; r < 16; ++r) b[r] = tab[g.at(r)];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] += b[r];
   }
+  compute_here(limit);
 #pragma unroll
   for (int r = 0; r < 16; ++r) s[r] = acc_row(r, hi) < limit ? s[r] : -INFINITY;
 }
@@ -130,53 +173,64 @@ __global__ __launch_bounds__(256) void k_attn_small_fwd(AttnParams p, size_t per
   const int n_rel = p.table ? p.n_rel : 0;
   for (int i = threadIdx.x; i < p.heads * n_rel; i += blockDim.x)
     tab[i] = table_log2(p.table[(int64_t)(i / n_rel) * p.n_buckets + p.lut[i % n_rel]]);
+  float* slopes = tab + p.heads * n_rel;  // [heads]
+  for (int i = threadIdx.x; i < p.heads; i += blockDim.x) slopes[i] = p.slope ? p.slope[i] : 0.f;
   __syncthreads();
-  const int64_t id = (int64_t)blockIdx.x * (blockDim.x >> 6) + wave;
-  if (id >= (int64_t)p.count * groups) return;
-  const SmallLds<T, DP> lds(lds_raw + ((sizeof(float) * p.heads * n_rel + 15) & ~(size_t)15) + wave * per_wave, p.heads, 0);
-  const AttnWork w = p.work[id / groups];
+  const uint32_t id = blockIdx.x * (blockDim.x >> 6) + wave;
+  if (id >= (uint32_t)p.count * groups) return;
+  const SmallLds<T, DP> lds(lds_raw + ((sizeof(float) * p.heads * (n_rel + 1) + 15) & ~(size_t)15) + wave * per_wave, false);
+  const AttnWork w = load_work(p.work, uniform(id / groups));
   const int nq = w.cols, nk = w.row1 - w.row0;
   const bool live = col < nq;
   const int64_t q_row = (int64_t)w.col0 + (live ? col : 0), k_row = (int64_t)w.row0 + (col < nk ? col : 0);
   SmallGeometry g;
-  small_geometry<T, DP, false>(p, w, lds, g, nk, q_row, lane, col, hi);
+  small_geometry<T, DP>(p, w, lds, g, nk, q_row, lane, col, hi);
   const float scale = p.scale * kLog2e;
-  const int share = p.heads / p.kv_heads, each = p.heads / groups, h0 = (int)(id % groups) * each;
+  const int share = uniform(p.heads / p.kv_heads), each = uniform(p.heads / groups), h0 = uniform(id % groups) * each;
+  const uint32_t q_at = (live ? col : 0) * (uint32_t)p.q_row;
+  const uint32_t k_at = (col < nk ? col : 0) * (uint32_t)p.k_row, v_at = (col < nk ? col : 0) * (uint32_t)p.v_row;
+  const int lane_of_item = lane;
+  typename vec8<T>::type qf[DP / 16], kf[DP / 16], vf[DP / 16];
+  auto load = [&](int head) {
+    const int kv = uniform(head / share);
+    load_rows<T, DP>(qf, (const T*)p.q + w.col0 * p.q_row + head * p.q_head, q_at, p.dim, hi);
+    load_rows<T, DP>(kf, (const T*)p.k + w.row0 * p.k_row + kv * p.k_head, k_at, p.dim, hi);
+    load_rows<T, DP>(vf, (const T*)p.v + w.row0 * p.v_row + kv * p.v_head, v_at, p.dim, hi);
+  };
+  load(h0);
   for (int head = h0; head < h0 + each; ++head) {
-    const int kv = head / share;
-    typename vec8<T>::type qf[DP / 16], kf[DP / 16], vf[DP / 16];
-#pragma unroll
-    for (int c = 0; c < DP / 16; ++c) {
-      qf[c] = load_col<T>((const T*)p.q + q_row * p.q_row + head * p.q_head, c * 16 + hi * 8, p.dim, live);
-      kf[c] = load_col<T>((const T*)p.k + k_row * p.k_row + kv * p.k_head, c * 16 + hi * 8, p.dim, col < nk);
-      vf[c] = load_col<T>((const T*)p.v + k_row * p.v_row + kv * p.v_head, c * 16 + hi * 8, p.dim, col < nk);
-    }
+    const int lane = here(lane_of_item), col = lane & 31, hi = lane >> 5;
+    keep_rows<T, DP>(qf, p.dim, hi, live);
+    keep_rows<T, DP>(kf, p.dim, hi, col < nk);
+    keep_rows<T, DP>(vf, p.dim, hi, col < nk);
     f32x16 acc = acc_zero();
 #pragma unroll
     for (int c = 0; c < DP / 16; ++c)
       if (c * 16 < p.dim) acc = Mma<T>::run(kf[c], qf[c], acc);
     tile_sync<false>();
-    put_rows<T, DP>(lds.a, vf, col, hi);
+    put_rows<T, DP>(lds.dout, vf, col, hi);
     tile_sync<false>();
+    if (head + 1 < h0 + each) load(head + 1);  // in flight while this head is computed
     float s[16];
-    small_scores<T>(p, g, acc, scale, p.slope ? p.slope[head] * kLog2e : 0.f, tab + head * n_rel, live ? nk : 0, hi, s);
+    small_scores<T>(p, g, acc, scale, slopes[head] * kLog2e, tab + head * n_rel, live ? nk : 0, hi, s);
     const float top = small_exp(s);
     float l = tile_sum(s);
     l += other_half(l);
     const float inv = l == 0.f ? 0.f : 1.f / l;
     const typename vec8<T>::type p0 = pack8<T>(s), p1 = pack8<T>(s + 8);
     if (live && hi == 0 && p.stats) p.stats[head * p.rows_q + q_row] = make_float2(top, l);
-    T* op = (T*)p.out + q_row * p.out_row + head * p.out_head;
+    T* op = (T*)p.out + w.col0 * p.out_row + head * p.out_head;
+    const uint32_t o_at = col * (uint32_t)p.out_row;
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d) {
       if (d * 32 >= p.dim) continue;
       f32x16 o = acc_zero();
-      o = Mma<T>::run(load_t<T, DP>(lds.a, 0, d * 32, lane, hi), p0, o);
-      o = Mma<T>::run(load_t<T, DP>(lds.a, 1, d * 32, lane, hi), p1, o);
+      o = Mma<T>::run(load_t<T, DP>(lds.dout, 0, d * 32, lane, hi), p0, o);
+      if (nk > 16) o = Mma<T>::run(load_t<T, DP>(lds.dout, 1, d * 32, lane, hi), p1, o);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const int e = d * 32 + 8 * k + 4 * hi;
-        if (live && e < p.dim) store4<T>(op + e, o[4 * k] * inv, o[4 * k + 1] * inv, o[4 * k + 2] * inv, o[4 * k + 3] * inv);
+        if (live && e < p.dim) store4<T>(op + (o_at + e), o[4 * k] * inv, o[4 * k + 1] * inv, o[4 * k + 2] * inv, o[4 * k + 3] * inv);
       }
     }
   }
@@ -184,50 +238,62 @@ __global__ __launch_bounds__(256) void k_attn_small_fwd(AttnParams p, size_t per
 
 // groups: 1 (a wave walks all heads and writes the positions' gradient), or kv_heads (a wave takes the heads of one key
 // head, where there are few fragments; the positions' gradients are joined afterwards)
-template <typename T, int DP>
-__global__ __launch_bounds__(256) void k_attn_small_bwd(AttnParams p, size_t per_wave, int groups) {
+template <typename T, int DP, bool SHARE>
+__global__ __launch_bounds__(256, (small_waves<T, DP>())) void k_attn_small_bwd(AttnParams p, size_t per_wave, int groups) {
   extern __shared__ __attribute__((aligned(16))) char lds_raw[];
   constexpr bool HALF = sizeof(T) == 2 && !__is_same(T, __bf16);
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int col = lane & 31, hi = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane_of_wave = threadIdx.x & 63;
   float* tab = (float*)lds_raw;
   const int n_rel = p.table ? p.n_rel : 0;
   for (int i = threadIdx.x; i < p.heads * n_rel; i += blockDim.x)
     tab[i] = table_log2(p.table[(int64_t)(i / n_rel) * p.n_buckets + p.lut[i % n_rel]]);
+  float* slopes = tab + p.heads * n_rel;  // [heads]
+  for (int i = threadIdx.x; i < p.heads; i += blockDim.x) slopes[i] = p.slope ? p.slope[i] : 0.f;
   __syncthreads();
-  const int64_t id = (int64_t)blockIdx.x * (blockDim.x >> 6) + wave;
-  if (id >= (int64_t)p.workers * groups) return;
-  const SmallLds<T, DP> lds(lds_raw + ((sizeof(float) * p.heads * n_rel + 15) & ~(size_t)15) + wave * per_wave, p.heads, n_rel);
-  const int worker = (int)(id / groups), group = (int)(id % groups);
-  const int share = p.heads / p.kv_heads, each = p.heads / groups, h0 = group * each;
-  for (int i = lane; i < p.heads * n_rel; i += 64) lds.hist[i] = 0.f;
-  for (int i = lane; i < p.heads * 64; i += 64) lds.slope[i] = 0.f;
+  const uint32_t id = blockIdx.x * (blockDim.x >> 6) + wave;
+  if (id >= (uint32_t)p.workers * groups) return;
+  const SmallLds<T, DP> lds(lds_raw + ((sizeof(float) * p.heads * (n_rel + 1) + 15) & ~(size_t)15) + wave * per_wave, true);
+  const int worker = uniform(id / groups), group = uniform(id % groups);
+  const int share = SHARE ? uniform(p.heads / p.kv_heads) : 1, each = uniform(p.heads / groups), h0 = group * each;
+  for (int i = lane_of_wave; i < p.heads * n_rel; i += 64) lds.hist[i] = 0.f;
+  float dslope = 0.f;  // of head `lane`
   const float scale = p.scale * kLog2e;
 
   for (int item = worker; item < p.count; item += p.workers) {
-    const AttnWork w = p.work[item];
+    const AttnWork w = load_work(p.work, item);
+    const int lane = here(lane_of_wave), col = lane & 31, hi = lane >> 5;
     const int nq = w.cols, nk = w.row1 - w.row0;
     const bool live = col < nq, key = col < nk;
     const int64_t q_row = (int64_t)w.col0 + (live ? col : 0), k_row = (int64_t)w.row0 + (key ? col : 0);
     SmallGeometry g;
-    small_geometry<T, DP, true>(p, w, lds, g, nk, q_row, lane, col, hi);
+    small_geometry<T, DP>(p, w, lds, g, nk, q_row, lane, col, hi);
     float weight[16];  // sum over heads of slope dS
 #pragma unroll
     for (int r = 0; r < 16; ++r) weight[r] = 0.f;
-    f32x16 dk[DP / 32], dv[DP / 32];
+    f32x16 dk[DP / 32], dv[DP / 32];  // over the heads that share a key head
+    if (SHARE)
 #pragma unroll
-    for (int d = 0; d < DP / 32; ++d) dk[d] = acc_zero(), dv[d] = acc_zero();
+      for (int d = 0; d < DP / 32; ++d) dk[d] = acc_zero(), dv[d] = acc_zero();
 
+    const uint32_t q_at = (live ? col : 0) * (uint32_t)p.q_row, d_at = (live ? col : 0) * (uint32_t)p.do_row;
+    const uint32_t k_at = (key ? col : 0) * (uint32_t)p.k_row, v_at = (key ? col : 0) * (uint32_t)p.v_row;
+    typename vec8<T>::type qf[DP / 16], df[DP / 16], kf[DP / 16], vf[DP / 16];
+    auto load = [&](int head) {
+      const int kv = SHARE ? uniform(head / share) : head;
+      load_rows<T, DP>(qf, (const T*)p.q + w.col0 * p.q_row + head * p.q_head, q_at, p.dim, hi);
+      load_rows<T, DP>(kf, (const T*)p.k + w.row0 * p.k_row + kv * p.k_head, k_at, p.dim, hi);
+      load_rows<T, DP>(df, (const T*)p.dout + w.col0 * p.do_row + head * p.do_head, d_at, p.dim, hi);
+      load_rows<T, DP>(vf, (const T*)p.v + w.row0 * p.v_row + kv * p.v_head, v_at, p.dim, hi);
+    };
+    load(h0);
+    const int lane_of_item = lane;
     for (int head = h0; head < h0 + each; ++head) {
-      const int kv = head / share;
-      typename vec8<T>::type qf[DP / 16], df[DP / 16], kf[DP / 16], vf[DP / 16];
-#pragma unroll
-      for (int c = 0; c < DP / 16; ++c) {
-        qf[c] = load_col<T>((const T*)p.q + q_row * p.q_row + head * p.q_head, c * 16 + hi * 8, p.dim, live);
-        kf[c] = load_col<T>((const T*)p.k + k_row * p.k_row + kv * p.k_head, c * 16 + hi * 8, p.dim, key);
-        df[c] = load_col<T>((const T*)p.dout + q_row * p.do_row + head * p.do_head, c * 16 + hi * 8, p.dim, live);
-        vf[c] = load_col<T>((const T*)p.v + k_row * p.v_row + kv * p.v_head, c * 16 + hi * 8, p.dim, key);
-      }
+      const int lane = here(lane_of_item), col = lane & 31, hi = lane >> 5;
+      const int kv = SHARE ? uniform(head / share) : head;
+      keep_rows<T, DP>(qf, p.dim, hi, live);
+      keep_rows<T, DP>(kf, p.dim, hi, key);
+      keep_rows<T, DP>(df, p.dim, hi, live);
+      keep_rows<T, DP>(vf, p.dim, hi, key);
       f32x16 acc = acc_zero(), dp = acc_zero();
 #pragma unroll
       for (int c = 0; c < DP / 16; ++c)
@@ -235,7 +301,12 @@ __global__ __launch_bounds__(256) void k_attn_small_bwd(AttnParams p, size_t per
           acc = Mma<T>::run(kf[c], qf[c], acc);
           dp = Mma<T>::run(vf[c], df[c], dp);
         }
-      const float slope = p.slope ? p.slope[head] : 0.f;
+      tile_sync<false>();
+      put_rows<T, DP>(lds.dout, df, col, hi);
+      put_rows<T, DP>(lds.q, qf, col, hi);
+      put_rows<T, DP>(lds.k, kf, col, hi);
+      if (head + 1 < h0 + each) load(head + 1);  // in flight while this head is computed
+      const float slope = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, slopes[head])));
       float s[16], t[16];
       small_scores<T>(p, g, acc, scale, slope * kLog2e, tab + head * n_rel, live ? nk : 0, hi, s);
       small_exp(s);
@@ -258,15 +329,17 @@ __global__ __launch_bounds__(256) void k_attn_small_bwd(AttnParams p, size_t per
           sum -= t[r] * g.far[r];
           weight[r] += slope * t[r];
         }
-        lds.slope[head * 64 + lane] += sum;
+        sum = wave_sum(sum);
+        if (lane == head) dslope += sum;
       }
       if (p.part_hist) {
         float run = 0.f;
+        g.here();
 #pragma unroll
         for (int r = 0; r < 16; ++r) {  // (runs of keys of one residue are added up in the lane first)
           run += t[r];
-          if (r == 15 || g.at[r < 15 ? r + 1 : 15] != g.at[r]) {
-            __hip_atomic_fetch_add(lds.hist + head * n_rel + g.at[r], run, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+          if (r == 15 || g.at(r < 15 ? r + 1 : 15) != g.at(r)) {
+            __hip_atomic_fetch_add(lds.hist + head * n_rel + g.at(r), run, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
             run = 0.f;
           }
         }
@@ -287,60 +360,59 @@ __global__ __launch_bounds__(256) void k_attn_small_bwd(AttnParams p, size_t per
 #pragma unroll
         for (int r = 0; r < 16; ++r) t[r] *= up, s[r] *= PUP;
       }
-      tile_sync<false>();
-      put_rows<T, DP>(lds.a, df, col, hi);
-      put_scores<T>(lds.b, s, col, hi);
+      put_scores<T>(lds.score, s, col, hi);
       tile_sync<false>();
 #pragma unroll
       for (int d = 0; d < DP / 32; ++d)
-        if (d * 32 < p.dim)
-          tile_mma<T>(dv[d], load_t<T, DP>(lds.a, 0, d * 32, lane, hi), load_t<T, 32>(lds.b, 0, 0, lane, hi),
-                      load_t<T, DP>(lds.a, 1, d * 32, lane, hi), load_t<T, 32>(lds.b, 1, 0, lane, hi));
+        if (d * 32 < p.dim) {
+          if (!SHARE) dv[d] = acc_zero();
+          dv[d] = Mma<T>::run(load_t<T, DP>(lds.dout, 0, d * 32, lane, hi), load_t<T, 32>(lds.score, 0, 0, lane, hi), dv[d]);
+          if (nq > 16)  // (the other half of the contraction is all zeros)
+            dv[d] = Mma<T>::run(load_t<T, DP>(lds.dout, 1, d * 32, lane, hi), load_t<T, 32>(lds.score, 1, 0, lane, hi), dv[d]);
+        }
       tile_sync<false>();
-      put_rows<T, DP>(lds.a, qf, col, hi);
-      put_scores<T>(lds.b, t, col, hi);
+      put_scores<T>(lds.score, t, col, hi);
       tile_sync<false>();
 #pragma unroll
       for (int d = 0; d < DP / 32; ++d) {
         if (d * 32 >= p.dim) continue;
         f32x16 x = acc_zero();
-        x = Mma<T>::run(load_t<T, DP>(lds.a, 0, d * 32, lane, hi), load_t<T, 32>(lds.b, 0, 0, lane, hi), x);
-        x = Mma<T>::run(load_t<T, DP>(lds.a, 1, d * 32, lane, hi), load_t<T, 32>(lds.b, 1, 0, lane, hi), x);
+        x = Mma<T>::run(load_t<T, DP>(lds.q, 0, d * 32, lane, hi), load_t<T, 32>(lds.score, 0, 0, lane, hi), x);
+        if (nq > 16) x = Mma<T>::run(load_t<T, DP>(lds.q, 1, d * 32, lane, hi), load_t<T, 32>(lds.score, 1, 0, lane, hi), x);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) dk[d][r] += x[r] * down;
+        for (int r = 0; r < 16; ++r) dk[d][r] = SHARE ? dk[d][r] + x[r] * down : x[r] * down;
       }
-      tile_sync<false>();
-      put_rows<T, DP>(lds.a, kf, col, hi);
-      tile_sync<false>();
       const typename vec8<T>::type t0 = pack8<T>(t), t1 = pack8<T>(t + 8);
       const float f = p.scale * down;
-      T* oq = (T*)p.dq + (q_row * p.heads + head) * p.dim;
+      T* oq = (T*)p.dq + ((int64_t)w.col0 * p.heads + head) * p.dim;
+      const uint32_t oq_at = (uint32_t)(col * p.heads) * p.dim;
 #pragma unroll
       for (int d = 0; d < DP / 32; ++d) {
         if (d * 32 >= p.dim) continue;
         f32x16 x = acc_zero();
-        x = Mma<T>::run(load_t<T, DP>(lds.a, 0, d * 32, lane, hi), t0, x);
-        x = Mma<T>::run(load_t<T, DP>(lds.a, 1, d * 32, lane, hi), t1, x);
+        x = Mma<T>::run(load_t<T, DP>(lds.k, 0, d * 32, lane, hi), t0, x);
+        if (nk > 16) x = Mma<T>::run(load_t<T, DP>(lds.k, 1, d * 32, lane, hi), t1, x);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const int e = d * 32 + 8 * k + 4 * hi;
-          if (live && e < p.dim) store4<T>(oq + e, x[4 * k] * f, x[4 * k + 1] * f, x[4 * k + 2] * f, x[4 * k + 3] * f);
+          if (live && e < p.dim) store4<T>(oq + (oq_at + e), x[4 * k] * f, x[4 * k + 1] * f, x[4 * k + 2] * f, x[4 * k + 3] * f);
         }
       }
-      if (head % share == share - 1) {
+      if (!SHARE || head % share == share - 1) {
         constexpr float PDOWN = 1.f / PUP;
-        T* ok = (T*)p.dk + (k_row * p.kv_heads + kv) * p.dim;
-        T* ov = (T*)p.dv + (k_row * p.kv_heads + kv) * p.dim;
+        T* ok = (T*)p.dk + ((int64_t)w.row0 * p.kv_heads + kv) * p.dim;
+        T* ov = (T*)p.dv + ((int64_t)w.row0 * p.kv_heads + kv) * p.dim;
+        const uint32_t ok_at = (uint32_t)(col * p.kv_heads) * p.dim;
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d) {
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const int e = d * 32 + 8 * k + 4 * hi;
             if (!key || e >= p.dim) continue;
-            store4<T>(ok + e, dk[d][4 * k] * p.scale, dk[d][4 * k + 1] * p.scale, dk[d][4 * k + 2] * p.scale, dk[d][4 * k + 3] * p.scale);
-            store4<T>(ov + e, dv[d][4 * k] * PDOWN, dv[d][4 * k + 1] * PDOWN, dv[d][4 * k + 2] * PDOWN, dv[d][4 * k + 3] * PDOWN);
+            store4<T>(ok + (ok_at + e), dk[d][4 * k] * p.scale, dk[d][4 * k + 1] * p.scale, dk[d][4 * k + 2] * p.scale, dk[d][4 * k + 3] * p.scale);
+            store4<T>(ov + (ok_at + e), dv[d][4 * k] * PDOWN, dv[d][4 * k + 1] * PDOWN, dv[d][4 * k + 2] * PDOWN, dv[d][4 * k + 3] * PDOWN);
           }
-          dk[d] = acc_zero(), dv[d] = acc_zero();
+          if (SHARE) dk[d] = acc_zero(), dv[d] = acc_zero();
         }
       }
     }
@@ -354,8 +426,11 @@ __global__ __launch_bounds__(256) void k_attn_small_bwd(AttnParams p, size_t per
       for (int r = 0; r < 16; ++r) {
         const int row = acc_row(r, hi);
         const float4 k = lds.kpos[row];
-        const float f = live ? weight[r] * g.inv[r] : 0.f;
-        x -= f * (q.x - k.x), y -= f * (q.y - k.y), z -= f * (q.z - k.z);
+        const float dx = q.x - k.x, dy = q.y - k.y, dz = q.z - k.z;
+        float inv;
+        pair_dist(dx, dy, dz, inv);
+        const float f = live ? weight[r] * inv : 0.f;
+        x -= f * dx, y -= f * dy, z -= f * dz;
         lds.pull[col * kPullLd + row] = f;
       }
       tile_sync<false>();
@@ -386,10 +461,11 @@ __global__ __launch_bounds__(256) void k_attn_small_bwd(AttnParams p, size_t per
   }
 
   tile_sync<false>();
+  const int lane = lane_of_wave;
   const int64_t part = p.part0 + worker;
   for (int head = h0; head < h0 + each; ++head) {
     if (p.part_slope) {
-      const float sum = wave_sum(lds.slope[head * 64 + lane]);
+      const float sum = __shfl(dslope, head, 64);
       if (lane < kCoopWaves) p.part_slope[(head * (int64_t)p.parts + part) * kCoopWaves + lane] = lane ? 0.f : sum;
     }
     if (p.part_hist)
@@ -400,7 +476,7 @@ __global__ __launch_bounds__(256) void k_attn_small_bwd(AttnParams p, size_t per
 template <typename T, int DP>
 static int small_launch(AttnParams p, int groups, bool backward, hipStream_t st) {
   const int n_rel = p.table ? p.n_rel : 0;
-  const size_t tab = (sizeof(float) * p.heads * n_rel + 15) & ~(size_t)15;
+  const size_t tab = (sizeof(float) * p.heads * (n_rel + 1) + 15) & ~(size_t)15;
   const size_t bytes = SmallLds<T, DP>::bytes(p.heads, n_rel, backward);
   const int64_t total = (int64_t)(backward ? p.workers : p.count) * groups;
   int waves = total <= 1024 ? 1 : 4;
@@ -408,8 +484,13 @@ static int small_launch(AttnParams p, int groups, bool backward, hipStream_t st)
   const size_t lds = tab + waves * bytes;
   const dim3 grid((unsigned)((total + waves - 1) / waves)), block(64 * waves);
   if (backward) {
-    if (!allow_lds((const void*)k_attn_small_bwd<T, DP>, lds)) return -5;
-    hipLaunchKernelGGL((k_attn_small_bwd<T, DP>), grid, block, lds, st, p, bytes, groups);
+    if (p.heads == p.kv_heads) {
+      if (!allow_lds((const void*)k_attn_small_bwd<T, DP, false>, lds)) return -5;
+      hipLaunchKernelGGL((k_attn_small_bwd<T, DP, false>), grid, block, lds, st, p, bytes, groups);
+    } else {
+      if (!allow_lds((const void*)k_attn_small_bwd<T, DP, true>, lds)) return -5;
+      hipLaunchKernelGGL((k_attn_small_bwd<T, DP, true>), grid, block, lds, st, p, bytes, groups);
+    }
   } else {
     if (!allow_lds((const void*)k_attn_small_fwd<T, DP>, lds)) return -5;
     hipLaunchKernelGGL((k_attn_small_fwd<T, DP>), grid, block, lds, st, p, bytes, groups);
