@@ -27,11 +27,12 @@ constexpr int kMaxReach = 1023;   // clipped residue difference: 2 reach + 1 tab
 struct AttnWork {
   int col0, cols;  // first column row, number of columns (<= 32, or <= 128 where the workgroup shares tiles)
   int row0, row1;  // the rows it meets
-  int slot;        // >= 0: partial result of a split run of keys, joined afterwards
+  int slot;        // >= 0: one of several pieces of a run of rows; its partial results go to slots slot + wave
+  int slot0, slots, step;  // the pieces' slots: slot0 + wave + i step, i < slots
 };
-// Partial results to join: `cols` query rows from col0, slots slot0 ... slot0 + slots - 1
+// Partial results to join: `cols` (<= 32) columns from col0, slots slot0 + i step, i < slots
 struct AttnJoin {
-  int col0, cols, slot0, slots;
+  int col0, cols, slot0, slots, step;
 };
 
 struct AttnParams {
@@ -52,8 +53,10 @@ struct AttnParams {
   void* out;
   int64_t out_row, out_head;
   float2* stats;          // [heads][rows_q] {maximum in units of log 2, sum of exponentials}
-  float* part_o;          // split keys: [slot][heads][32][dim] unnormalised output
-  float2* part_ml;        // [slot][heads][32]
+  // pieces of split runs
+  float *part_o, *part_o2;  // [slot][heads][32][dim]: unnormalised output; dq; dk and dv
+  float2* part_ml;          // [slot][heads][32]: maximum and sum; sums of e and of e dP
+  float* part_g;            // [slot][heads][32][4]: a column's positions' gradient
   const AttnJoin* join;
   // backward
   float2* delta;          // [heads][rows_q] {D, 1 / sum of exponentials}
@@ -85,7 +88,8 @@ __device__ __forceinline__ AttnWork load_work(const AttnWork* work, int64_t at) 
   AttnWork w = work[at];
   w.col0 = __builtin_amdgcn_readfirstlane(w.col0), w.cols = __builtin_amdgcn_readfirstlane(w.cols);
   w.row0 = __builtin_amdgcn_readfirstlane(w.row0), w.row1 = __builtin_amdgcn_readfirstlane(w.row1);
-  w.slot = __builtin_amdgcn_readfirstlane(w.slot);
+  w.slot = __builtin_amdgcn_readfirstlane(w.slot), w.slot0 = __builtin_amdgcn_readfirstlane(w.slot0);
+  w.slots = __builtin_amdgcn_readfirstlane(w.slots), w.step = __builtin_amdgcn_readfirstlane(w.step);
   return w;
 }
 
@@ -272,6 +276,24 @@ __device__ __forceinline__ void tile_mma(f32x16& c, typename vec8<T>::type a0, t
     c = Mma<T>::run(a0, b0, c);
     c = Mma<T>::run(a1, b1, c);
   }
+}
+
+// Whether all differences of a tile are clipped to one end of the table: its index, or -1.  `row_res` is the residue of
+// tile row (lane & 31), lo and hi the smallest and the largest residue of the wave's columns; sign +1: rows are keys.
+__device__ __forceinline__ int clipped_end(int row_res, int lo, int hi, int sign, int reach) {
+  const int up = sign > 0 ? __builtin_elementwise_sub_sat(row_res, hi) : __builtin_elementwise_sub_sat(lo, row_res);
+  const int down = sign > 0 ? __builtin_elementwise_sub_sat(row_res, lo) : __builtin_elementwise_sub_sat(hi, row_res);
+  return __all(up >= reach) ? 2 * reach : __all(down <= -reach) ? 0 : -1;
+}
+// smallest and largest of the wave's columns
+__device__ __forceinline__ void column_range(int v, int& lo, int& hi) {
+  lo = hi = v;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const int a = __shfl_xor(lo, o, 64), b = __shfl_xor(hi, o, 64);
+    lo = a < lo ? a : lo, hi = b > hi ? b : hi;
+  }
+  lo = __builtin_amdgcn_readfirstlane(lo), hi = __builtin_amdgcn_readfirstlane(hi);
 }
 
 __device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, 64); }

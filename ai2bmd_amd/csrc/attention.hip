@@ -9,8 +9,11 @@ struct vsn_attn {
   struct Side {
     vsn::AttnWork *small_work = nullptr, *lone_work = nullptr, *coop_work = nullptr;
     vsn::AttnJoin* join = nullptr;
-    int small = 0, lone = 0, coop = 0, joins = 0, slots = 0;
-    vsn::AttnPlanView view() const { return {small_work, lone_work, coop_work, small, lone, coop, join, joins}; }
+    vsn::AttnBlock* block = nullptr;
+    int small = 0, lone = 0, coop = 0, joins = 0, blocks = 0, slots = 0, long_rows = 0;
+    vsn::AttnPlanView view() const {
+      return {small_work, lone_work, coop_work, small, lone, coop, long_rows, block, blocks, join, joins};
+    }
   };
   int device = 0, heads = 0, kv_heads = 0, dim = 0, reach = 0, n_rel = 0, n_buckets = 0;
   int64_t used_q = 0, used_k = 0;
@@ -26,21 +29,23 @@ namespace {
 // compute units.
 constexpr int kCoopCols = kTile * kCoopWaves;
 constexpr int64_t kCoopMin = 256;
-// A run of keys is split where the items alone leave most of the 1024 SIMDs without a wave and a piece still keeps
-// enough tiles to be worth joining.
-constexpr int64_t kSplitBelow = 1024, kSplitWaves = 2048;
-constexpr int kSplitTiles = 16;
+// A run of rows is split into pieces where the items alone are too few waves for the 1024 SIMDs to be filled evenly
+// (12 rounds of one wave each); a piece keeps at least 4 tiles, which is what joining it costs.
+constexpr int64_t kPieceWaves = 12288;
+constexpr int kPieceTiles = 4;
 
 constexpr int kSmallSums = 4096;  // floats of table sums per wave
 
 struct Lists {
   std::vector<AttnWork> small, lone, coop;
   std::vector<AttnJoin> join;
+  std::vector<AttnBlock> block;
   int slots = 0;
+  bool long_rows = false;
 };
 
 Lists make_lists(int64_t n, const int64_t* col_start, const int64_t* col_end, const int64_t* row_start,
-                 const int64_t* row_end, int heads, bool small, bool split) {
+                 const int64_t* row_end, int heads, bool small) {
   Lists out;
   int64_t groups = 0;
   for (int64_t f = 0; f < n; ++f) {
@@ -48,50 +53,50 @@ Lists make_lists(int64_t n, const int64_t* col_start, const int64_t* col_end, co
     if (cols > 2 * kTile) groups += (cols + kCoopCols - 1) / kCoopCols * heads;
   }
   const bool share = groups >= kCoopMin;
-  int64_t tiles = 0;
+  std::vector<AttnWork> all;
+  int64_t waves = 0, tiles = 0;  // of 32 columns; tiles of 32 x 32
   for (int64_t f = 0; f < n; ++f) {
     const int64_t cols = col_end[f] - col_start[f], rows = row_end[f] - row_start[f];
+    AttnWork w = {};
+    w.slot = -1;
+    w.row0 = (int)row_start[f], w.row1 = (int)row_end[f];
     if (small && cols && rows && cols <= kTile && rows <= kTile) {
-      AttnWork w = {};
-      w.col0 = (int)col_start[f], w.cols = (int)cols, w.row0 = (int)row_start[f], w.row1 = (int)row_end[f], w.slot = -1;
+      w.col0 = (int)col_start[f], w.cols = (int)cols;
       out.small.push_back(w);
       continue;
     }
-    const bool coop = share && cols > 2 * kTile;
-    const int64_t step = coop ? kCoopCols : kTile;
+    const int64_t step = share && cols > 2 * kTile ? kCoopCols : kTile;
     for (int64_t c = 0; c < cols; c += step) {
-      AttnWork w = {};
-      w.col0 = (int)(col_start[f] + c);
-      w.cols = (int)std::min<int64_t>(step, cols - c);
-      w.row0 = (int)row_start[f];
-      w.row1 = (int)row_end[f];
-      w.slot = -1;
-      (coop ? out.coop : out.lone).push_back(w);
-      if (!coop) tiles += (rows + kTile - 1) / kTile;
+      w.col0 = (int)(col_start[f] + c), w.cols = (int)std::min<int64_t>(step, cols - c);
+      w.step = (int)(step / kTile);
+      all.push_back(w);
+      out.block.push_back({w.col0, w.cols});
+      const int64_t each = (w.cols + kTile - 1) / kTile;
+      waves += each * heads, tiles += each * heads * ((rows + kTile - 1) / kTile);
     }
   }
-  const int64_t waves = (int64_t)out.lone.size() * heads;
-  if (split && waves && waves < kSplitBelow && out.coop.empty()) {
-    std::vector<AttnWork> pieces;
-    for (const AttnWork& w : out.lone) {
-      const int64_t have = ((int64_t)w.row1 - w.row0 + kTile - 1) / kTile;
-      const int64_t per = std::max<int64_t>({2, (tiles * heads + kSplitWaves - 1) / kSplitWaves,
-                                             (have + kMaxSlots - 1) / kMaxSlots});
-      const int64_t parts = (have + per - 1) / per;
-      if (have < kSplitTiles || parts < 2) {
-        pieces.push_back(w);
-        continue;
-      }
-      out.join.push_back({w.col0, w.cols, out.slots, (int)parts});
-      for (int64_t i = 0; i < parts; ++i) {
-        AttnWork piece = w;
-        piece.row0 = (int)(w.row0 + i * per * kTile);
-        piece.row1 = (int)std::min<int64_t>(w.row1, w.row0 + (i + 1) * per * kTile);
-        piece.slot = out.slots++;
-        pieces.push_back(piece);
-      }
+  const bool split = waves < kPieceWaves;
+  const int64_t least = std::max<int64_t>(kPieceTiles, (tiles + kPieceWaves - 1) / kPieceWaves);
+  for (const AttnWork& w : all) {
+    std::vector<AttnWork>& to = w.step > 1 ? out.coop : out.lone;
+    const int64_t have = ((int64_t)w.row1 - w.row0 + kTile - 1) / kTile;
+    const int64_t per = std::max<int64_t>(least, (have + kMaxSlots - 1) / kMaxSlots);
+    out.long_rows |= have > 1;
+    if (!split || have < 2 * per) {
+      to.push_back(w);
+      continue;
     }
-    out.lone.swap(pieces);
+    AttnWork piece = w;
+    piece.slots = (int)((have + per - 1) / per), piece.slot0 = out.slots;
+    for (int i = 0; i < piece.slots; ++i) {
+      piece.row0 = (int)(w.row0 + i * per * kTile);
+      piece.row1 = (int)std::min<int64_t>(w.row1, w.row0 + (i + 1) * per * kTile);
+      piece.slot = out.slots;
+      out.slots += w.step;
+      to.push_back(piece);
+    }
+    for (int k = 0; k * kTile < w.cols; ++k)
+      out.join.push_back({w.col0 + k * kTile, std::min(kTile, w.cols - k * kTile), piece.slot0 + k, piece.slots, w.step});
   }
   return out;
 }
@@ -105,7 +110,8 @@ bool upload(const std::vector<E>& v, E** dev) {
 
 bool upload_side(const Lists& l, vsn_attn::Side& s) {
   s.small = (int)l.small.size(), s.lone = (int)l.lone.size(), s.coop = (int)l.coop.size(), s.joins = (int)l.join.size(), s.slots = l.slots;
-  return upload(l.small, &s.small_work) && upload(l.lone, &s.lone_work) && upload(l.coop, &s.coop_work) && upload(l.join, &s.join);
+  s.blocks = (int)l.block.size(), s.long_rows = l.long_rows;
+  return upload(l.small, &s.small_work) && upload(l.lone, &s.lone_work) && upload(l.coop, &s.coop_work) && upload(l.join, &s.join) && upload(l.block, &s.block);
 }
 
 void free_side(vsn_attn::Side& s) {
@@ -113,6 +119,7 @@ void free_side(vsn_attn::Side& s) {
   hipFree(s.lone_work);
   hipFree(s.coop_work);
   hipFree(s.join);
+  hipFree(s.block);
 }
 
 bool ranges_ok(int64_t n, const int64_t* start, const int64_t* end) {
@@ -140,7 +147,7 @@ struct Workspace {
 };
 
 struct BackwardSpace {
-  int64_t delta, pos_q, pos_k, slope, hist, size;
+  int64_t delta, pos_q, pos_k, slope, hist, ml, o, o2, g, size;
   AttnWorkers workers;
   int parts;
 };
@@ -157,6 +164,12 @@ BackwardSpace backward_space(const vsn_attn& a, int64_t rows_q, int64_t rows_k) 
   s.pos_k = w.take(rows_k * a.kv_heads * 12);
   s.slope = w.take((int64_t)s.parts * a.heads * kCoopWaves * 4);
   s.hist = w.take((int64_t)s.parts * a.heads * a.n_rel * 4);
+  // pieces: the dq pass and the dk / dv pass use the same space one after the other
+  const int64_t q_cols = (int64_t)a.by_query.slots * a.heads * kTile, k_cols = (int64_t)a.by_key.slots * a.kv_heads * kTile;
+  s.ml = w.take(q_cols * 8);
+  s.o = w.take(std::max(q_cols, k_cols) * a.dim * 4);
+  s.o2 = w.take(k_cols * a.dim * 4);
+  s.g = w.take(std::max(q_cols, k_cols) * 16);
   s.size = w.size;
   return s;
 }
@@ -250,9 +263,9 @@ extern "C" int vsn_attn_create(vsn_attn_handle* out, int device_id, int64_t n, c
     }
     // one-tile fragments go by a kernel of their own where a wave's per-head sums fit its share of LDS
     const bool small = heads <= 64 && (int64_t)heads * a->n_rel <= kSmallSums;
-    ok = upload_side(make_lists(n, qs, qe, host_start, host_end, heads, small, true), a->fwd) &&
-         upload_side(make_lists(n, qs, qe, host_start, host_end, heads, small, false), a->by_query) &&
-         upload_side(make_lists(n, host_start, host_end, qs, qe, kv_heads, small, false), a->by_key) &&
+    ok = upload_side(make_lists(n, qs, qe, host_start, host_end, heads, small), a->fwd) &&
+         upload_side(make_lists(n, qs, qe, host_start, host_end, heads, small), a->by_query) &&
+         upload_side(make_lists(n, host_start, host_end, qs, qe, kv_heads, small), a->by_key) &&
          upload(lut, &a->lut);
   } catch (...) {  // out of host memory
     ok = false;
@@ -325,6 +338,8 @@ extern "C" int vsn_attn_backward(vsn_attn_handle a, const vsn_attn_io* io, const
     p.part_pos_q = (float*)(base + s.pos_q);
     p.part_pos_k = (float*)(base + s.pos_k);
   }
+  p.part_ml = (float2*)(base + s.ml);
+  p.part_o = (float*)(base + s.o), p.part_o2 = (float*)(base + s.o2), p.part_g = (float*)(base + s.g);
   if (g->dslope) p.part_slope = (float*)(base + s.slope);
   if (g->dtable) p.part_hist = (float*)(base + s.hist);
   p.dpos = g->dpos, p.dq_pos = g->dquery_pos, p.dslope = g->dslope, p.dtable = g->dtable;

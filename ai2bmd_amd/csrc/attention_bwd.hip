@@ -10,8 +10,9 @@
 // share.  Seven products instead of five, against a pass that would have to add dq (or dk, dv) across workgroups in an
 // order of its own.  The maximum and the sum are kept apart (not as one logarithm), so P keeps its precision however
 // large the scores are.  D is summed from the scores before anything is rounded (do_i.o_i would carry the rounding of P
-// in the forward product into every float32 gradient): a walk over the keys of its own ahead of the dq pass, except where
-// one tile holds all keys of a fragment, as it does for most fragments, and everything is still in registers.
+// in the forward product into every float32 gradient): a pass of its own ahead of the dq pass, except where one tile
+// holds all keys of a fragment and everything is still in registers.
+// Long runs of rows are split into pieces of equal length (make_lists); a piece leaves float32 sums that a join adds up.
 // P and dS are rounded to the rows' type where they enter a product.  float16 has few exponents for that: P goes in
 // times 2^14, and dS times a power of two per column that follows the largest one seen so far.
 // All sums are in a fixed order; the table's are kept per wave in LDS.
@@ -33,7 +34,20 @@ struct ColumnScale {
   }
 };
 
-template <typename T, int DP, bool COOP>
+// a column of an accumulator as a row of an output
+template <typename O, int DP>
+__device__ __forceinline__ void store_column(O* o, const f32x16 (&c)[DP / 32], float f, int dim, int hi) {
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int e = d * 32 + 8 * g + 4 * hi;
+      if (e < dim) store4<O>(o + e, c[d][4 * g] * f, c[d][4 * g + 1] * f, c[d][4 * g + 2] * f, c[d][4 * g + 3] * f);
+    }
+}
+
+// DELTA: the pass for D of fragments of several tiles; else the dq pass
+template <typename T, int DP, bool COOP, bool DELTA>
 __global__ __launch_bounds__(256, (tile_waves<T, DP>())) void k_attn_bwd_q(AttnParams p, size_t lds_per_wave) {
   extern __shared__ __attribute__((aligned(16))) char lds_raw[];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, lane_of_wave = lane;
@@ -48,7 +62,7 @@ __global__ __launch_bounds__(256, (tile_waves<T, DP>())) void k_attn_bwd_q(AttnP
   const AttnLds<T, DP> lds(base);
   float* hist_all = lds.tab + p.n_rel;  // one histogram per wave
   float* hist = hist_all + (COOP ? wave * p.n_rel : 0);
-  const bool count = p.part_hist != nullptr;
+  const bool count = !DELTA && p.part_hist != nullptr;
 
   const int kv = uniform(head / (p.heads / p.kv_heads));
   const T* kp = (const T*)p.k + kv * p.k_head;
@@ -67,6 +81,8 @@ __global__ __launch_bounds__(256, (tile_waves<T, DP>())) void k_attn_bwd_q(AttnP
     const bool busy = (COOP ? wave * kTile : 0) < w.cols;
     const bool whole = (COOP ? wave * kTile : 0) + kTile <= w.cols;
     const int64_t row = (int64_t)w.col0 + (live ? mine : 0);
+    const bool once = w.slot < 0 && w.row1 - w.row0 <= kTile;
+    if (DELTA && once) continue;
 
     typename vec8<T>::type qf[DP / 16], df[DP / 16];
     const T* qp = (const T*)p.q + row * p.q_row + head * p.q_head;
@@ -81,7 +97,11 @@ __global__ __launch_bounds__(256, (tile_waves<T, DP>())) void k_attn_bwd_q(AttnP
     float px = 0, py = 0, pz = 0;
     LongSum gx, gy, gz;
     if (p.slope) px = p.q_pos[3 * row], py = p.q_pos[3 * row + 1], pz = p.q_pos[3 * row + 2];
-    const int res = p.table ? p.q_res[row] : 0;
+    int res = 0, res_lo = 0, res_hi = 0;
+    if (p.table) {
+      res = p.q_res[row];
+      column_range(res, res_lo, res_hi);
+    }
 
     f32x16 dq[DP / 32];
 #pragma unroll
@@ -94,8 +114,20 @@ __global__ __launch_bounds__(256, (tile_waves<T, DP>())) void k_attn_bwd_q(AttnP
       tiles.load(kp + w.row0 * p.k_row, p.k_row, vp + w.row0 * p.v_row, p.v_row, w.row1 - w.row0, p.dim, tid);
     float delta = 0.f, inv_l = 0.f;
     LongSum sum_e, sum_edp;
-    const bool once = w.row1 - w.row0 <= kTile;
-    bool sum_delta = true;  // the walk for D (with `once`: that tile itself)
+    if (!DELTA && !once) {
+      if (w.slot < 0) {
+        const float2 d = p.delta[head * p.rows_q + row];
+        delta = d.x, inv_l = d.y;
+      } else {
+        float e = 0.f, edp = 0.f;
+        for (int i = 0; i < w.slots; ++i) {
+          const float2 d = p.part_ml[((int64_t)(w.slot0 + (COOP ? wave : 0) + i * w.step) * p.heads + head) * kTile + col];
+          if (live) e += d.x, edp += d.y;
+        }
+        inv_l = e == 0.f ? 0.f : 1.f / e;
+        delta = edp * inv_l;
+      }
+    }
     for (int k0 = w.row0; k0 < w.row1;) {
       const int n = w.row1 - k0 < kTile ? w.row1 - k0 : kTile;
       if (!AHEAD) tiles.load(kp + k0 * p.k_row, p.k_row, vp + k0 * p.v_row, p.v_row, n, p.dim, tid);
@@ -107,9 +139,7 @@ __global__ __launch_bounds__(256, (tile_waves<T, DP>())) void k_attn_bwd_q(AttnP
         if (p.table) lds.res[tid] = p.k_res[kr];
       }
       tile_sync<COOP>();
-      const bool first = sum_delta;
       k0 += kTile;
-      if (first && !once && k0 >= w.row1) k0 = w.row0, sum_delta = false;
       if (AHEAD && k0 < w.row1)
         tiles.load(kp + k0 * p.k_row, p.k_row, vp + k0 * p.v_row, p.v_row, w.row1 - k0, p.dim, tid);
       if (!busy) continue;
@@ -133,9 +163,17 @@ __global__ __launch_bounds__(256, (tile_waves<T, DP>())) void k_attn_bwd_q(AttnP
           s[r] -= slope2 * pair_dist(px - k.x, py - k.y, pz - k.z, inv);
         }
       }
+      int end = -1;
       if (p.table) {
+        end = clipped_end(lds.res[col], res_lo, res_hi, 1, p.reach);
+        if (end >= 0) {
+          const float t = lds.tab[end];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] += lds.tab[rel_index(lds.res[acc_row(r, hi)], res, p.reach)];
+          for (int r = 0; r < 16; ++r) s[r] += t;
+        } else {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[r] += lds.tab[rel_index(lds.res[acc_row(r, hi)], res, p.reach)];
+        }
       }
       if (n < kTile || !whole) {
         const int limit = live ? n : 0;
@@ -144,19 +182,17 @@ __global__ __launch_bounds__(256, (tile_waves<T, DP>())) void k_attn_bwd_q(AttnP
       }
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(s[r] - ref);
-      if (first) {
+      if (DELTA || once) {
         // the sum of exponentials once more, from the very values that D is summed from: then sum_j dS_ij is 0
         float t[16];
 #pragma unroll
         for (int r = 0; r < 16; ++r) t[r] = s[r] * dp[r];
         sum_e.add(tile_sum(s));
         sum_edp.add(tile_sum(t));
-        if (once || !sum_delta) {
-          const float l = sum_e.both_halves();
-          inv_l = l == 0.f ? 0.f : 1.f / l;
-          delta = sum_edp.both_halves() * inv_l;
-        }
-        if (!once) continue;
+        if (DELTA) continue;
+        const float l = sum_e.both_halves();
+        inv_l = l == 0.f ? 0.f : 1.f / l;
+        delta = sum_edp.both_halves() * inv_l;
       }
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] *= inv_l * (dp[r] - delta);  // dS from here on
@@ -176,7 +212,9 @@ __global__ __launch_bounds__(256, (tile_waves<T, DP>())) void k_attn_bwd_q(AttnP
         dslope.add(ts);
         gx.add(tx), gy.add(ty), gz.add(tz);
       }
-      if (count) {
+      if (count && end >= 0) {
+        (end ? high : low).add(tile_sum(s));
+      } else if (count) {
         // runs of keys of one residue are added up in the lane first; the clipped ends stay in the lane altogether
         float run = 0.f, first_end = 0.f, last_end = 0.f;
         int at = rel_index(lds.res[acc_row(0, hi)], res, p.reach);
@@ -220,27 +258,35 @@ __global__ __launch_bounds__(256, (tile_waves<T, DP>())) void k_attn_bwd_q(AttnP
       }
     }
 
+    const int64_t part = ((int64_t)(w.slot + (COOP ? wave : 0)) * p.heads + head) * kTile + col;  // of a piece
+    if (DELTA) {
+      const float e = sum_e.both_halves(), edp = sum_edp.both_halves(), inv = e == 0.f ? 0.f : 1.f / e;
+      if (live && hi == 0) {
+        if (w.slot >= 0)
+          p.part_ml[part] = make_float2(e, edp);
+        else
+          p.delta[head * p.rows_q + row] = make_float2(edp * inv, inv);
+      }
+      continue;
+    }
     if (p.part_pos_q) {
       const float x = gx.both_halves(), y = gy.both_halves(), z = gz.both_halves();
       if (live && hi == 0) {
-        float* g = p.part_pos_q + (head * p.rows_q + row) * 3;
+        float* g = w.slot >= 0 ? p.part_g + part * 4 : p.part_pos_q + (head * p.rows_q + row) * 3;
         g[0] = -slope * x, g[1] = -slope * y, g[2] = -slope * z;
       }
     }
     if (live && hi == 0) p.delta[head * p.rows_q + row] = make_float2(delta, inv_l);
     if (live) {
       const float f = HALF ? p.scale / cs.f : p.scale;
-      T* o = (T*)p.dq + (row * p.heads + head) * p.dim;
-#pragma unroll
-      for (int d = 0; d < DP / 32; ++d)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const int e = d * 32 + 8 * g + 4 * hi;
-          if (e < p.dim) store4<T>(o + e, dq[d][4 * g] * f, dq[d][4 * g + 1] * f, dq[d][4 * g + 2] * f, dq[d][4 * g + 3] * f);
-        }
+      if (w.slot >= 0)
+        store_column<float, DP>(p.part_o + part * p.dim, dq, f, p.dim, hi);
+      else
+        store_column<T, DP>((T*)p.dq + (row * p.heads + head) * p.dim, dq, f, p.dim, hi);
     }
   }
 
+  if (DELTA) return;
   const int64_t part = p.part0 + worker;
   if (p.part_slope) {
     const float sum = wave_sum(dslope.value());
@@ -301,7 +347,11 @@ __global__ __launch_bounds__(256, (tile_waves<T, DP>())) void k_attn_bwd_k(AttnP
   float px = 0, py = 0, pz = 0;
   LongSum gx, gy, gz;
   if (p.slope) px = p.k_pos[3 * row], py = p.k_pos[3 * row + 1], pz = p.k_pos[3 * row + 2];
-  const int res = p.table ? p.k_res[row] : 0;
+  int res = 0, res_lo = 0, res_hi = 0;
+  if (p.table) {
+    res = p.k_res[row];
+    column_range(res, res_lo, res_hi);
+  }
 
   f32x16 dk[DP / 32], dv[DP / 32];
 #pragma unroll
@@ -362,8 +412,15 @@ __global__ __launch_bounds__(256, (tile_waves<T, DP>())) void k_attn_bwd_k(AttnP
         }
       }
       if (p.table) {
+        const int end = clipped_end(lds.res[col], res_lo, res_hi, -1, p.reach);
+        if (end >= 0) {
+          const float t = lds.tab[end];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] += lds.tab[rel_index(res, lds.res[acc_row(r, hi)], p.reach)];
+          for (int r = 0; r < 16; ++r) s[r] += t;
+        } else {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[r] += lds.tab[rel_index(res, lds.res[acc_row(r, hi)], p.reach)];
+        }
       }
       if (n < kTile || !whole) {
         const int limit = live ? n : 0;
@@ -415,40 +472,66 @@ __global__ __launch_bounds__(256, (tile_waves<T, DP>())) void k_attn_bwd_k(AttnP
     }
   }
 
+  const int64_t part = ((int64_t)(w.slot + (COOP ? wave : 0)) * p.kv_heads + kv) * kTile + col;  // of a piece
   if (p.part_pos_k) {
     const float x = gx.both_halves(), y = gy.both_halves(), z = gz.both_halves();
     if (live && hi == 0) {
-      float* g = p.part_pos_k + (kv * p.rows_k + row) * 3;
+      float* g = w.slot >= 0 ? p.part_g + part * 4 : p.part_pos_k + (kv * p.rows_k + row) * 3;
       g[0] = x, g[1] = y, g[2] = z;
     }
   }
   if (!live) return;
   const float f = HALF ? p.scale / cs.f : p.scale;
   constexpr float PDOWN = 1.f / PUP;
-  T* ok = (T*)p.dk + (row * p.kv_heads + kv) * p.dim;
-  T* ov = (T*)p.dv + (row * p.kv_heads + kv) * p.dim;
-#pragma unroll
-  for (int d = 0; d < DP / 32; ++d)
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int e = d * 32 + 8 * g + 4 * hi;
-      if (e >= p.dim) continue;
-      store4<T>(ok + e, dk[d][4 * g] * f, dk[d][4 * g + 1] * f, dk[d][4 * g + 2] * f, dk[d][4 * g + 3] * f);
-      store4<T>(ov + e, dv[d][4 * g] * PDOWN, dv[d][4 * g + 1] * PDOWN, dv[d][4 * g + 2] * PDOWN, dv[d][4 * g + 3] * PDOWN);
+  if (w.slot >= 0) {
+    store_column<float, DP>(p.part_o + part * p.dim, dk, f, p.dim, hi);
+    store_column<float, DP>(p.part_o2 + part * p.dim, dv, PDOWN, p.dim, hi);
+  } else {
+    store_column<T, DP>((T*)p.dk + (row * p.kv_heads + kv) * p.dim, dk, f, p.dim, hi);
+    store_column<T, DP>((T*)p.dv + (row * p.kv_heads + kv) * p.dim, dv, PDOWN, p.dim, hi);
+  }
+}
+
+// Adds up the pieces of a block of columns: one workgroup per (block, head), a thread per four elements of a column.
+template <typename T>
+__global__ __launch_bounds__(256) void k_attn_bwd_pieces(AttnParams p, int heads, T* out, T* out2, float* pos, int64_t rows) {
+  const AttnJoin j = p.join[blockIdx.x];
+  const int head = blockIdx.y, quads = p.dim / 4;
+  for (int i = threadIdx.x; i < j.cols * quads; i += 256) {
+    const int col = i / quads, d = i % quads * 4;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+    for (int s = 0; s < j.slots; ++s) {
+      const int64_t at = (((int64_t)(j.slot0 + s * j.step) * heads + head) * kTile + col) * p.dim + d;
+      const float4 x = *(const float4*)(p.part_o + at);
+      a.x += x.x, a.y += x.y, a.z += x.z, a.w += x.w;
+      if (out2) {
+        const float4 y = *(const float4*)(p.part_o2 + at);
+        b.x += y.x, b.y += y.y, b.z += y.z, b.w += y.w;
+      }
     }
+    const int64_t to = (((int64_t)j.col0 + col) * heads + head) * p.dim + d;
+    store4<T>(out + to, a.x, a.y, a.z, a.w);
+    if (out2) store4<T>(out2 + to, b.x, b.y, b.z, b.w);
+  }
+  if (pos && threadIdx.x < j.cols * 3) {
+    const int col = threadIdx.x / 3, c = threadIdx.x % 3;
+    float t = 0.f;
+    for (int s = 0; s < j.slots; ++s) t += p.part_g[(((int64_t)(j.slot0 + s * j.step) * heads + head) * kTile + col) * 4 + c];
+    pos[(head * rows + j.col0 + col) * 3 + c] = t;
+  }
 }
 
 // Joins the partial sums in a fixed order: positions over heads (a workgroup per work item of the segments), then one
 // workgroup per head for its slope and one per (head, bucket) for the table, both summed in float64.
 struct AttnPosSegment {
-  const AttnWork* work;
-  int count;
-  int of_rows;           // the item's rows (1) or its columns (0)
+  const AttnWork* work;    // small fragments: their rows (of_rows) or columns, or
+  const AttnBlock* block;  // blocks of columns
+  int count, of_rows;
   int parts_q, parts_k;  // partial sums of each side that make up the result
   float* out;
 };
 struct AttnPosJoin {
-  AttnPosSegment seg[6];
+  AttnPosSegment seg[4];
   int n;
 };
 
@@ -458,8 +541,13 @@ __global__ __launch_bounds__(256) void k_attn_bwd_join(AttnParams p, AttnPosJoin
   for (int i = 0; i < join.n; ++i) {
     const AttnPosSegment g = join.seg[i];
     if (b < g.count) {
-      const AttnWork w = g.work[b];
-      const int64_t first = g.of_rows ? w.row0 : w.col0, n = g.of_rows ? w.row1 - w.row0 : w.cols;
+      int64_t first, n;
+      if (g.work) {
+        const AttnWork w = g.work[b];
+        first = g.of_rows ? w.row0 : w.col0, n = g.of_rows ? w.row1 - w.row0 : w.cols;
+      } else {
+        first = g.block[b].col0, n = g.block[b].cols;
+      }
       for (int64_t at = first * 3 + tid; at < (first + n) * 3; at += 256) {
         float t = 0.f;
         for (int h = 0; h < g.parts_k; ++h) t += p.part_pos_k[h * p.rows_k * 3 + at];
@@ -508,6 +596,27 @@ __global__ __launch_bounds__(256) void k_attn_bwd_join(AttnParams p, AttnPosJoin
   if (tid == 0) *out = (float)(red[0] + red[1] + red[2] + red[3]);
 }
 
+template <typename T, int DP, bool DELTA>
+static int q_launch(const AttnPlanView& by_query, AttnParams p, int lone_workers, int coop_workers, size_t lone_bytes,
+                    size_t coop_bytes, hipStream_t st) {
+  if (by_query.lone) {
+    p.work = by_query.lone_work, p.count = by_query.lone, p.workers = DELTA ? by_query.lone : lone_workers, p.part0 = 0;
+    const int64_t total = (int64_t)p.workers * p.heads;
+    const int waves = lone_waves(total, lone_bytes);
+    if (!allow_lds((const void*)k_attn_bwd_q<T, DP, false, DELTA>, waves * lone_bytes)) return -5;
+    hipLaunchKernelGGL((k_attn_bwd_q<T, DP, false, DELTA>), dim3((unsigned)((total + waves - 1) / waves)),
+                       dim3(64 * waves), waves * lone_bytes, st, p, lone_bytes);
+  }
+  if (by_query.coop) {
+    p.work = by_query.coop_work, p.count = by_query.coop, p.workers = DELTA ? by_query.coop : coop_workers;
+    p.part0 = lone_workers;
+    if (!allow_lds((const void*)k_attn_bwd_q<T, DP, true, DELTA>, coop_bytes)) return -5;
+    hipLaunchKernelGGL((k_attn_bwd_q<T, DP, true, DELTA>), dim3((unsigned)((int64_t)p.workers * p.heads)),
+                       dim3(64 * kCoopWaves), coop_bytes, st, p, coop_bytes);
+  }
+  return 0;
+}
+
 template <typename T, int DP>
 static int bwd_launch(const AttnPlanView& by_query, const AttnPlanView& by_key, AttnParams p, int lone_workers,
                       int coop_workers, hipStream_t st) {
@@ -515,19 +624,16 @@ static int bwd_launch(const AttnPlanView& by_query, const AttnPlanView& by_key, 
   const size_t tab = AttnLds<T, DP>::bytes(n_rel);
   const size_t lone_q = AttnLds<T, DP>::bytes(n_rel + (p.part_hist ? p.n_rel : 0));
   const size_t coop_q = AttnLds<T, DP>::bytes(n_rel + (p.part_hist ? kCoopWaves * p.n_rel : 0));
-  if (by_query.lone) {
-    p.work = by_query.lone_work, p.count = by_query.lone, p.workers = lone_workers, p.part0 = 0;
-    const int64_t total = (int64_t)lone_workers * p.heads;
-    const int waves = lone_waves(total, lone_q);
-    if (!allow_lds((const void*)k_attn_bwd_q<T, DP, false>, waves * lone_q)) return -5;
-    hipLaunchKernelGGL((k_attn_bwd_q<T, DP, false>), dim3((unsigned)((total + waves - 1) / waves)), dim3(64 * waves),
-                       waves * lone_q, st, p, lone_q);
+  if (by_query.long_rows) {
+    const int rc = q_launch<T, DP, true>(by_query, p, lone_workers, coop_workers, tab, tab, st);
+    if (rc) return rc;
   }
-  if (by_query.coop) {
-    p.work = by_query.coop_work, p.count = by_query.coop, p.workers = coop_workers, p.part0 = lone_workers;
-    if (!allow_lds((const void*)k_attn_bwd_q<T, DP, true>, coop_q)) return -5;
-    hipLaunchKernelGGL((k_attn_bwd_q<T, DP, true>), dim3((unsigned)((int64_t)coop_workers * p.heads)),
-                       dim3(64 * kCoopWaves), coop_q, st, p, coop_q);
+  const int rc = q_launch<T, DP, false>(by_query, p, lone_workers, coop_workers, lone_q, coop_q, st);
+  if (rc) return rc;
+  if (by_query.joins) {
+    p.join = by_query.join;
+    hipLaunchKernelGGL((k_attn_bwd_pieces<T>), dim3(by_query.joins, p.heads), dim3(256), 0, st, p, p.heads, (T*)p.dq,
+                       (T*)nullptr, p.part_pos_q, p.rows_q);
   }
   if (by_key.lone) {
     p.work = by_key.lone_work, p.count = by_key.lone;
@@ -543,6 +649,11 @@ static int bwd_launch(const AttnPlanView& by_query, const AttnPlanView& by_key, 
     hipLaunchKernelGGL((k_attn_bwd_k<T, DP, true>), dim3((unsigned)((int64_t)by_key.coop * p.kv_heads)),
                        dim3(64 * kCoopWaves), tab, st, p, tab);
   }
+  if (by_key.joins) {
+    p.join = by_key.join;
+    hipLaunchKernelGGL((k_attn_bwd_pieces<T>), dim3(by_key.joins, p.kv_heads), dim3(256), 0, st, p, p.kv_heads,
+                       (T*)p.dk, (T*)p.dv, p.part_pos_k, p.rows_k);
+  }
   return 0;
 }
 
@@ -550,20 +661,18 @@ static int join_launch(const AttnPlanView& by_query, const AttnPlanView& by_key,
                        hipStream_t st) {
   AttnPosJoin join = {};
   int64_t blocks = 0;
-  auto add = [&](const AttnWork* work, int count, int of_rows, int parts_q, int parts_k, float* out) {
+  auto add = [&](const AttnWork* work, const AttnBlock* block, int count, int of_rows, int parts_q, int parts_k, float* out) {
     if (!count) return;
-    join.seg[join.n++] = {work, count, of_rows, parts_q, parts_k, out};
+    join.seg[join.n++] = {work, block, count, of_rows, parts_q, parts_k, out};
     blocks += count;
   };
   if (p.dpos) {
     const bool self = !p.dq_pos;
-    add(by_key.lone_work, by_key.lone, 0, self ? p.heads : 0, p.kv_heads, p.dpos);
-    add(by_key.coop_work, by_key.coop, 0, self ? p.heads : 0, p.kv_heads, p.dpos);
-    if (groups > 1) add(by_query.small_work, by_query.small, 1, self ? groups : 0, groups, p.dpos);
+    add(nullptr, by_key.block, by_key.blocks, 0, self ? p.heads : 0, p.kv_heads, p.dpos);
+    if (groups > 1) add(by_query.small_work, nullptr, by_query.small, 1, self ? groups : 0, groups, p.dpos);
     if (!self) {
-      add(by_query.lone_work, by_query.lone, 0, p.heads, 0, p.dq_pos);
-      add(by_query.coop_work, by_query.coop, 0, p.heads, 0, p.dq_pos);
-      if (groups > 1) add(by_query.small_work, by_query.small, 0, groups, 0, p.dq_pos);
+      add(nullptr, by_query.block, by_query.blocks, 0, p.heads, 0, p.dq_pos);
+      if (groups > 1) add(by_query.small_work, nullptr, by_query.small, 0, groups, 0, p.dq_pos);
     }
   }
   const int n_slope = p.dslope ? p.heads : 0, n_table = p.dtable ? p.heads * p.n_buckets : 0;

@@ -40,9 +40,10 @@ __global__ __launch_bounds__(256, (tile_waves<T, DP>())) void k_attn_fwd(AttnPar
     slope = p.slope[head] * kLog2e;
     px = p.q_pos[3 * row], py = p.q_pos[3 * row + 1], pz = p.q_pos[3 * row + 2];
   }
-  int res = 0;
+  int res = 0, res_lo = 0, res_hi = 0;
   if (p.table) {
     res = p.q_res[row];
+    column_range(res, res_lo, res_hi);
     for (int i = tid; i < p.n_rel; i += THREADS) lds.tab[i] = table_log2(p.table[(int64_t)head * p.n_buckets + p.lut[i]]);
   }
 
@@ -89,8 +90,15 @@ __global__ __launch_bounds__(256, (tile_waves<T, DP>())) void k_attn_fwd(AttnPar
       }
     }
     if (p.table) {
+      const int end = clipped_end(lds.res[col], res_lo, res_hi, 1, p.reach);
+      if (end >= 0) {  // far along the chain: one entry for the whole tile
+        const float t = lds.tab[end];
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] += lds.tab[rel_index(lds.res[acc_row(r, hi)], res, p.reach)];
+        for (int r = 0; r < 16; ++r) s[r] += t;
+      } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] += lds.tab[rel_index(lds.res[acc_row(r, hi)], res, p.reach)];
+      }
     }
     if (n < kTile || !whole) {
       const int limit = live ? n : 0;
@@ -126,7 +134,7 @@ __global__ __launch_bounds__(256, (tile_waves<T, DP>())) void k_attn_fwd(AttnPar
   const float total = l.both_halves();
   if (!live) return;
   if (w.slot >= 0) {
-    const int64_t at = ((int64_t)w.slot * p.heads + head) * kTile + col;
+    const int64_t at = ((int64_t)(w.slot + (COOP ? wave : 0)) * p.heads + head) * kTile + col;
     if (hi == 0) p.part_ml[at] = make_float2(m, total);
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d)
@@ -161,7 +169,7 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnParams p) {
   const int col = blockIdx.x % kTile, head = blockIdx.y, tid = threadIdx.x;
   if (col >= j.cols) return;
   float m = -INFINITY;
-  for (int s = tid; s < j.slots; s += 256) m = fmaxf(m, p.part_ml[((int64_t)(j.slot0 + s) * p.heads + head) * kTile + col].x);
+  for (int s = tid; s < j.slots; s += 256) m = fmaxf(m, p.part_ml[((int64_t)(j.slot0 + s * j.step) * p.heads + head) * kTile + col].x);
   for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
   if ((tid & 63) == 0) red[tid >> 6] = m;
   __syncthreads();
@@ -169,7 +177,7 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnParams p) {
   const float ref = m == -INFINITY ? 0.f : m;
   float l = 0.f;
   for (int s = tid; s < j.slots; s += 256) {
-    const float2 ml = p.part_ml[((int64_t)(j.slot0 + s) * p.heads + head) * kTile + col];
+    const float2 ml = p.part_ml[((int64_t)(j.slot0 + s * j.step) * p.heads + head) * kTile + col];
     weight[s] = __builtin_amdgcn_exp2f(ml.x - ref);
     l += weight[s] * ml.y;
   }
@@ -183,7 +191,7 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnParams p) {
   float4 a = make_float4(0, 0, 0, 0);
   if (g < groups)
     for (int s = g; s < j.slots; s += groups) {
-      const float4 o = *(const float4*)(p.part_o + (((int64_t)(j.slot0 + s) * p.heads + head) * kTile + col) * p.dim + d);
+      const float4 o = *(const float4*)(p.part_o + (((int64_t)(j.slot0 + s * j.step) * p.heads + head) * kTile + col) * p.dim + d);
       const float f = weight[s];
       a.x += f * o.x, a.y += f * o.y, a.z += f * o.z, a.w += f * o.w;
     }

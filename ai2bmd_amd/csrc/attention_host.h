@@ -9,9 +9,15 @@ constexpr size_t kLdsPerCu = 160 * 1024;
 
 // the work lists of one pass: `small` items are fragments of one tile, `lone` items a wave each with tiles of its own,
 // `coop` items a workgroup of four
+struct AttnBlock {
+  int col0, cols;
+};
 struct AttnPlanView {
   const AttnWork *small_work, *lone_work, *coop_work;
   int small, lone, coop;
+  int long_rows;  // whether an item has more than one tile of rows
+  const AttnBlock* block;  // runs of columns of the lone and coop items
+  int blocks;
   const AttnJoin* join;
   int joins;
 };

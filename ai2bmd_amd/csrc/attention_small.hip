@@ -182,7 +182,7 @@ __global__ __launch_bounds__(256) void k_attn_small_fwd(AttnParams p, size_t per
   const AttnWork w = load_work(p.work, uniform(id / groups));
   const int nq = w.cols, nk = w.row1 - w.row0;
   const bool live = col < nq;
-  const int64_t q_row = (int64_t)w.col0 + (live ? col : 0), k_row = (int64_t)w.row0 + (col < nk ? col : 0);
+  const int64_t q_row = (int64_t)w.col0 + (live ? col : 0);
   SmallGeometry g;
   small_geometry<T, DP>(p, w, lds, g, nk, q_row, lane, col, hi);
   const float scale = p.scale * kLog2e;
