@@ -253,13 +253,35 @@ __device__ __forceinline__ float pair_dist(float dx, float dy, float dz, float& 
 // index of the clipped difference of two residue numbers; the difference saturates
 __device__ __forceinline__ int rel_index(int key_res, int query_res, int reach) {
   const int d = __builtin_elementwise_sub_sat(key_res, query_res);
-  return (d < -reach ? -reach : d > reach ? reach : d) + reach;
+  return __builtin_elementwise_min(__builtin_elementwise_max(d, -reach), reach) + reach;
 }
 
 // a table entry in units of log 2; the lowest float32 stays a finite value (a mask of it must not turn into -inf)
 __device__ __forceinline__ float table_log2(float t) {
   const float v = t * kLog2e;
   return fabsf(t) < INFINITY ? __builtin_amdgcn_fmed3f(v, -3.4028235e38f, 3.4028235e38f) : v;
+}
+
+// This head's table by clipped difference, in LDS.  Loads go out eight at a time: one after the other, two dependent
+// loads per 64 entries cost a wave of a 257-entry table more than its tiles.
+__device__ __forceinline__ void expand_table(float* tab, const float* table, const int* lut, int n_rel, int tid,
+                                             int threads) {
+  for (int base = 0; base < n_rel; base += 8 * threads) {
+    int at[8];
+    float v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int i = base + k * threads + tid;
+      at[k] = lut[i < n_rel ? i : 0];
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = table[at[k]];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int i = base + k * threads + tid;
+      if (i < n_rel) tab[i] = table_log2(v[k]);
+    }
+  }
 }
 
 // c += a * b over one tile of 32 rows
@@ -323,12 +345,17 @@ struct LongSum {
   __device__ __forceinline__ float value() const { return s + c; }
 };
 
-// Waves per SIMD that the tile kernels are compiled for.  16-bit rows of up to 32 columns fit three without spilling
-// (17 882 atoms: dq pass 10.2 -> 8.1 ms, dk / dv pass 5.6 -> 4.3 ms, forward 2.8 -> 2.6 ms; four spill and lose it again);
-// wider or float32 rows are left to the compiler.
+// Waves per SIMD that the tile kernels are compiled for: as many as fit without spilling, left alone the compiler hoists
+// its loads into twice the registers.  Three against one or two at 17 882 atoms bf16, dim 32: dq pass 10.2 -> 8.1 ms, dk / dv
+// pass 5.6 -> 4.3 ms (four spill and lose it again); two against one at 6007 atoms f16, dim 64: dq pass 1003 -> 607 us,
+// dk / dv pass 867 -> 530 us, forward 324 -> 226 us.
 template <typename T, int DP>
-constexpr int tile_waves() {
-  return sizeof(T) == 2 && DP <= 32 ? 3 : 1;
+constexpr int forward_waves() {
+  return DP <= 32 ? 3 : DP > 64 && sizeof(T) == 4 ? 1 : 2;
+}
+template <typename T, int DP>
+constexpr int backward_waves() {
+  return DP <= 32 && sizeof(T) == 2 ? 3 : DP <= 64 ? 2 : 1;
 }
 
 // wave-private (or shared) LDS of one work item

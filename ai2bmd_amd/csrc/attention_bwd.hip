@@ -48,7 +48,7 @@ __device__ __forceinline__ void store_column(O* o, const f32x16 (&c)[DP / 32], f
 
 // DELTA: the pass for D of fragments of several tiles; else the dq pass
 template <typename T, int DP, bool COOP, bool DELTA>
-__global__ __launch_bounds__(256, (tile_waves<T, DP>())) void k_attn_bwd_q(AttnParams p, size_t lds_per_wave) {
+__global__ __launch_bounds__(256, (backward_waves<T, DP>())) void k_attn_bwd_q(AttnParams p, size_t lds_per_wave) {
   extern __shared__ __attribute__((aligned(16))) char lds_raw[];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, lane_of_wave = lane;
   const int col = lane & 31, hi = lane >> 5;
@@ -68,8 +68,7 @@ __global__ __launch_bounds__(256, (tile_waves<T, DP>())) void k_attn_bwd_q(AttnP
   const T* kp = (const T*)p.k + kv * p.k_head;
   const T* vp = (const T*)p.v + kv * p.v_head;
   const float slope = p.slope ? p.slope[head] : 0.f, slope2 = slope * kLog2e, scale = p.scale * kLog2e;
-  if (p.table)
-    for (int i = tid; i < p.n_rel; i += THREADS) lds.tab[i] = table_log2(p.table[(int64_t)head * p.n_buckets + p.lut[i]]);
+  if (p.table) expand_table(lds.tab, p.table + (int64_t)head * p.n_buckets, p.lut, p.n_rel, tid, THREADS);
   if (count)
     for (int i = lane; i < p.n_rel; i += 64) hist[i] = 0.f;
   LongSum dslope, low, high;  // low, high: the two clipped ends of the table
@@ -317,7 +316,7 @@ __global__ __launch_bounds__(256, (tile_waves<T, DP>())) void k_attn_bwd_q(AttnP
 }
 
 template <typename T, int DP, bool COOP>
-__global__ __launch_bounds__(256, (tile_waves<T, DP>())) void k_attn_bwd_k(AttnParams p, size_t lds_per_wave) {
+__global__ __launch_bounds__(256, (backward_waves<T, DP>())) void k_attn_bwd_k(AttnParams p, size_t lds_per_wave) {
   extern __shared__ __attribute__((aligned(16))) char lds_raw[];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, lane_of_wave = lane;
   const int col = lane & 31, hi = lane >> 5;
@@ -367,7 +366,7 @@ __global__ __launch_bounds__(256, (tile_waves<T, DP>())) void k_attn_bwd_k(AttnP
     const float slope = p.slope ? p.slope[head] : 0.f, slope2 = slope * kLog2e;
     if (p.table) {
       tile_sync<COOP>();
-      for (int i = tid; i < p.n_rel; i += THREADS) lds.tab[i] = table_log2(p.table[(int64_t)head * p.n_buckets + p.lut[i]]);
+      expand_table(lds.tab, p.table + (int64_t)head * p.n_buckets, p.lut, p.n_rel, tid, THREADS);
     }
     TilePair<T, DP, THREADS> tiles;
     constexpr bool AHEAD = TilePair<T, DP, THREADS>::N <= 8;
@@ -500,6 +499,7 @@ __global__ __launch_bounds__(256) void k_attn_bwd_pieces(AttnParams p, int heads
   for (int i = threadIdx.x; i < j.cols * quads; i += 256) {
     const int col = i / quads, d = i % quads * 4;
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+#pragma unroll 4
     for (int s = 0; s < j.slots; ++s) {
       const int64_t at = (((int64_t)(j.slot0 + s * j.step) * heads + head) * kTile + col) * p.dim + d;
       const float4 x = *(const float4*)(p.part_o + at);
@@ -559,7 +559,8 @@ __global__ __launch_bounds__(256) void k_attn_bwd_join(AttnParams p, AttnPosJoin
     b -= g.count;
   }
   __shared__ double red[4];
-  __shared__ int lut[2 * kMaxReach + 1];
+  __shared__ int rels[2 * kMaxReach + 1];
+  __shared__ int n_rels;
   double t = 0.0;
   float* out;
   if (b < n_slope) {
@@ -574,20 +575,29 @@ __global__ __launch_bounds__(256) void k_attn_bwd_join(AttnParams p, AttnPosJoin
     out = p.dslope + b;
   } else {
     const int at = b - n_slope, head = at / p.n_buckets, bucket = at % p.n_buckets;
-    for (int i = tid; i < p.n_rel; i += 256) lut[i] = p.lut[i];
-    __syncthreads();
-    // as many lanes along the partial sums as there are, the others along the differences
-    const int along = p.parts > 128 ? 256 : p.parts > 64 ? 128 : 64, step = 256 / along;
-    for (int rel = tid / along; rel < p.n_rel; rel += step)
-      if (lut[rel] == bucket) {
-        const float* part = p.part_hist + ((int64_t)head * p.n_rel + rel) * p.parts;
-        float u[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int i = tid % along; i < p.parts; i += 4 * along)
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            if (i + k * along < p.parts) u[k] += part[i + k * along];
-        t += ((double)u[0] + u[1]) + ((double)u[2] + u[3]);
+    if (tid < 64) {  // the differences of this bucket, in their order
+      int n = 0;
+      for (int base = 0; base < p.n_rel; base += 64) {
+        const bool hit = base + tid < p.n_rel && p.lut[base + tid] == bucket;
+        const uint64_t mask = __ballot(hit);
+        if (hit) rels[n + __popcll(mask & ((1ull << tid) - 1))] = base + tid;
+        n += __popcll(mask);
       }
+      if (tid == 0) n_rels = n;
+    }
+    __syncthreads();
+    const float* part = p.part_hist + (int64_t)head * p.n_rel * p.parts;
+    const int total = n_rels * p.parts;  // (workers() bounds n_rel * parts)
+    for (int i = tid; i < total; i += 8 * 256) {
+      float u[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int e = i + k * 256;
+        u[k] = e < total ? part[(int64_t)rels[e / p.parts] * p.parts + e % p.parts] : 0.f;
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) t += u[k];
+    }
     out = p.dtable + at;
   }
   for (int o = 32; o > 0; o >>= 1) t += __shfl_xor(t, o, 64);

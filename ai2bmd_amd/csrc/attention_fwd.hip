@@ -9,7 +9,7 @@
 namespace vsn {
 
 template <typename T, int DP, bool COOP>
-__global__ __launch_bounds__(256, (tile_waves<T, DP>())) void k_attn_fwd(AttnParams p, size_t lds_per_wave) {
+__global__ __launch_bounds__(256, (forward_waves<T, DP>())) void k_attn_fwd(AttnParams p, size_t lds_per_wave) {
   extern __shared__ __attribute__((aligned(16))) char lds_raw[];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, lane_of_wave = lane;
   const int col = lane & 31, hi = lane >> 5;
@@ -44,7 +44,7 @@ __global__ __launch_bounds__(256, (tile_waves<T, DP>())) void k_attn_fwd(AttnPar
   if (p.table) {
     res = p.q_res[row];
     column_range(res, res_lo, res_hi);
-    for (int i = tid; i < p.n_rel; i += THREADS) lds.tab[i] = table_log2(p.table[(int64_t)head * p.n_buckets + p.lut[i]]);
+    expand_table(lds.tab, p.table + (int64_t)head * p.n_buckets, p.lut, p.n_rel, tid, THREADS);
   }
 
   f32x16 o[DP / 32];
@@ -158,18 +158,49 @@ __global__ __launch_bounds__(256, (tile_waves<T, DP>())) void k_attn_fwd(AttnPar
     }
 }
 
-// Joins the partial results of split keys: one workgroup per (query row, head).  The slots' weights exp(m_s - max m) are
-// put in LDS first, then dim / 4 lanes x (256 / (dim / 4)) groups of slots add up the rows.
+// Joins the pieces' outputs, each weighted by 2^(m_s - max m).  A few pieces: one workgroup per (block of columns, head),
+// a thread per four elements of a column, which finds the weights itself.
 template <typename T>
 __global__ __launch_bounds__(256) void k_attn_join(AttnParams p) {
+  const AttnJoin j = p.join[blockIdx.x];
+  const int head = blockIdx.y, quads = p.dim / 4;
+  for (int i = threadIdx.x; i < j.cols * quads; i += 256) {
+    const int col = i / quads, d = i % quads * 4;
+    const int64_t first = ((int64_t)j.slot0 * p.heads + head) * kTile + col, step = (int64_t)j.step * p.heads * kTile;
+    float m = -INFINITY;
+#pragma unroll 8
+    for (int s = 0; s < j.slots; ++s) m = fmaxf(m, p.part_ml[first + s * step].x);
+    const float ref = m == -INFINITY ? 0.f : m;
+    float l = 0.f;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int s = 0; s < j.slots; ++s) {
+      const float2 ml = p.part_ml[first + s * step];
+      const float4 o = *(const float4*)(p.part_o + (first + s * step) * p.dim + d);
+      const float f = __builtin_amdgcn_exp2f(ml.x - ref);
+      l += f * ml.y;
+      a.x += f * o.x, a.y += f * o.y, a.z += f * o.z, a.w += f * o.w;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int64_t row = (int64_t)j.col0 + col;
+    store4<T>((T*)p.out + row * p.out_row + head * p.out_head + d, a.x * inv, a.y * inv, a.z * inv, a.w * inv);
+    if (d == 0 && p.stats) p.stats[head * p.rows_q + row] = make_float2(m, l);
+  }
+}
+
+// Many pieces: one workgroup per (column, head).  The weights are put in LDS first, then dim / 4 lanes x (256 / (dim / 4))
+// groups of pieces add up the rows.
+template <typename T>
+__global__ __launch_bounds__(256) void k_attn_join_many(AttnParams p) {
   __shared__ float weight[kMaxSlots];
   __shared__ float red[8];
   __shared__ float4 sum[256];
   const AttnJoin j = p.join[blockIdx.x / kTile];
   const int col = blockIdx.x % kTile, head = blockIdx.y, tid = threadIdx.x;
   if (col >= j.cols) return;
+  const int64_t first = ((int64_t)j.slot0 * p.heads + head) * kTile + col, step = (int64_t)j.step * p.heads * kTile;
   float m = -INFINITY;
-  for (int s = tid; s < j.slots; s += 256) m = fmaxf(m, p.part_ml[((int64_t)(j.slot0 + s * j.step) * p.heads + head) * kTile + col].x);
+  for (int s = tid; s < j.slots; s += 256) m = fmaxf(m, p.part_ml[first + s * step].x);
   for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
   if ((tid & 63) == 0) red[tid >> 6] = m;
   __syncthreads();
@@ -177,7 +208,7 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnParams p) {
   const float ref = m == -INFINITY ? 0.f : m;
   float l = 0.f;
   for (int s = tid; s < j.slots; s += 256) {
-    const float2 ml = p.part_ml[((int64_t)(j.slot0 + s * j.step) * p.heads + head) * kTile + col];
+    const float2 ml = p.part_ml[first + s * step];
     weight[s] = __builtin_amdgcn_exp2f(ml.x - ref);
     l += weight[s] * ml.y;
   }
@@ -191,7 +222,7 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnParams p) {
   float4 a = make_float4(0, 0, 0, 0);
   if (g < groups)
     for (int s = g; s < j.slots; s += groups) {
-      const float4 o = *(const float4*)(p.part_o + (((int64_t)(j.slot0 + s * j.step) * p.heads + head) * kTile + col) * p.dim + d);
+      const float4 o = *(const float4*)(p.part_o + (first + s * step) * p.dim + d);
       const float f = weight[s];
       a.x += f * o.x, a.y += f * o.y, a.z += f * o.z, a.w += f * o.w;
     }
@@ -202,8 +233,7 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnParams p) {
       const float4 o = sum[k * lanes + tid];
       a.x += o.x, a.y += o.y, a.z += o.z, a.w += o.w;
     }
-    a.x *= inv, a.y *= inv, a.z *= inv, a.w *= inv;
-    store4<T>((T*)p.out + row * p.out_row + head * p.out_head + d, a.x, a.y, a.z, a.w);
+    store4<T>((T*)p.out + row * p.out_row + head * p.out_head + d, a.x * inv, a.y * inv, a.z * inv, a.w * inv);
   }
   if (tid == 0 && p.stats) p.stats[head * p.rows_q + row] = make_float2(m, l);
 }
@@ -225,9 +255,13 @@ static int fwd_launch(const AttnPlanView& plan, AttnParams p, hipStream_t st) {
     hipLaunchKernelGGL((k_attn_fwd<T, DP, true>), dim3((unsigned)((int64_t)plan.coop * p.heads)),
                        dim3(64 * kCoopWaves), bytes, st, p, bytes);
   }
-  if (plan.joins) {
+  if (plan.few) {
     p.join = plan.join;
-    hipLaunchKernelGGL((k_attn_join<T>), dim3(plan.joins * kTile, p.heads), dim3(256), 0, st, p);
+    hipLaunchKernelGGL((k_attn_join<T>), dim3(plan.few, p.heads), dim3(256), 0, st, p);
+  }
+  if (plan.joins > plan.few) {
+    p.join = plan.join + plan.few;
+    hipLaunchKernelGGL((k_attn_join_many<T>), dim3((plan.joins - plan.few) * kTile, p.heads), dim3(256), 0, st, p);
   }
   return hipGetLastError() == hipSuccess ? 0 : -5;
 }

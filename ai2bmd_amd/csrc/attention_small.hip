@@ -171,8 +171,8 @@ __global__ __launch_bounds__(256) void k_attn_small_fwd(AttnParams p, size_t per
   const int col = lane & 31, hi = lane >> 5;
   float* tab = (float*)lds_raw;  // [heads][n_rel]
   const int n_rel = p.table ? p.n_rel : 0;
-  for (int i = threadIdx.x; i < p.heads * n_rel; i += blockDim.x)
-    tab[i] = table_log2(p.table[(int64_t)(i / n_rel) * p.n_buckets + p.lut[i % n_rel]]);
+  for (int h = 0; n_rel && h < p.heads; ++h)
+    expand_table(tab + h * n_rel, p.table + (int64_t)h * p.n_buckets, p.lut, n_rel, threadIdx.x, blockDim.x);
   float* slopes = tab + p.heads * n_rel;  // [heads]
   for (int i = threadIdx.x; i < p.heads; i += blockDim.x) slopes[i] = p.slope ? p.slope[i] : 0.f;
   __syncthreads();
@@ -245,8 +245,8 @@ __global__ __launch_bounds__(256, (small_waves<T, DP>())) void k_attn_small_bwd(
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane_of_wave = threadIdx.x & 63;
   float* tab = (float*)lds_raw;
   const int n_rel = p.table ? p.n_rel : 0;
-  for (int i = threadIdx.x; i < p.heads * n_rel; i += blockDim.x)
-    tab[i] = table_log2(p.table[(int64_t)(i / n_rel) * p.n_buckets + p.lut[i % n_rel]]);
+  for (int h = 0; n_rel && h < p.heads; ++h)
+    expand_table(tab + h * n_rel, p.table + (int64_t)h * p.n_buckets, p.lut, n_rel, threadIdx.x, blockDim.x);
   float* slopes = tab + p.heads * n_rel;  // [heads]
   for (int i = threadIdx.x; i < p.heads; i += blockDim.x) slopes[i] = p.slope ? p.slope[i] : 0.f;
   __syncthreads();
