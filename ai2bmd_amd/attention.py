@@ -109,10 +109,13 @@ class FragmentAttention:
     # -- arguments ---------------------------------------------------------------------------------------------------
     def _rows(self, t, name: str, heads: int, least: int, dtype, exact=None):
         """The tensor as it is where the kernels can address it (dense last axis, 16-byte steps), else a copy."""
-        on_device(t, name, self.device)
+        if not t.is_cuda or t.device != self.device:
+            on_device(t, name, self.device)
         if t.dtype != dtype:
             raise ValueError(f"{name}: {dtype} expected, not {t.dtype}")
-        if t.dim() != 3 or t.shape[1:] != (heads, self.head_dim) or t.shape[0] < least or exact not in (None, t.shape[0]):
+        shape = t.shape
+        if len(shape) != 3 or shape[1] != heads or shape[2] != self.head_dim or shape[0] < least \
+                or exact not in (None, shape[0]):
             raise ValueError(f"{name}: [{'>= %d' % least if exact is None else exact}, {heads}, {self.head_dim}] "
                              f"expected, got {tuple(t.shape)}")
         if t.numel() == 0:
@@ -125,10 +128,11 @@ class FragmentAttention:
         return t
 
     def _small(self, t, name: str, shape, dtype):
-        on_device(t, name, self.device)
-        if t.dtype != dtype or tuple(t.shape) != tuple(shape):
+        if not t.is_cuda or t.device != self.device:
+            on_device(t, name, self.device)
+        if t.dtype != dtype or t.shape != shape:
             raise ValueError(f"{name}: {dtype} {tuple(shape)} expected, got {t.dtype} {tuple(t.shape)}")
-        return t.contiguous()
+        return t if t.is_contiguous() else t.contiguous()
 
     def _io(self, q, k, v, pos, slope, residue, table, query_pos, query_residue, scale):
         """(arguments of the C call without its outputs, the tensors that have to stay alive until it is queued)"""

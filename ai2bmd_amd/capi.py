@@ -73,7 +73,6 @@ class VsnAttnGrads(C.Structure):
 VECNORM = {"none": 0, "rms": 1, "max_min": 2}
 RBF = {"expnorm": 0, "gauss": 1}
 ACTIVATION = {"silu": 0, "swish": 0, "ssp": 1, "tanh": 2, "sigmoid": 3}  # utils.py:93-116 act_class_mapping
-DTYPE = {"float32": 0, "bfloat16": 1, "float16": 2}  # VSN_F32, VSN_BF16, VSN_F16 (include/vsn.h)
 P2P_HANDLE_BYTES = 128  # VSN_P2P_HANDLE_BYTES (include/vsn.h)
 _lib = None
 

@@ -242,6 +242,18 @@ __device__ __forceinline__ void store4(T* p, float a, float b, float c, float d)
     *(uint2*)p = *(uint2*)v;
 }
 
+// a column of an accumulator as a row of an output
+template <typename O, int DP>
+__device__ __forceinline__ void store_column(O* o, const f32x16 (&c)[DP / 32], float f, int dim, int hi) {
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int e = d * 32 + 8 * g + 4 * hi;
+      if (e < dim) store4<O>(o + e, c[d][4 * g] * f, c[d][4 * g + 1] * f, c[d][4 * g + 2] * f, c[d][4 * g + 3] * f);
+    }
+}
+
 // |a - b| from the difference's components, and its reciprocal; 0 and a huge finite number where the points coincide
 // (the difference itself is 0 there, so the direction is 0).  One reciprocal root instead of a root and a division.
 __device__ __forceinline__ float pair_dist(float dx, float dy, float dz, float& inv) {

@@ -7,12 +7,12 @@
 
 struct vsn_attn {
   struct Side {
-    vsn::AttnWork *small_work = nullptr, *lone_work = nullptr, *coop_work = nullptr;
+    vsn::AttnWork *small_work = nullptr, *pair_work = nullptr, *lone_work = nullptr, *coop_work = nullptr;
     vsn::AttnJoin* join = nullptr;
     vsn::AttnBlock* block = nullptr;
-    int small = 0, lone = 0, coop = 0, joins = 0, few = 0, blocks = 0, slots = 0, long_rows = 0;
+    int small = 0, pair = 0, lone = 0, coop = 0, joins = 0, few = 0, blocks = 0, slots = 0, long_rows = 0;
     vsn::AttnPlanView view() const {
-      return {small_work, lone_work, coop_work, small, lone, coop, long_rows, block, blocks, join, joins, few};
+      return {small_work, pair_work, lone_work, coop_work, small, pair, lone, coop, long_rows, block, blocks, join, joins, few};
     }
   };
   int device = 0, heads = 0, kv_heads = 0, dim = 0, reach = 0, n_rel = 0, n_buckets = 0;
@@ -39,15 +39,15 @@ constexpr int kPieceTiles = 2;
 constexpr int kSmallSums = 4096;  // floats of table sums per wave
 
 struct Lists {
-  std::vector<AttnWork> small, lone, coop;
+  std::vector<AttnWork> small, pair, lone, coop;
   std::vector<AttnJoin> join;
   std::vector<AttnBlock> block;
-  int slots = 0;
+  int slots = 0, few = 0;
   bool long_rows = false;
 };
 
 Lists make_lists(int64_t n, const int64_t* col_start, const int64_t* col_end, const int64_t* row_start,
-                 const int64_t* row_end, int heads, bool small) {
+                 const int64_t* row_end, int heads, bool small, bool pair) {
   Lists out;
   int64_t groups = 0;
   for (int64_t f = 0; f < n; ++f) {
@@ -65,6 +65,11 @@ Lists make_lists(int64_t n, const int64_t* col_start, const int64_t* col_end, co
     if (small && cols && rows && cols <= kTile && rows <= kTile) {
       w.col0 = (int)col_start[f], w.cols = (int)cols;
       out.small.push_back(w);
+      continue;
+    }
+    if (pair && cols && rows && cols <= 2 * kTile && rows <= 2 * kTile) {
+      w.col0 = (int)col_start[f], w.cols = (int)cols;
+      out.pair.push_back(w);
       continue;
     }
     const int64_t step = share && cols > 2 * kTile ? kCoopCols : kTile;
@@ -100,7 +105,10 @@ Lists make_lists(int64_t n, const int64_t* col_start, const int64_t* col_end, co
     for (int k = 0; k * kTile < w.cols; ++k)
       out.join.push_back({w.col0 + k * kTile, std::min(kTile, w.cols - k * kTile), piece.slot0 + k, piece.slots, w.step});
   }
-  std::stable_partition(out.join.begin(), out.join.end(), [](const AttnJoin& j) { return j.slots <= kFewSlots; });
+  // One launch joins all where there are few blocks; else those of a few pieces go first, by a launch of their own.
+  const bool one = out.join.size() <= 64;
+  const auto few = std::stable_partition(out.join.begin(), out.join.end(), [](const AttnJoin& j) { return j.slots <= kFewSlots; });
+  out.few = one && few != out.join.end() ? 0 : (int)(few - out.join.begin());
   return out;
 }
 
@@ -112,14 +120,15 @@ bool upload(const std::vector<E>& v, E** dev) {
 }
 
 bool upload_side(const Lists& l, vsn_attn::Side& s) {
-  s.small = (int)l.small.size(), s.lone = (int)l.lone.size(), s.coop = (int)l.coop.size(), s.joins = (int)l.join.size(), s.slots = l.slots;
-  s.few = (int)std::count_if(l.join.begin(), l.join.end(), [](const AttnJoin& j) { return j.slots <= kFewSlots; });
+  s.small = (int)l.small.size(), s.pair = (int)l.pair.size(), s.lone = (int)l.lone.size(), s.coop = (int)l.coop.size(), s.joins = (int)l.join.size(), s.slots = l.slots;
+  s.few = l.few;
   s.blocks = (int)l.block.size(), s.long_rows = l.long_rows;
-  return upload(l.small, &s.small_work) && upload(l.lone, &s.lone_work) && upload(l.coop, &s.coop_work) && upload(l.join, &s.join) && upload(l.block, &s.block);
+  return upload(l.small, &s.small_work) && upload(l.pair, &s.pair_work) && upload(l.lone, &s.lone_work) && upload(l.coop, &s.coop_work) && upload(l.join, &s.join) && upload(l.block, &s.block);
 }
 
 void free_side(vsn_attn::Side& s) {
   hipFree(s.small_work);
+  hipFree(s.pair_work);
   hipFree(s.lone_work);
   hipFree(s.coop_work);
   hipFree(s.join);
@@ -158,10 +167,11 @@ struct BackwardSpace {
 
 BackwardSpace backward_space(const vsn_attn& a, int64_t rows_q, int64_t rows_k) {
   BackwardSpace s;
-  s.workers.lone = workers(a.by_query.lone, a.heads, a.n_rel, 4096);
+  s.workers.lone = workers(a.by_query.lone, a.heads, a.n_rel, a.n_rel ? 2048 : 4096);
   s.workers.coop = workers(a.by_query.coop, a.heads, a.n_rel, 2048);
   s.workers.small = workers(a.by_query.small, 1, a.n_rel * a.heads, 4096);
-  s.parts = s.workers.lone + s.workers.coop + s.workers.small;
+  s.workers.pair = workers(a.by_query.pair, a.heads, a.n_rel, 4096);
+  s.parts = s.workers.lone + s.workers.coop + s.workers.small + s.workers.pair;
   Workspace w;
   s.delta = w.take(rows_q * a.heads * 8);
   s.pos_q = w.take(rows_q * a.heads * 12);
@@ -265,11 +275,16 @@ extern "C" int vsn_attn_create(vsn_attn_handle* out, int device_id, int64_t n, c
       a->reach = reach, a->n_rel = 2 * reach + 1, a->n_buckets = n_buckets;
       lut.assign(host_buckets, host_buckets + a->n_rel);
     }
-    // one-tile fragments go by a kernel of their own where a wave's per-head sums fit its share of LDS
-    const bool small = heads <= 64 && (int64_t)heads * a->n_rel <= kSmallSums;
-    ok = upload_side(make_lists(n, qs, qe, host_start, host_end, heads, small), a->fwd) &&
-         upload_side(make_lists(n, qs, qe, host_start, host_end, heads, small), a->by_query) &&
-         upload_side(make_lists(n, host_start, host_end, qs, qe, kv_heads, small), a->by_key) &&
+    // One-tile fragments go by a kernel of their own where a wave's per-head sums fit its share of LDS - and where there
+    // are enough of them, or nothing else: a launch for a few next to others costs more than the tiles it saves (8 read-out
+    // rows, two of them over one tile: 48 -> 38 us).
+    int64_t tiles = 0;
+    for (int64_t f = 0; f < n; ++f) tiles += host_end[f] - host_start[f] <= kTile && qe[f] - qs[f] <= kTile;
+    const bool small = heads <= 64 && (int64_t)heads * a->n_rel <= kSmallSums && (tiles >= 32 || tiles == n);
+    const bool pair = heads == kv_heads && head_dim <= 64;  // (wider or shared heads would not fit its registers)
+    ok = upload_side(make_lists(n, qs, qe, host_start, host_end, heads, small, false), a->fwd) &&
+         upload_side(make_lists(n, qs, qe, host_start, host_end, heads, small, pair), a->by_query) &&
+         upload_side(make_lists(n, host_start, host_end, qs, qe, kv_heads, small, pair), a->by_key) &&
          upload(lut, &a->lut);
   } catch (...) {  // out of host memory
     ok = false;

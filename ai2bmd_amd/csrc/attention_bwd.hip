@@ -34,18 +34,6 @@ struct ColumnScale {
   }
 };
 
-// a column of an accumulator as a row of an output
-template <typename O, int DP>
-__device__ __forceinline__ void store_column(O* o, const f32x16 (&c)[DP / 32], float f, int dim, int hi) {
-#pragma unroll
-  for (int d = 0; d < DP / 32; ++d)
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int e = d * 32 + 8 * g + 4 * hi;
-      if (e < dim) store4<O>(o + e, c[d][4 * g] * f, c[d][4 * g + 1] * f, c[d][4 * g + 2] * f, c[d][4 * g + 3] * f);
-    }
-}
-
 // DELTA: the pass for D of fragments of several tiles; else the dq pass
 template <typename T, int DP, bool COOP, bool DELTA>
 __global__ __launch_bounds__(256, (backward_waves<T, DP>())) void k_attn_bwd_q(AttnParams p, size_t lds_per_wave) {
@@ -524,14 +512,14 @@ __global__ __launch_bounds__(256) void k_attn_bwd_pieces(AttnParams p, int heads
 // Joins the partial sums in a fixed order: positions over heads (a workgroup per work item of the segments), then one
 // workgroup per head for its slope and one per (head, bucket) for the table, both summed in float64.
 struct AttnPosSegment {
-  const AttnWork* work;    // small fragments: their rows (of_rows) or columns, or
+  const AttnWork* work;    // fragments of one or two tiles: their rows (of_rows) or columns, or
   const AttnBlock* block;  // blocks of columns
   int count, of_rows;
   int parts_q, parts_k;  // partial sums of each side that make up the result
   float* out;
 };
 struct AttnPosJoin {
-  AttnPosSegment seg[4];
+  AttnPosSegment seg[6];
   int n;
 };
 
@@ -679,9 +667,11 @@ static int join_launch(const AttnPlanView& by_query, const AttnPlanView& by_key,
   if (p.dpos) {
     const bool self = !p.dq_pos;
     add(nullptr, by_key.block, by_key.blocks, 0, self ? p.heads : 0, p.kv_heads, p.dpos);
+    add(by_query.pair_work, nullptr, by_query.pair, 1, self ? p.heads : 0, p.kv_heads, p.dpos);
     if (groups > 1) add(by_query.small_work, nullptr, by_query.small, 1, self ? groups : 0, groups, p.dpos);
     if (!self) {
       add(nullptr, by_query.block, by_query.blocks, 0, p.heads, 0, p.dq_pos);
+      add(by_query.pair_work, nullptr, by_query.pair, 0, p.heads, 0, p.dq_pos);
       if (groups > 1) add(by_query.small_work, nullptr, by_query.small, 0, groups, 0, p.dq_pos);
     }
   }
@@ -705,6 +695,12 @@ int attn_backward(int dtype, const AttnPlanView& by_query, const AttnPlanView& b
     case VSN_F32: rc = bwd_dim<float>(by_query, by_key, p, n.lone, n.coop, st); break;
     case VSN_BF16: rc = bwd_dim<__bf16>(by_query, by_key, p, n.lone, n.coop, st); break;
     default: rc = bwd_dim<_Float16>(by_query, by_key, p, n.lone, n.coop, st); break;
+  }
+  if (!rc && by_query.pair) {
+    AttnParams pair = p;
+    pair.work = by_query.pair_work, pair.count = by_query.pair;
+    pair.workers = n.pair, pair.part0 = n.lone + n.coop + n.small;
+    rc = attn_pair_backward(dtype, pair, st);
   }
   const int groups = small_groups(by_query.small, p.kv_heads);
   if (!rc && by_query.small) {

@@ -8,14 +8,14 @@ constexpr int kMaxSlots = 1024;          // partial results of one query block
 constexpr int kFewSlots = 32;
 constexpr size_t kLdsPerCu = 160 * 1024;
 
-// the work lists of one pass: `small` items are fragments of one tile, `lone` items a wave each with tiles of its own,
+// the work lists of one pass: `small` items are fragments of one tile, `pair` items of two (backward), `lone` items a wave each with tiles of its own,
 // `coop` items a workgroup of four
 struct AttnBlock {
   int col0, cols;
 };
 struct AttnPlanView {
-  const AttnWork *small_work, *lone_work, *coop_work;
-  int small, lone, coop;
+  const AttnWork *small_work, *pair_work, *lone_work, *coop_work;
+  int small, pair, lone, coop;
   int long_rows;  // whether an item has more than one tile of rows
   const AttnBlock* block;  // runs of columns of the lone and coop items
   int blocks;
@@ -42,10 +42,12 @@ inline int small_groups(int items, int kv_heads) { return items >= 512 ? 1 : kv_
 
 // workers of the backward passes that add up slope and table gradients, per list
 struct AttnWorkers {
-  int lone, coop, small;
+  int lone, coop, small, pair;
 };
 
 int attn_small(int dtype, const AttnParams& p, int groups, bool backward, hipStream_t st);
+// fragments of up to 64 queries and keys, heads of up to 64 columns, key heads that are not shared
+int attn_pair_backward(int dtype, const AttnParams& p, hipStream_t st);
 int attn_forward(int dtype, const AttnPlanView& plan, const AttnParams& p, hipStream_t st);
 // dq pass (with delta, dslope, dtable and the queries' share of dpos), dk / dv pass, small fragments, then the joins
 int attn_backward(int dtype, const AttnPlanView& by_query, const AttnPlanView& by_key, const AttnParams& p,

@@ -473,6 +473,306 @@ __global__ __launch_bounds__(256, (small_waves<T, DP>())) void k_attn_small_bwd(
   }
 }
 
+// ---- fragments of two tiles: up to 64 queries and 64 keys ----
+// A wave takes a fragment and one key head.  All keys of a query are in registers (two tiles side by side), so here too
+// every score is computed once: 4 tiles instead of the 12 that the passes of attention_bwd.hip visit.  492 of 4096 fragments
+// (33 ... 44 rows), 8 heads: f32 139 us (the three passes 195), bf16 133 us (166).  Bound by latency: 16-bit rows spill at
+// two waves per SIMD and still beat one wave (152 us); float32 rows do not.
+template <typename T, int DP>
+struct PairLds {
+  static constexpr size_t A = TileShape<T, DP>::BYTES, B = TileShape<T, 32>::BYTES;
+  static constexpr size_t PULL = sizeof(float) * kTile * kPullLd;
+  static constexpr size_t S = B > PULL ? B : PULL;
+  T *k, *q, *dout, *score;  // k: two tiles; score: P, dS, and the pulls of one tile
+  float* pull;
+  float4 *kpos, *qpos;      // [64]
+  int *kres, *qres;
+  float *tab, *hist;
+  __device__ __forceinline__ PairLds(char* p, int n_rel) {
+    k = (T*)p;
+    q = (T*)(p + 2 * A);
+    dout = (T*)(p + 3 * A);
+    score = (T*)(p + 4 * A);
+    pull = (float*)(p + 4 * A);
+    kpos = (float4*)(p + ((4 * A + S + 15) & ~(size_t)15));
+    qpos = kpos + 2 * kTile;
+    kres = (int*)(qpos + 2 * kTile);
+    qres = kres + 2 * kTile;
+    tab = (float*)(qres + 2 * kTile);
+    hist = tab + n_rel;
+  }
+  static size_t bytes(int n_rel) {
+    return (((4 * A + S + 15) & ~(size_t)15) + 4 * kTile * (sizeof(float4) + sizeof(int)) + 2 * sizeof(float) * n_rel + 15) & ~(size_t)15;
+  }
+};
+
+template <typename T, int DP>
+__global__ __launch_bounds__(256, (sizeof(T) == 4 ? 1 : 2)) void k_attn_pair_bwd(AttnParams p, size_t per_wave) {
+  extern __shared__ __attribute__((aligned(16))) char lds_raw[];
+  constexpr bool HALF = sizeof(T) == 2 && !__is_same(T, __bf16);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane_of_wave = threadIdx.x & 63;
+  const uint32_t id = blockIdx.x * (blockDim.x >> 6) + wave;
+  if (id >= (uint32_t)p.workers * p.heads) return;
+  const int head = uniform(id % p.heads), worker = uniform(id / p.heads);  // (key heads are not shared: heads == kv_heads)
+  const int n_rel = p.table ? p.n_rel : 0;
+  const PairLds<T, DP> lds(lds_raw + wave * per_wave, n_rel);
+  if (p.table) expand_table(lds.tab, p.table + (int64_t)head * p.n_buckets, p.lut, n_rel, lane_of_wave, 64);
+  for (int i = lane_of_wave; i < n_rel; i += 64) lds.hist[i] = 0.f;
+  const float scale = p.scale * kLog2e, slope = p.slope ? p.slope[head] : 0.f, slope2 = slope * kLog2e;
+  constexpr float PUP = HALF ? 0x1p14f : 1.f;
+  float dslope = 0.f;
+
+  for (int item = worker; item < p.count; item += p.workers) {
+    const AttnWork w = load_work(p.work, item);
+    const int nq = w.cols, nk = w.row1 - w.row0;
+    const int lane = here(lane_of_wave), col = lane & 31, hi = lane >> 5;
+    tile_sync<false>();
+    {
+      const int64_t kr = (int64_t)w.row0 + (lane < nk ? lane : 0), qr = (int64_t)w.col0 + (lane < nq ? lane : 0);
+      if (p.slope) {
+        lds.kpos[lane] = make_float4(p.k_pos[3 * kr], p.k_pos[3 * kr + 1], p.k_pos[3 * kr + 2], 0.f);
+        lds.qpos[lane] = make_float4(p.q_pos[3 * qr], p.q_pos[3 * qr + 1], p.q_pos[3 * qr + 2], 0.f);
+      }
+      if (p.table) lds.kres[lane] = p.k_res[kr], lds.qres[lane] = p.q_res[qr];
+    }
+    typename vec8<T>::type vf[2][DP / 16];
+    const T* kb = (const T*)p.k + w.row0 * p.k_row + head * p.k_head;
+    const T* vb = (const T*)p.v + w.row0 * p.v_row + head * p.v_head;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int key = j * kTile + col;
+      typename vec8<T>::type kf[DP / 16];
+      load_rows<T, DP>(kf, kb, (key < nk ? key : 0) * (uint32_t)p.k_row, p.dim, hi);
+      load_rows<T, DP>(vf[j], vb, (key < nk ? key : 0) * (uint32_t)p.v_row, p.dim, hi);
+      keep_rows<T, DP>(kf, p.dim, hi, key < nk);
+      keep_rows<T, DP>(vf[j], p.dim, hi, key < nk);
+      put_rows<T, DP>(lds.k + j * kTile * TileShape<T, DP>::LD, kf, col, hi);
+    }
+    f32x16 dk[2][DP / 32], dv[2][DP / 32];
+    float gk[2][3];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      gk[j][0] = gk[j][1] = gk[j][2] = 0.f;
+#pragma unroll
+      for (int d = 0; d < DP / 32; ++d) dk[j][d] = acc_zero(), dv[j][d] = acc_zero();
+    }
+    const int lane_of_item = lane;
+
+    for (int i0 = 0; i0 < nq; i0 += kTile) {
+      const int lane = here(lane_of_item), col = lane & 31, hi = lane >> 5;
+      const bool live = i0 + col < nq;
+      const int n_i = nq - i0 < kTile ? nq - i0 : kTile;
+      const int64_t q_row = (int64_t)w.col0 + i0 + (live ? col : 0);
+      const uint32_t in = live ? i0 + col : 0;
+      typename vec8<T>::type qf[DP / 16], df[DP / 16];
+      load_rows<T, DP>(qf, (const T*)p.q + w.col0 * p.q_row + head * p.q_head, in * (uint32_t)p.q_row, p.dim, hi);
+      load_rows<T, DP>(df, (const T*)p.dout + w.col0 * p.do_row + head * p.do_head, in * (uint32_t)p.do_row, p.dim, hi);
+      keep_rows<T, DP>(qf, p.dim, hi, live);
+      keep_rows<T, DP>(df, p.dim, hi, live);
+      tile_sync<false>();
+      put_rows<T, DP>(lds.q, qf, col, hi);
+      put_rows<T, DP>(lds.dout, df, col, hi);
+      tile_sync<false>();
+
+      float s[2][16], t[2][16];
+      const float4 q = lds.qpos[i0 + col];
+      const int res = p.table ? lds.qres[i0 + col] : 0;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const T* kt = lds.k + j * kTile * TileShape<T, DP>::LD;
+        f32x16 acc = acc_zero(), dp = acc_zero();
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c)
+          if (c * 16 < p.dim) {
+            acc = Mma<T>::run(load_n<T, DP>(kt, c, col, hi), qf[c], acc);
+            dp = Mma<T>::run(vf[j][c], df[c], dp);
+          }
+        int limit = live ? nk - j * kTile : 0;
+        compute_here(limit);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int row = j * kTile + acc_row(r, hi);
+          float x = acc[r] * scale;
+          if (p.slope) {
+            const float4 k = lds.kpos[row];
+            float inv;
+            x -= slope2 * pair_dist(q.x - k.x, q.y - k.y, q.z - k.z, inv);
+          }
+          if (p.table) x += lds.tab[rel_index(lds.kres[row], res, p.reach)];
+          s[j][r] = acc_row(r, hi) < limit ? x : -INFINITY;
+          t[j][r] = dp[r];
+        }
+      }
+      float top = s[0][0];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, fmaxf(s[0][r], s[1][r]));
+      top = fmaxf(top, other_half(top));
+      const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[j][r] = __builtin_amdgcn_exp2f(s[j][r] - ref);
+      float l = tile_sum(s[0]) + tile_sum(s[1]), delta;
+      {
+        float u[16];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) u[r] = s[0][r] * t[0][r] + s[1][r] * t[1][r];
+        delta = tile_sum(u);
+      }
+      l += other_half(l);
+      delta += other_half(delta);
+      const float inv_l = l == 0.f ? 0.f : 1.f / l;
+      delta *= inv_l;
+      float gx = 0.f, gy = 0.f, gz = 0.f, largest = 0.f;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          s[j][r] *= inv_l;                        // P
+          t[j][r] = s[j][r] * (t[j][r] - delta);  // dS
+          if (HALF) largest = fmaxf(largest, fabsf(t[j][r]));
+        }
+      float up = 1.f, down = 1.f;
+      if constexpr (HALF) {
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) largest = fmaxf(largest, __shfl_xor(largest, o, 64));
+        if (largest >= 0x1p-80f && largest < INFINITY) {
+          up = ldexpf(1.f, 14 - ilogbf(largest));
+          down = ldexpf(1.f, ilogbf(largest) - 14);
+        }
+      }
+      f32x16 dq[DP / 32];
+#pragma unroll
+      for (int d = 0; d < DP / 32; ++d) dq[d] = acc_zero();
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int n_j = nk - j * kTile;  // (the second tile may be empty: all its terms are 0)
+        const T* kt = lds.k + j * kTile * TileShape<T, DP>::LD;
+        if (n_j <= 0) continue;
+        if (p.part_hist) {
+          float run = 0.f;
+          int at = rel_index(lds.kres[j * kTile + acc_row(0, hi)], res, p.reach);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            run += t[j][r];
+            const int then = r < 15 ? rel_index(lds.kres[j * kTile + acc_row(r < 15 ? r + 1 : 15, hi)], res, p.reach) : -1;
+            if (then != at) {
+              __hip_atomic_fetch_add(lds.hist + at, run, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+              run = 0.f;
+            }
+            at = then;
+          }
+        }
+        if (p.slope) {
+          tile_sync<false>();
+          float sum = 0.f;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const float4 k = lds.kpos[j * kTile + acc_row(r, hi)];
+            const float dx = q.x - k.x, dy = q.y - k.y, dz = q.z - k.z;
+            float inv;
+            sum -= t[j][r] * pair_dist(dx, dy, dz, inv);
+            const float f = live ? slope * t[j][r] * inv : 0.f;
+            gx -= f * dx, gy -= f * dy, gz -= f * dz;
+            if (p.dpos) lds.pull[col * kPullLd + acc_row(r, hi)] = f;
+          }
+          dslope += sum;
+          tile_sync<false>();
+          if (p.dpos) {
+            const float4 k = lds.kpos[j * kTile + col];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const int row = acc_row(r, hi);
+              if (row < n_i) {
+                const float4 o = lds.qpos[i0 + row];
+                const float f = lds.pull[row * kPullLd + col];
+                gk[j][0] += f * (o.x - k.x), gk[j][1] += f * (o.y - k.y), gk[j][2] += f * (o.z - k.z);
+              }
+            }
+          }
+        }
+        float u[16];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[j][r] *= PUP, u[r] = t[j][r] * up;
+        tile_sync<false>();
+        put_scores<T>(lds.score, s[j], col, hi);
+        tile_sync<false>();
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+          if (d * 32 < p.dim) {
+            dv[j][d] = Mma<T>::run(load_t<T, DP>(lds.dout, 0, d * 32, lane, hi), load_t<T, 32>(lds.score, 0, 0, lane, hi), dv[j][d]);
+            if (n_i > 16)
+              dv[j][d] = Mma<T>::run(load_t<T, DP>(lds.dout, 1, d * 32, lane, hi), load_t<T, 32>(lds.score, 1, 0, lane, hi), dv[j][d]);
+          }
+        tile_sync<false>();
+        put_scores<T>(lds.score, u, col, hi);
+        tile_sync<false>();
+        const typename vec8<T>::type u0 = pack8<T>(u), u1 = pack8<T>(u + 8);
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) {
+          if (d * 32 >= p.dim) continue;
+          f32x16 x = acc_zero();
+          x = Mma<T>::run(load_t<T, DP>(lds.q, 0, d * 32, lane, hi), load_t<T, 32>(lds.score, 0, 0, lane, hi), x);
+          if (n_i > 16) x = Mma<T>::run(load_t<T, DP>(lds.q, 1, d * 32, lane, hi), load_t<T, 32>(lds.score, 1, 0, lane, hi), x);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) dk[j][d][r] += x[r] * down;
+          dq[d] = Mma<T>::run(load_t<T, DP>(kt, 0, d * 32, lane, hi), u0, dq[d]);
+          if (n_j > 16) dq[d] = Mma<T>::run(load_t<T, DP>(kt, 1, d * 32, lane, hi), u1, dq[d]);
+        }
+      }
+      if (live) store_column<T, DP>((T*)p.dq + (q_row * p.heads + head) * p.dim, dq, p.scale * down, p.dim, hi);
+      if (p.dpos) {
+        gx += other_half(gx), gy += other_half(gy), gz += other_half(gz);
+        float* g = p.part_pos_q + (head * p.rows_q + q_row) * 3;
+        if (live && hi == 0) g[0] = gx, g[1] = gy, g[2] = gz;
+      }
+    }
+
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const bool key = j * kTile + col < nk;
+      const int64_t k_row = (int64_t)w.row0 + (key ? j * kTile + col : 0);
+      if (key) {
+        store_column<T, DP>((T*)p.dk + (k_row * p.heads + head) * p.dim, dk[j], p.scale, p.dim, hi);
+        store_column<T, DP>((T*)p.dv + (k_row * p.heads + head) * p.dim, dv[j], 1.f / PUP, p.dim, hi);
+      }
+      if (p.dpos) {
+        const float x = gk[j][0] + other_half(gk[j][0]), y = gk[j][1] + other_half(gk[j][1]), z = gk[j][2] + other_half(gk[j][2]);
+        float* g = p.part_pos_k + (head * p.rows_k + k_row) * 3;
+        if (key && hi == 0) g[0] = x, g[1] = y, g[2] = z;
+      }
+    }
+  }
+
+  tile_sync<false>();
+  const int64_t part = p.part0 + worker;
+  if (p.part_slope) {
+    const float sum = wave_sum(dslope);
+    if (lane_of_wave < kCoopWaves) p.part_slope[(head * (int64_t)p.parts + part) * kCoopWaves + lane_of_wave] = lane_of_wave ? 0.f : sum;
+  }
+  if (p.part_hist)
+    for (int i = lane_of_wave; i < n_rel; i += 64) p.part_hist[((int64_t)head * n_rel + i) * p.parts + part] = lds.hist[i];
+}
+
+template <typename T, int DP>
+static int pair_launch(const AttnParams& p, hipStream_t st) {
+  const size_t bytes = PairLds<T, DP>::bytes(p.table ? p.n_rel : 0);
+  const int64_t total = (int64_t)p.workers * p.heads;
+  const int waves = lone_waves(total, bytes);
+  if (!allow_lds((const void*)k_attn_pair_bwd<T, DP>, waves * bytes)) return -5;
+  hipLaunchKernelGGL((k_attn_pair_bwd<T, DP>), dim3((unsigned)((total + waves - 1) / waves)), dim3(64 * waves),
+                     waves * bytes, st, p, bytes);
+  return 0;
+}
+
+int attn_pair_backward(int dtype, const AttnParams& p, hipStream_t st) {
+  switch (dtype) {
+    case VSN_F32: return p.dim <= 32 ? pair_launch<float, 32>(p, st) : pair_launch<float, 64>(p, st);
+    case VSN_BF16: return p.dim <= 32 ? pair_launch<__bf16, 32>(p, st) : pair_launch<__bf16, 64>(p, st);
+    default: return p.dim <= 32 ? pair_launch<_Float16, 32>(p, st) : pair_launch<_Float16, 64>(p, st);
+  }
+}
+
 template <typename T, int DP>
 static int small_launch(AttnParams p, int groups, bool backward, hipStream_t st) {
   const int n_rel = p.table ? p.n_rel : 0;

@@ -6,17 +6,16 @@ Like everything here it is differentiated by hand: the two functions are called 
 """
 from __future__ import annotations
 
-import ctypes as C
-
 import torch
 
 from . import capi
 
 MAX_WIDTH = 4096
+DTYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # VSN_F32, VSN_BF16, VSN_F16 (include/vsn.h)
 
 
 def dtype_code(t: torch.Tensor, name: str) -> int:
-    code = capi.DTYPE.get(str(t.dtype).replace("torch.", ""))
+    code = DTYPE.get(t.dtype)
     if code is None:
         raise ValueError(f"{name}: float32, bfloat16 or float16 expected, not {t.dtype}")
     return code
@@ -31,53 +30,59 @@ def on_device(t: torch.Tensor, name: str, device=None) -> None:
 
 def no_graph(*tensors) -> None:
     """The operators build no autograd graph; a result that silently cut one would train nothing."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError("no autograd graph is built: call under torch.no_grad() and use the backward function")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError("no autograd graph is built: call under torch.no_grad() and use the backward function")
 
 
 def ptr(t):
-    return C.c_void_p(t.data_ptr() if t is not None else 0)
+    return t.data_ptr() if t is not None else None
 
 
-def stream_of(t: torch.Tensor):
-    return C.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+def stream_of(t: torch.Tensor) -> int:
+    """The current stream of the tensor's device, without the Stream object that torch.cuda.current_stream makes (3 us)."""
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
 
 
-def _rows(t: torch.Tensor, name: str):
+def _rows(t: torch.Tensor, width: int):
     """(tensor, rows, elements between rows): the tensor as it is where its rows are evenly spaced, else a copy."""
-    width = t.shape[-1]
-    if t.numel() == 0:
-        return t, t.numel() // max(width, 1), width
+    rows = t.numel() // width
+    if t.is_contiguous() or rows == 0:
+        return t, rows, width
     if t.stride(-1) == 1 or width == 1:
         lead = [(n, s) for n, s in zip(t.shape[:-1], t.stride()[:-1]) if n != 1]
         if all(lead[i][1] == lead[i + 1][0] * lead[i + 1][1] for i in range(len(lead) - 1)):
             step = lead[-1][1] if lead else width
             if step >= width:
-                return t, t.numel() // width, step
-    return t.contiguous(), t.numel() // width, width
+                return t, rows, step
+    return t.contiguous(), rows, width
 
 
 def _param(p, x, name: str) -> None:
-    if p is None:
-        return
-    on_device(p, name, x.device)
-    if p.shape != (x.shape[-1],) or not p.is_contiguous():
+    if not p.is_cuda or p.device != x.device:
+        on_device(p, name, x.device)
+    if p.shape != x.shape[-1:] or not p.is_contiguous():
         raise ValueError(f"{name}: contiguous [{x.shape[-1]}] expected, got {tuple(p.shape)}")
-    if p.dtype not in (x.dtype, torch.float32):
+    if p.dtype != x.dtype and p.dtype != torch.float32:
         raise ValueError(f"{name}: {x.dtype} or float32 expected, not {p.dtype}")
 
 
-def _check(x, weight, bias) -> int:
+def _check(x, weight, bias):
+    """(width, type codes of the rows and of the parameters)"""
     on_device(x, "x")
-    dtype_code(x, "x")
-    if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_WIDTH:
+    code = dtype_code(x, "x")
+    width = x.shape[-1] if x.dim() else 0
+    if not 1 <= width <= MAX_WIDTH:
         raise ValueError(f"x: a last axis of 1 ... {MAX_WIDTH} expected, got {tuple(x.shape)}")
-    _param(weight, x, "weight")
-    _param(bias, x, "bias")
+    if weight is not None:
+        _param(weight, x, "weight")
+    if bias is not None:
+        _param(bias, x, "bias")
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise ValueError("weight and bias differ in type")
     of = weight if weight is not None else bias
-    return dtype_code(of if of is not None else x, "weight")
+    return width, code, code if of is None else DTYPE[of.dtype]
 
 
 def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, out=None):
@@ -86,7 +91,7 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, out=None):
     `x` [..., width], float32 / bfloat16 / float16; evenly spaced rows are read in place, other layouts are copied.
     `weight`, `bias` [width] of x's type or float32 (None: 1 and 0).  `out`: contiguous, of x's shape and type; it may be x.
     `stats` float32 [rows, 2] (mean, 1 / sqrt(var + eps)) goes to layer_norm_backward.  On the current stream of x's device."""
-    code = _check(x, weight, bias)
+    width, code, param_code = _check(x, weight, bias)
     no_graph(x, weight, bias)
     if not eps >= 0:
         raise ValueError("eps: a number >= 0 expected")
@@ -94,11 +99,11 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, out=None):
         on_device(out, "out", x.device)
         if out.shape != x.shape or out.dtype != x.dtype or not out.is_contiguous():
             raise ValueError("out: contiguous, with x's shape and type expected")
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else out
-    src, rows, ld = _rows(x, "x")
+    y = x.new_empty(x.shape) if out is None else out
+    src, rows, ld = _rows(x, width)
     stats = torch.empty(rows, 2, dtype=torch.float32, device=x.device)
-    rc = capi.lib().vsn_layernorm(x.device.index, dtype_code(x, "x"), code, ptr(src), ld, ptr(weight), ptr(bias), rows,
-                                  x.shape[-1], eps, ptr(y), x.shape[-1], ptr(stats), stream_of(x))
+    rc = capi.lib().vsn_layernorm(x.device.index, code, param_code, src.data_ptr(), ld, ptr(weight), ptr(bias), rows,
+                                  width, eps, y.data_ptr(), width, stats.data_ptr(), stream_of(x))
     if rc:
         raise RuntimeError(f"vsn_layernorm failed ({rc})")
     return y, stats
@@ -108,26 +113,25 @@ def layer_norm_backward(dy, x, stats, weight=None, bias=None):
     """Gradients (dx, dweight, dbias) of layer_norm at `x`, with the `stats` it returned, from dy = dL/dy.
 
     dweight / dbias have the parameters' type and are None where the parameter is.  Sums run in a fixed order."""
-    code = _check(x, weight, bias)
+    width, code, param_code = _check(x, weight, bias)
     no_graph(dy, x, weight, bias)
     on_device(dy, "dy", x.device)
     on_device(stats, "stats", x.device)
     if dy.shape != x.shape or dy.dtype != x.dtype:
         raise ValueError("dy: x's shape and type expected")
-    width = x.shape[-1]
-    src, rows, ld = _rows(x, "x")
+    src, rows, ld = _rows(x, width)
     if stats.shape != (rows, 2) or stats.dtype != torch.float32 or not stats.is_contiguous():
         raise ValueError(f"stats: contiguous float32 [{rows}, 2] expected")
-    grad, _, ldg = _rows(dy, "dy")
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    grad, _, ldg = _rows(dy, width)
+    dx = x.new_empty(x.shape)
     dw = torch.empty_like(weight) if weight is not None else None
     db = torch.empty_like(bias) if bias is not None else None
     lib = capi.lib()
     size = lib.vsn_layernorm_workspace(rows, width) if weight is not None or bias is not None else 0
     work = torch.empty(size // 4, dtype=torch.float32, device=x.device) if size else None
-    rc = lib.vsn_layernorm_backward(x.device.index, dtype_code(x, "x"), code, ptr(grad), ldg, ptr(src), ld, ptr(stats),
-                                    ptr(weight), rows, width, ptr(dx), width, ptr(dw), ptr(db), ptr(work), size,
-                                    stream_of(x))
+    rc = lib.vsn_layernorm_backward(x.device.index, code, param_code, grad.data_ptr(), ldg, src.data_ptr(), ld,
+                                    stats.data_ptr(), ptr(weight), rows, width, dx.data_ptr(), width, ptr(dw), ptr(db),
+                                    ptr(work), size, stream_of(x))
     if rc:
         raise RuntimeError(f"vsn_layernorm_backward failed ({rc})")
     return dx, dw, db
