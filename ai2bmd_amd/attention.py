@@ -21,7 +21,7 @@ import torch
 from . import capi
 from .norm import dtype_code, no_graph, on_device, ptr, stream_of
 
-MAX_REACH, MAX_BUCKETS = 1023, 4096
+MAX_REACH, MAX_BUCKETS, MAX_ROW_STEP = 1023, 4096, 1 << 25
 AttentionGrads = namedtuple("AttentionGrads", "dq dk dv dpos dquery_pos dslope dtable")
 
 
@@ -64,7 +64,7 @@ class FragmentAttention:
     `query_start`, `query_end`: rows of the query array, where queries are not the fragment's own rows (one read-out row
     per fragment: arange(B), arange(B) + 1).  `num_kv_heads` divides `num_heads`: shared key and value heads.
     `buckets` int [2 reach + 1]: see relative_buckets; `num_buckets`: columns of the table (default: as many as used).
-    A plan holds no results; several calls may use it at once."""
+    A plan holds no results; several calls may use it at once.  Make it outside of a graph capture."""
 
     def __init__(self, start, end, num_heads: int, head_dim: int, num_kv_heads: int = None, query_start=None,
                  query_end=None, buckets=None, num_buckets: int = None, device="cuda:0") -> None:
@@ -122,7 +122,7 @@ class FragmentAttention:
             return t
         step = 16 // t.element_size()
         row, head, last = t.stride()
-        if last != 1 or row % step or head % step or row < 0 or (heads > 1 and head < self.head_dim) \
+        if last != 1 or row % step or head % step or row > MAX_ROW_STEP or (heads > 1 and head < self.head_dim) \
                 or t.data_ptr() % 16:
             return t.clone(memory_format=torch.contiguous_format)
         return t
@@ -188,7 +188,7 @@ class FragmentAttention:
         (layouts the kernels cannot address are copied first).  pos float32 [rows_k, 3] with slope [heads]; residue
         int32 [rows_k] with table float32 [heads, buckets]; query_pos / query_residue where the queries have rows of
         their own.  `scale` defaults to head_dim ** -0.5.  A row without keys, or whose scores are all -inf, gives 0.
-        Rows behind the last fragment give 0; in a given `out` they stay as they were.  Runs on the current stream."""
+        Rows behind the last fragment give 0; in a given `out` (apart from the inputs) they stay as they were.  Runs on the current stream."""
         io, held = self._io(q, k, v, pos, slope, residue, table, query_pos, query_residue, scale)
         rows = held[0].shape[0]
         shape = (rows, self.num_heads, self.head_dim)

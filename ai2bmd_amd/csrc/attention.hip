@@ -150,6 +150,15 @@ int workers(int items, int heads, int n_rel, int most) {
   return (int)std::min<int64_t>(items, cap);
 }
 
+constexpr int64_t kMaxRowStep = (int64_t)1 << 25;
+
+// launches count their waves in 32 bits
+bool countable(const Lists& l, int heads) {
+  const int64_t most = ((int64_t)1 << 31) / heads;
+  return (int64_t)l.small.size() < most && (int64_t)l.pair.size() < most && (int64_t)l.lone.size() < most &&
+         (int64_t)l.coop.size() < most && (int64_t)l.join.size() < ((int64_t)1 << 26);
+}
+
 struct Workspace {
   int64_t size = 0;
   int64_t take(int64_t bytes) {
@@ -199,8 +208,9 @@ int64_t forward_space(const vsn_attn& a, int64_t* ml) {
 
 bool lines_up(const void* p, int64_t row, int64_t head, int heads, int dim, int size) {
   const int64_t step = 16 / size;
-  return p && (uintptr_t)p % 16 == 0 && row % step == 0 && head % step == 0 && row >= 0 && head >= 0 &&
-         (heads == 1 || head >= dim);
+  // (rows further apart than kMaxRowStep elements would overflow a lane's 32-bit offset within a tile)
+  return p && (uintptr_t)p % 16 == 0 && row % step == 0 && head % step == 0 && row >= 0 && row <= kMaxRowStep &&
+         head >= 0 && (heads == 1 || head >= dim);
 }
 
 // rows and heads of an output that do not run into one another
@@ -282,9 +292,14 @@ extern "C" int vsn_attn_create(vsn_attn_handle* out, int device_id, int64_t n, c
     for (int64_t f = 0; f < n; ++f) tiles += host_end[f] - host_start[f] <= kTile && qe[f] - qs[f] <= kTile;
     const bool small = heads <= 64 && (int64_t)heads * a->n_rel <= kSmallSums && (tiles >= 32 || tiles == n);
     const bool pair = heads == kv_heads && head_dim <= 64;  // (wider or shared heads would not fit its registers)
-    ok = upload_side(make_lists(n, qs, qe, host_start, host_end, heads, small, false), a->fwd) &&
-         upload_side(make_lists(n, qs, qe, host_start, host_end, heads, small, pair), a->by_query) &&
-         upload_side(make_lists(n, host_start, host_end, qs, qe, kv_heads, small, pair), a->by_key) &&
+    const Lists fwd = make_lists(n, qs, qe, host_start, host_end, heads, small, false);
+    const Lists by_query = make_lists(n, qs, qe, host_start, host_end, heads, small, pair);
+    const Lists by_key = make_lists(n, host_start, host_end, qs, qe, kv_heads, small, pair);
+    if (!countable(fwd, heads) || !countable(by_query, heads) || !countable(by_key, kv_heads)) {
+      delete a;
+      return -22;
+    }
+    ok = upload_side(fwd, a->fwd) && upload_side(by_query, a->by_query) && upload_side(by_key, a->by_key) &&
          upload(lut, &a->lut);
   } catch (...) {  // out of host memory
     ok = false;

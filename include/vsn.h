@@ -323,13 +323,14 @@ int vsn_layernorm_backward(int device_id, int dtype, int param_dtype, const void
  *     per fragment.  Ranges contiguous and ascending from 0, as in vsn_forces; empty ones are allowed.  head_dim: a
  *     multiple of 8, 8 ... 128; kv_heads divides heads.  n_buckets > 0: host_buckets[2 reach + 1] gives the bucket of
  *     each difference clipped to -reach ... reach (reach <= 1023).  A plan holds no results and may be used from any
- *     stream, by several calls at once.
+ *     stream, by several calls at once; make it outside of a stream capture.
  *   vsn_attn_io   `q` [rows_q][heads][head_dim], `k`, `v` [rows_k][kv_heads][head_dim], `out` as q: last axis dense, the
- *     strides (elements) of rows and heads multiples of 16 bytes, addresses too.  rows_* may exceed the plan's: rows
+ *     strides (elements) of rows (at most 2^25) and heads multiples of 16 bytes, addresses too.  rows_* may exceed the plan's: rows
  *     behind the last fragment are neither read nor written.  q_pos / k_pos f32 [rows][3] and slope f32 [heads]: all
  *     or none.  q_res / k_res i32 [rows] and table f32 [heads][n_buckets]: all or none.  stats f32
  *     [heads][rows_q][2] (maximum in units of log 2, sum of exponentials) is all that a backward call needs of the forward one (NULL in a
- *     forward call: not wanted); `out` is not read by a backward call.
+ *     forward call: not wanted); `out` is not read by a backward call
+ *     and overlaps none of the inputs.
  *   vsn_attn_grads   dout as out; dq, dk, dv dense.  dpos f32 [rows_k][3]: of both ends of a pair where dquery_pos is
  *     NULL (queries = keys), else of the keys' positions, and dquery_pos f32 [rows_q][3] of the queries'.  dpos, dslope
  *     f32 [heads], dtable f32 [heads][n_buckets] are overwritten and may be NULL.  Fixed summation order.

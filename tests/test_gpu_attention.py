@@ -187,6 +187,38 @@ def test_heads(T, heads, kv, dim):
 
 
 @pytest.mark.parametrize("T", TYPES, ids=str)
+@pytest.mark.parametrize("heads,kv,dim", [(1, 1, 8), (3, 1, 16), (4, 2, 40), (6, 3, 96), (4, 1, 128), (8, 8, 64)])
+def test_heads_of_one_tile_fragments(T, heads, kv, dim):
+    Case([19, 3, 32, 1, 16, 17], T, heads=heads, kv=kv, dim=dim, lut=CLIP).check()
+
+
+@pytest.mark.parametrize("T", TYPES, ids=str)
+@pytest.mark.parametrize("kv", [4, 2])
+def test_many_one_tile_fragments(T, kv):
+    """more than 512: a wave walks all heads and writes the positions' gradient itself"""
+    sizes = [1 + (7 * i) % 32 for i in range(520)]
+    Case(sizes, T, heads=4, kv=kv, dim=16, lut=COARSE).check()
+    Case(sizes, T, heads=4, kv=kv, dim=16, lut=CLIP, queries=[1 + (5 * i) % 32 for i in range(520)]).check()
+
+
+@pytest.mark.parametrize("T", TYPES, ids=str)
+def test_few_one_tile_fragments_with_queries_of_their_own(T):
+    Case([12, 32, 1, 30], T, lut=CLIP, queries=[3, 1, 32, 2]).check()
+
+
+@pytest.mark.parametrize("T", TYPES, ids=str)
+@pytest.mark.parametrize("dim,kv", [(32, 8), (64, 8), (32, 4)])
+def test_all_kinds_of_fragments_together(T, dim, kv):
+    Case([12, 30, 0, 33, 64] * 14 + [150, 300, 97], T, dim=dim, kv=kv, lut=COARSE, extra=3).check()
+
+
+def test_nothing_at_all():
+    for queries in (None, [0, 0]):
+        got = Case([0, 0], torch.float32, lut=CLIP, queries=queries).check()
+        assert not got["dslope"].any() and not got["dtable"].any() and got["out"].numel() == 0
+
+
+@pytest.mark.parametrize("T", TYPES, ids=str)
 def test_queries_of_their_own(T):
     """one row per fragment; several; none; and fragments without keys, whose rows are 0"""
     Case([300, 1, 0, 45, 64], T, queries=[1, 1, 1, 1, 1], lut=CLIP).check()
@@ -246,23 +278,24 @@ def test_large_scores_keep_their_precision(T):
 
 
 @pytest.mark.parametrize("T", TYPES, ids=str)
-def test_nothing_leaks_between_fragments_or_from_behind(T):
-    case = Case([20, 45, 12, 200], T, lut=CLIP, extra=7)
+@pytest.mark.parametrize("sizes", [[20, 45, 12, 200], [20, 28, 12, 30], [20, 100, 12, 30] + [9] * 40], ids=["tiles", "small", "mixed"])
+def test_nothing_leaks_between_fragments_or_from_behind(T, sizes):
+    case = Case(sizes, T, lut=CLIP, extra=7)
+    last, used = int(case.end[1]), int(case.end[-1])
     plan = case.plan()
     before = case.results(plan)
     for x in (case.q, case.k, case.v, case.dout, case.terms["pos"]):
-        x[20:65] = float("nan")
-        x[277:] = float("inf")
-    case.k[66] = case.k[66]  # (the third fragment stays as it was)
-    case.terms["residue"][277:] = -2 ** 31
+        x[20:last] = float("nan")
+        x[used:] = float("inf")
+    case.terms["residue"][used:] = -2 ** 31
     after = case.results(plan)
-    rows = torch.ones(284, dtype=torch.bool, device="cuda")
-    rows[20:65] = False
-    rows[277:] = False
+    rows = torch.ones(used + 7, dtype=torch.bool, device="cuda")
+    rows[20:last] = False
+    rows[used:] = False
     for name in ("out", "dq", "dk", "dv", "dpos"):
         assert torch.equal(after[name][rows], before[name][rows]), name
-        assert not after[name][277:].any()
-    assert torch.isnan(after["out"][20:65]).all()
+        assert not after[name][used:].any()
+    assert torch.isnan(after["out"][20:last]).all()
 
 
 @pytest.mark.parametrize("T", TYPES, ids=str)
@@ -342,9 +375,10 @@ def test_gradients_against_differences():
 
 
 @pytest.mark.parametrize("T", TYPES, ids=str)
-def test_repeats_streams_and_graph_replays(T):
-    case = Case([150, 12, 130, 65, 64, 260] * 4, T, lut=CLIP)
-    rows = Case([1700, 40, 900], T, queries=[1, 1, 1], kv=2)
+@pytest.mark.parametrize("dim", [32, 128])
+def test_repeats_streams_and_graph_replays(T, dim):
+    case = Case([150, 12, 130, 65, 64, 260] * 4 + [20] * 30, T, lut=CLIP, dim=dim)
+    rows = Case([1700, 40, 900], T, queries=[1, 1, 1], kv=2, dim=dim)
     plan, plan_rows = case.plan(), rows.plan()
     first, first_rows = case.results(plan), rows.results(plan_rows)
     same = lambda a, b: all(torch.equal(a[n], b[n]) for n in b)
