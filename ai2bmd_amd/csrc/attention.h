@@ -254,13 +254,12 @@ __device__ __forceinline__ void store_column(O* o, const f32x16 (&c)[DP / 32], f
     }
 }
 
-// |a - b| from the difference's components, and its reciprocal; 0 and a huge finite number where the points coincide
-// (the difference itself is 0 there, so the direction is 0).  One reciprocal root instead of a root and a division.
-__device__ __forceinline__ float pair_dist(float dx, float dy, float dz, float& inv) {
-  const float d2 = dx * dx + dy * dy + dz * dz;
-  inv = __builtin_amdgcn_rsqf(__builtin_amdgcn_fmed3f(d2, 1e-37f, 3e38f));
-  return d2 * inv;
+// |a - b| from the difference's components (the root instruction, off by at most one step), and its reciprocal: a huge
+// finite number where the points coincide, where the difference itself and with it the direction is 0.
+__device__ __forceinline__ float pair_dist(float dx, float dy, float dz) {
+  return __builtin_amdgcn_sqrtf(dx * dx + dy * dy + dz * dz);
 }
+__device__ __forceinline__ float inverse_dist(float far) { return __builtin_amdgcn_rcpf(fmaxf(far, 1e-18f)); }
 
 // index of the clipped difference of two residue numbers; the difference saturates
 __device__ __forceinline__ int rel_index(int key_res, int query_res, int reach) {

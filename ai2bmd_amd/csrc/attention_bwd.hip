@@ -142,12 +142,13 @@ __global__ __launch_bounds__(256, (backward_waves<T, DP>())) void k_attn_bwd_q(A
       float s[16];
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = acc[r] * scale;
+      float far[16];
       if (p.slope) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const float4 k = lds.pos[acc_row(r, hi)];
-          float inv;
-          s[r] -= slope2 * pair_dist(px - k.x, py - k.y, pz - k.z, inv);
+          far[r] = pair_dist(px - k.x, py - k.y, pz - k.z);
+          s[r] -= slope2 * far[r];
         }
       }
       int end = -1;
@@ -190,10 +191,8 @@ __global__ __launch_bounds__(256, (backward_waves<T, DP>())) void k_attn_bwd_q(A
         for (int r = 0; r < 16; ++r) {
           const float4 k = lds.pos[acc_row(r, hi)];
           const float dx = px - k.x, dy = py - k.y, dz = pz - k.z;
-          float inv;
-          const float far = pair_dist(dx, dy, dz, inv);
-          ts -= s[r] * far;
-          const float pull = s[r] * inv;
+          ts -= s[r] * far[r];
+          const float pull = s[r] * inverse_dist(far[r]);
           tx += pull * dx, ty += pull * dy, tz += pull * dz;
         }
         dslope.add(ts);
@@ -390,12 +389,13 @@ __global__ __launch_bounds__(256, (backward_waves<T, DP>())) void k_attn_bwd_k(A
       float s[16];
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = acc[r] * scale;
+      float far[16];
       if (p.slope) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const float4 q = lds.pos[acc_row(r, hi)];
-          float inv;
-          s[r] -= slope2 * pair_dist(q.x - px, q.y - py, q.z - pz, inv);
+          far[r] = pair_dist(q.x - px, q.y - py, q.z - pz);
+          s[r] -= slope2 * far[r];
         }
       }
       if (p.table) {
@@ -428,9 +428,7 @@ __global__ __launch_bounds__(256, (backward_waves<T, DP>())) void k_attn_bwd_k(A
         for (int r = 0; r < 16; ++r) {
           const float4 q = lds.pos[acc_row(r, hi)];
           const float dx = q.x - px, dy = q.y - py, dz = q.z - pz;
-          float inv;
-          pair_dist(dx, dy, dz, inv);
-          const float pull = slope * s[r] * inv;
+          const float pull = slope * s[r] * inverse_dist(far[r]);
           tx += pull * dx, ty += pull * dy, tz += pull * dz;
         }
         gx.add(tx), gy.add(ty), gz.add(tz);

@@ -85,8 +85,7 @@ __global__ __launch_bounds__(256, (forward_waves<T, DP>())) void k_attn_fwd(Attn
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const float4 k = lds.pos[acc_row(r, hi)];
-        float inv;
-        s[r] -= slope * pair_dist(px - k.x, py - k.y, pz - k.z, inv);
+        s[r] -= slope * pair_dist(px - k.x, py - k.y, pz - k.z);
       }
     }
     if (p.table) {

@@ -116,8 +116,7 @@ __device__ __forceinline__ void small_geometry(const AttnParams& p, const AttnWo
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       const float4 k = lds.kpos[acc_row(r, hi)];
-      float inv;
-      g.far[r] = pair_dist(q.x - k.x, q.y - k.y, q.z - k.z, inv);
+      g.far[r] = pair_dist(q.x - k.x, q.y - k.y, q.z - k.z);
     }
   }
   if (p.table) {
@@ -427,9 +426,7 @@ __global__ __launch_bounds__(256, (small_waves<T, DP>())) void k_attn_small_bwd(
         const int row = acc_row(r, hi);
         const float4 k = lds.kpos[row];
         const float dx = q.x - k.x, dy = q.y - k.y, dz = q.z - k.z;
-        float inv;
-        pair_dist(dx, dy, dz, inv);
-        const float f = live ? weight[r] * inv : 0.f;
+        const float f = live ? weight[r] * inverse_dist(g.far[r]) : 0.f;
         x -= f * dx, y -= f * dy, z -= f * dz;
         lds.pull[col * kPullLd + row] = f;
       }
@@ -595,8 +592,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 ? 1 : 2)) void k_attn_pair_bwd
           float x = acc[r] * scale;
           if (p.slope) {
             const float4 k = lds.kpos[row];
-            float inv;
-            x -= slope2 * pair_dist(q.x - k.x, q.y - k.y, q.z - k.z, inv);
+            x -= slope2 * pair_dist(q.x - k.x, q.y - k.y, q.z - k.z);
           }
           if (p.table) x += lds.tab[rel_index(lds.kres[row], res, p.reach)];
           s[j][r] = acc_row(r, hi) < limit ? x : -INFINITY;
@@ -670,9 +666,9 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 ? 1 : 2)) void k_attn_pair_bwd
           for (int r = 0; r < 16; ++r) {
             const float4 k = lds.kpos[j * kTile + acc_row(r, hi)];
             const float dx = q.x - k.x, dy = q.y - k.y, dz = q.z - k.z;
-            float inv;
-            sum -= t[j][r] * pair_dist(dx, dy, dz, inv);
-            const float f = live ? slope * t[j][r] * inv : 0.f;
+            const float far = pair_dist(dx, dy, dz);
+            sum -= t[j][r] * far;
+            const float f = live ? slope * t[j][r] * inverse_dist(far) : 0.f;
             gx -= f * dx, gy -= f * dy, gz -= f * dz;
             if (p.dpos) lds.pull[col * kPullLd + acc_row(r, hi)] = f;
           }
