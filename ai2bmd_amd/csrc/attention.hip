@@ -1,5 +1,6 @@
 // Fragment attention: the plan (work lists of both passes, made once per fragment layout) and the entry points.
 #include <algorithm>
+#include <utility>
 #include <vector>
 
 #include "attention.h"
@@ -19,6 +20,7 @@ struct vsn_attn {
   int64_t used_q = 0, used_k = 0;
   Side fwd, by_query, by_key;
   int* lut = nullptr;
+  char* lists = nullptr;  // what all of these point into
 };
 
 namespace vsn {
@@ -112,28 +114,37 @@ Lists make_lists(int64_t n, const int64_t* col_start, const int64_t* col_end, co
   return out;
 }
 
-template <typename E>
-bool upload(const std::vector<E>& v, E** dev) {
-  if (v.empty()) return true;
-  return hipMalloc((void**)dev, v.size() * sizeof(E)) == hipSuccess &&
-         hipMemcpy(*dev, v.data(), v.size() * sizeof(E), hipMemcpyHostToDevice) == hipSuccess;
-}
-
-bool upload_side(const Lists& l, vsn_attn::Side& s) {
-  s.small = (int)l.small.size(), s.pair = (int)l.pair.size(), s.lone = (int)l.lone.size(), s.coop = (int)l.coop.size(), s.joins = (int)l.join.size(), s.slots = l.slots;
-  s.few = l.few;
-  s.blocks = (int)l.block.size(), s.long_rows = l.long_rows;
-  return upload(l.small, &s.small_work) && upload(l.pair, &s.pair_work) && upload(l.lone, &s.lone_work) && upload(l.coop, &s.coop_work) && upload(l.join, &s.join) && upload(l.block, &s.block);
-}
-
-void free_side(vsn_attn::Side& s) {
-  hipFree(s.small_work);
-  hipFree(s.pair_work);
-  hipFree(s.lone_work);
-  hipFree(s.coop_work);
-  hipFree(s.join);
-  hipFree(s.block);
-}
+// All lists of a plan in one device allocation: packed on the host, copied once, pointers set afterwards.
+struct Packed {
+  std::vector<char> host;
+  std::vector<std::pair<void**, size_t>> at;
+  template <typename E>
+  void add(const std::vector<E>& v, E** dev) {
+    if (v.empty()) return;
+    at.push_back({(void**)dev, host.size()});
+    const size_t bytes = (v.size() * sizeof(E) + 63) & ~(size_t)63;
+    host.resize(host.size() + bytes);
+    memcpy(host.data() + at.back().second, v.data(), v.size() * sizeof(E));
+  }
+  void add(const Lists& l, vsn_attn::Side& s) {
+    s.small = (int)l.small.size(), s.pair = (int)l.pair.size(), s.lone = (int)l.lone.size(), s.coop = (int)l.coop.size();
+    s.joins = (int)l.join.size(), s.few = l.few, s.slots = l.slots;
+    s.blocks = (int)l.block.size(), s.long_rows = l.long_rows;
+    add(l.small, &s.small_work);
+    add(l.pair, &s.pair_work);
+    add(l.lone, &s.lone_work);
+    add(l.coop, &s.coop_work);
+    add(l.join, &s.join);
+    add(l.block, &s.block);
+  }
+  bool upload(char** dev) {
+    if (host.empty()) return true;
+    if (hipMalloc((void**)dev, host.size()) != hipSuccess) return false;
+    if (hipMemcpy(*dev, host.data(), host.size(), hipMemcpyHostToDevice) != hipSuccess) return false;
+    for (auto& a : at) *a.first = *dev + a.second;
+    return true;
+  }
+};
 
 bool ranges_ok(int64_t n, const int64_t* start, const int64_t* end) {
   if (!start || !end) return false;
@@ -299,8 +310,12 @@ extern "C" int vsn_attn_create(vsn_attn_handle* out, int device_id, int64_t n, c
       delete a;
       return -22;
     }
-    ok = upload_side(fwd, a->fwd) && upload_side(by_query, a->by_query) && upload_side(by_key, a->by_key) &&
-         upload(lut, &a->lut);
+    Packed all;
+    all.add(fwd, a->fwd);
+    all.add(by_query, a->by_query);
+    all.add(by_key, a->by_key);
+    all.add(lut, &a->lut);
+    ok = all.upload(&a->lists);
   } catch (...) {  // out of host memory
     ok = false;
   }
@@ -315,10 +330,7 @@ extern "C" int vsn_attn_create(vsn_attn_handle* out, int device_id, int64_t n, c
 extern "C" void vsn_attn_destroy(vsn_attn_handle a) {
   if (!a) return;
   vsn::DeviceScope scope(a->device);
-  vsn::free_side(a->fwd);
-  vsn::free_side(a->by_query);
-  vsn::free_side(a->by_key);
-  hipFree(a->lut);
+  hipFree(a->lists);
   delete a;
 }
 

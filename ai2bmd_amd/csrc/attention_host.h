@@ -8,8 +8,8 @@ constexpr int kMaxSlots = 1024;          // partial results of one query block
 constexpr int kFewSlots = 32;
 constexpr size_t kLdsPerCu = 160 * 1024;
 
-// the work lists of one pass: `small` items are fragments of one tile, `pair` items of two (backward), `lone` items a wave each with tiles of its own,
-// `coop` items a workgroup of four
+// the work lists of one pass: `small` items are fragments of one tile, `pair` items of two (backward), `lone` items a wave
+// each with tiles of its own, `coop` items a workgroup of four
 struct AttnBlock {
   int col0, cols;
 };
