@@ -435,12 +435,10 @@ __global__ __launch_bounds__(256, (small_waves<T, DP>())) void k_attn_small_bwd(
       float u = 0.f, v = 0.f, t = 0.f;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const int row = acc_row(r, hi);
-        if (row < nq) {
-          const float4 o = lds.qpos[row];
-          const float f = lds.pull[row * kPullLd + col];
-          u += f * (o.x - k.x), v += f * (o.y - k.y), t += f * (o.z - k.z);
-        }
+        const int row = acc_row(r, hi);  // (rows beyond the last query pull by 0)
+        const float4 o = lds.qpos[row];
+        const float f = lds.pull[row * kPullLd + col];
+        u += f * (o.x - k.x), v += f * (o.y - k.y), t += f * (o.z - k.z);
       }
       x += other_half(x), y += other_half(y), z += other_half(z);
       u += other_half(u), v += other_half(v), t += other_half(t);
@@ -473,8 +471,8 @@ __global__ __launch_bounds__(256, (small_waves<T, DP>())) void k_attn_small_bwd(
 // ---- fragments of two tiles: up to 64 queries and 64 keys ----
 // A wave takes a fragment and one key head.  All keys of a query are in registers (two tiles side by side), so here too
 // every score is computed once: 4 tiles instead of the 12 that the passes of attention_bwd.hip visit.  492 of 4096 fragments
-// (33 ... 44 rows), 8 heads: f32 139 us (the three passes 195), bf16 133 us (166).  Bound by latency: 16-bit rows spill at
-// two waves per SIMD and still beat one wave (152 us); float32 rows do not.
+// (33 ... 44 rows), 8 heads: f32 127 us (the three passes 195), bf16 109 us (166).  Bound by latency: 16-bit rows spill at
+// two waves per SIMD and still beat one wave (127 us); float32 rows do not.
 template <typename T, int DP>
 struct PairLds {
   static constexpr size_t A = TileShape<T, DP>::BYTES, B = TileShape<T, 32>::BYTES;
@@ -587,17 +585,23 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 ? 1 : 2)) void k_attn_pair_bwd
         int limit = live ? nk - j * kTile : 0;
         compute_here(limit);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int row = j * kTile + acc_row(r, hi);
-          float x = acc[r] * scale;
-          if (p.slope) {
-            const float4 k = lds.kpos[row];
-            x -= slope2 * pair_dist(q.x - k.x, q.y - k.y, q.z - k.z);
+        for (int r = 0; r < 16; ++r) s[j][r] = acc[r] * scale, t[j][r] = dp[r];
+        if (p.slope) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const float4 k = lds.kpos[j * kTile + acc_row(r, hi)];
+            s[j][r] -= slope2 * pair_dist(q.x - k.x, q.y - k.y, q.z - k.z);
           }
-          if (p.table) x += lds.tab[rel_index(lds.kres[row], res, p.reach)];
-          s[j][r] = acc_row(r, hi) < limit ? x : -INFINITY;
-          t[j][r] = dp[r];
         }
+        if (p.table) {
+          float b[16];
+#pragma unroll
+          for (int r = 0; r < 16; ++r) b[r] = lds.tab[rel_index(lds.kres[j * kTile + acc_row(r, hi)], res, p.reach)];
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[j][r] += b[r];
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[j][r] = acc_row(r, hi) < limit ? s[j][r] : -INFINITY;
       }
       float top = s[0][0];
 #pragma unroll
@@ -678,8 +682,10 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 ? 1 : 2)) void k_attn_pair_bwd
             const float4 k = lds.kpos[j * kTile + col];
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
+              // rows beyond the last query pull by 0; 16-bit rows skip them, which keeps the loads from being hoisted into
+              // registers that spill (bf16 138 us without the branch, 109 us with it)
               const int row = acc_row(r, hi);
-              if (row < n_i) {
+              if (sizeof(T) == 4 || row < n_i) {
                 const float4 o = lds.qpos[i0 + row];
                 const float f = lds.pull[row * kPullLd + col];
                 gk[j][0] += f * (o.x - k.x), gk[j][1] += f * (o.y - k.y), gk[j][2] += f * (o.z - k.z);
