@@ -26,11 +26,11 @@ struct vsn_attn {
 namespace vsn {
 namespace {
 
-// A workgroup of four waves reads each tile of rows once for 128 columns, a lone wave once for 32.  Sharing pays where
-// there are workgroups enough for every compute unit; with fewer, 32 columns per wave spread over four times as many
-// compute units.
+// A workgroup of four waves reads each tile of rows once for 128 columns, a lone wave once for 32.  Sharing pays from a few
+// workgroups on, which pieces multiply, but narrow heads sooner: forward + backward of 3000 atoms bf16, dim 32, 192 workgroups
+// 353 us shared, 402 us alone; 1786 atoms f32, dim 64, 112 workgroups 615 us shared (its registers spill), 558 us alone.
 constexpr int kCoopCols = kTile * kCoopWaves;
-constexpr int64_t kCoopMin = 256;
+inline int64_t coop_min(int dim) { return dim <= 32 ? 64 : 256; }
 // A run of rows is split into pieces where the items alone are too few waves for the 1024 SIMDs to be filled evenly
 // (12 rounds of one wave each); a piece keeps at least 2 tiles.  One protein of 175
 // atoms, forward: whole runs 19.6 us, pieces of 2 tiles 14.3 us with the join, of 1 tile 12.4 us; four proteins of up to 746
@@ -49,14 +49,14 @@ struct Lists {
 };
 
 Lists make_lists(int64_t n, const int64_t* col_start, const int64_t* col_end, const int64_t* row_start,
-                 const int64_t* row_end, int heads, bool small, bool pair) {
+                 const int64_t* row_end, int heads, int dim, bool small, bool pair) {
   Lists out;
   int64_t groups = 0;
   for (int64_t f = 0; f < n; ++f) {
     const int64_t cols = col_end[f] - col_start[f];
     if (cols > 2 * kTile) groups += (cols + kCoopCols - 1) / kCoopCols * heads;
   }
-  const bool share = groups >= kCoopMin;
+  const bool share = groups >= coop_min(dim);
   std::vector<AttnWork> all;
   int64_t waves = 0, tiles = 0;  // of 32 columns; tiles of 32 x 32
   for (int64_t f = 0; f < n; ++f) {
@@ -303,9 +303,9 @@ extern "C" int vsn_attn_create(vsn_attn_handle* out, int device_id, int64_t n, c
     for (int64_t f = 0; f < n; ++f) tiles += host_end[f] - host_start[f] <= kTile && qe[f] - qs[f] <= kTile;
     const bool small = heads <= 64 && (int64_t)heads * a->n_rel <= kSmallSums && (tiles >= 32 || tiles == n);
     const bool pair = heads == kv_heads && head_dim <= 64;  // (wider or shared heads would not fit its registers)
-    const Lists fwd = make_lists(n, qs, qe, host_start, host_end, heads, small, false);
-    const Lists by_query = make_lists(n, qs, qe, host_start, host_end, heads, small, pair);
-    const Lists by_key = make_lists(n, host_start, host_end, qs, qe, kv_heads, small, pair);
+    const Lists fwd = make_lists(n, qs, qe, host_start, host_end, heads, head_dim, small, false);
+    const Lists by_query = make_lists(n, qs, qe, host_start, host_end, heads, head_dim, small, pair);
+    const Lists by_key = make_lists(n, host_start, host_end, qs, qe, kv_heads, head_dim, small, pair);
     if (!countable(fwd, heads) || !countable(by_query, heads) || !countable(by_key, kv_heads)) {
       delete a;
       return -22;

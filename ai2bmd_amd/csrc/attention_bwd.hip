@@ -159,8 +159,11 @@ __global__ __launch_bounds__(256, (backward_waves<T, DP>())) void k_attn_bwd_q(A
 #pragma unroll
           for (int r = 0; r < 16; ++r) s[r] += t;
         } else {
+          float b[16];
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s[r] += lds.tab[rel_index(lds.res[acc_row(r, hi)], res, p.reach)];
+          for (int r = 0; r < 16; ++r) b[r] = lds.tab[rel_index(lds.res[acc_row(r, hi)], res, p.reach)];
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[r] += b[r];
         }
       }
       if (n < kTile || !whole) {
@@ -405,8 +408,11 @@ __global__ __launch_bounds__(256, (backward_waves<T, DP>())) void k_attn_bwd_k(A
 #pragma unroll
           for (int r = 0; r < 16; ++r) s[r] += t;
         } else {
+          float b[16];
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s[r] += lds.tab[rel_index(res, lds.res[acc_row(r, hi)], p.reach)];
+          for (int r = 0; r < 16; ++r) b[r] = lds.tab[rel_index(res, lds.res[acc_row(r, hi)], p.reach)];
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[r] += b[r];
         }
       }
       if (n < kTile || !whole) {
