@@ -8,12 +8,16 @@
 // fragment.  Rows are loaded straight into matrix operands (a lane has its row's 16-byte pieces) and written to LDS from
 // there for the products that need them transposed; nothing is read twice.
 // Softmax statistics are recomputed: they cost less than reading them.
+// 3600 fragments of 12 ... 32 atoms, 8 heads of 32: float32 forward 77 us (3.7 TB/s), backward 162 us (3.1 TB/s); bf16 forward
+// 51 us, backward with the table 127 us.  Bound by one wave's chain of products, exchanges and LDS passes per head, of which
+// registers allow two waves per SIMD; the next head's rows are on their way meanwhile.
 #include "attention.h"
 #include "attention_host.h"
 
 namespace vsn {
 
-// Waves per SIMD that the backward kernel is compiled for (registers are what limits them).
+// Waves per SIMD that the backward kernel is compiled for (registers are what limits them: bf16 rows of 32 at one wave
+// 186 us, at two 121 us, at three, spilling, 417 us).
 template <typename T, int DP>
 constexpr int small_waves() {
   return DP > 64 || (DP > 32 && sizeof(T) == 4) ? 1 : 2;

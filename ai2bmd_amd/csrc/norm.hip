@@ -12,6 +12,8 @@
 // second launch, both in a fixed order (no atomics: equal inputs give equal bits).  All sums are float32.
 // Vector loads need only element alignment (gfx950 takes global addresses of any alignment); the row's last, partial
 // vector goes element by element.
+// One MI355X (a large copy runs at 4.73 TB/s): forward 1 310 720 x 256 f32 0.59 ms (4.5 TB/s); 80 000 x 256 bf16 forward 28 us
+// (2.9), backward 25 us (4.9) and 4 us for the second launch; 30 011 x 509 f16, rows at any address, 37 and 40 us (1.7, 2.3).
 #include "typed.h"
 
 namespace vsn {
