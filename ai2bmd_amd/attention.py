@@ -64,7 +64,8 @@ class FragmentAttention:
     `query_start`, `query_end`: rows of the query array, where queries are not the fragment's own rows (one read-out row
     per fragment: arange(B), arange(B) + 1).  `num_kv_heads` divides `num_heads`: shared key and value heads.
     `buckets` int [2 reach + 1]: see relative_buckets; `num_buckets`: columns of the table (default: as many as used).
-    A plan holds no results; several calls may use it at once.  Make it outside of a graph capture."""
+    A plan holds no results; several calls may use it at once.  Make it and let go of it outside of a graph capture (both
+    allocate or free device memory), and keep it as long as a graph that captured its calls is replayed."""
 
     def __init__(self, start, end, num_heads: int, head_dim: int, num_kv_heads: int = None, query_start=None,
                  query_end=None, buckets=None, num_buckets: int = None, device="cuda:0") -> None:
