@@ -57,10 +57,11 @@ __device__ __forceinline__ float row_sum(float v) {
   return v;
 }
 
+// (y may be x: a wave holds its rows before it stores them, and no other wave reads them)
 template <typename T, int VEC, int LPR, int NV>
-__global__ __launch_bounds__(256) void k_layernorm(const T* __restrict__ x, int64_t ldx, const void* __restrict__ w,
+__global__ __launch_bounds__(256) void k_layernorm(const T* x, int64_t ldx, const void* __restrict__ w,
                                                    const void* __restrict__ b, int param_f32, int64_t rows, int width,
-                                                   float inv_width, float eps, T* __restrict__ y, int64_t ldy,
+                                                   float inv_width, float eps, T* y, int64_t ldy,
                                                    float2* __restrict__ stats) {
   constexpr int RPB = 256 / LPR;  // rows of a workgroup per turn
   const int lane = threadIdx.x % LPR;
