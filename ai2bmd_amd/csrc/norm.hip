@@ -12,8 +12,9 @@
 // second launch, both in a fixed order (no atomics: equal inputs give equal bits).  All sums are float32.
 // Vector loads need only element alignment (gfx950 takes global addresses of any alignment); the row's last, partial
 // vector goes element by element.
-// One MI355X (a large copy runs at 4.73 TB/s): forward 1 310 720 x 256 f32 0.59 ms (4.5 TB/s); 80 000 x 256 bf16 forward 28 us
-// (2.9), backward 25 us (4.9) and 4 us for the second launch; 30 011 x 509 f16, rows at any address, 37 and 40 us (1.7, 2.3).
+// One MI355X (a large copy runs at 4.73 TB/s): forward 1 310 720 x 256 f32 0.45 ms (6.0 TB/s); 80 000 x 256 bf16 forward 16 us
+// (5.1, from the cache), backward 24 us (5.1) and 4 us for the second launch; 30 011 x 509 f16, rows at any address, 25 and
+// 45 us (2.5, 2.0) alone.
 #include "typed.h"
 
 namespace vsn {
@@ -43,12 +44,18 @@ __device__ __forceinline__ void store_row(T* __restrict__ p, int at, int width, 
       if (at + i < width) p[at + i] = (T)v[i];
   }
 }
-// weight / bias columns of one lane: the rows' type or float32; absent = `fill`
+// weight / bias columns of one lane: the rows' type or float32; absent = `fill`.  Whole vectors, as the rows are: a load per
+// element made up almost half of the forward pass (80 000 x 256 bf16 27 us, so 15 us; 5000 x 1024 bf16 13.4 us, so 6.0 us).
 template <typename T, int VEC>
 __device__ __forceinline__ void load_param(const void* p, int is_f32, int at, int width, float fill, float (&v)[VEC]) {
+  if (!p) {
 #pragma unroll
-  for (int i = 0; i < VEC; ++i)
-    v[i] = at + i >= width ? 0.f : !p ? fill : is_f32 ? ((const float*)p)[at + i] : (float)((const T*)p)[at + i];
+    for (int i = 0; i < VEC; ++i) v[i] = at + i < width ? fill : 0.f;
+  } else if (is_f32) {
+    load_row<float, VEC>((const float*)p, at, width, v);
+  } else {
+    load_row<T, VEC>((const T*)p, at, width, v);
+  }
 }
 template <int LPR>
 __device__ __forceinline__ float row_sum(float v) {
@@ -208,6 +215,18 @@ static int norm_groups(int64_t rows, int rows_per_group, int cap) {
   return (int)(need < cap ? need : cap);
 }
 
+// Workgroups of the forward pass.  As many as the chip holds at once, each walking its share of the rows, so that weight and
+// bias are read once for many rows: 80 000 x 256 bf16 15.2 us, with one turn each 17.4; 30 011 x 509 f16 17.5 and 22.8;
+// 1 310 720 x 80 bf16 83 and 155; 700 000 x 509 f16 399 and 588; 150 000 x 4096 f32 985 and 1111.  Float32 rows of ordinary
+// width that do not fit the 256 MB cache go the other way, as fresh waves keep more loads in flight than a wave's next turn:
+// 1 310 720 x 256 f32 552 us walking, 449 with one turn each; 200 000 x 256 78 and 72; 2 600 000 x 64 274 and 222;
+// 600 000 x 1024 984 and 853.
+template <typename T>
+static int norm_forward_cap(int64_t rows, int width) {
+  const bool beyond_cache = rows * width * 2 * (int64_t)sizeof(T) > (int64_t)256 << 20;
+  return sizeof(T) == 4 && width >= 64 && width <= 1024 && beyond_cache ? 1 << 20 : 2048;
+}
+
 struct NormArgs {
   const void *x, *dy, *w, *b;
   void *y, *dx, *dw, *db;
@@ -224,7 +243,8 @@ static void norm_launch(const NormArgs& a, hipStream_t st) {
   const int rpb = 256 / LPR;
   if (!a.backward) {
     if (!a.rows) return;
-    hipLaunchKernelGGL((k_layernorm<T, VEC, LPR, NV>), dim3(norm_groups(a.rows, rpb, 4096)), dim3(256), 0, st,
+    const int groups = norm_groups(a.rows, rpb, norm_forward_cap<T>(a.rows, a.width));
+    hipLaunchKernelGGL((k_layernorm<T, VEC, LPR, NV>), dim3(groups), dim3(256), 0, st,
                        (const T*)a.x, a.ldx, a.w, a.b, a.param_f32, a.rows, a.width, inv, a.eps, (T*)a.y, a.ldy,
                        (float2*)a.stats);
     return;
