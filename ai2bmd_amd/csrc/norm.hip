@@ -11,17 +11,31 @@
 // so do the column sums of the backward pass, which are joined over the workgroup in LDS and over the workgroups by a
 // second launch, both in a fixed order (no atomics: equal inputs give equal bits).  All sums are float32.
 // Vector loads need only element alignment (gfx950 takes global addresses of any alignment); the row's last, partial
-// vector goes element by element.
-// One MI355X (a large copy runs at 4.73 TB/s): forward 1 310 720 x 256 f32 0.45 ms (6.0 TB/s); 80 000 x 256 bf16 forward 16 us
-// (5.1, from the cache), backward 24 us (5.1) and 4 us for the second launch; 30 011 x 509 f16, rows at any address, 25 and
-// 45 us (2.5, 2.0) alone.
+// vector is stored element by element.
+// One MI355X (a large copy runs at 4.73 TB/s): forward 1 310 720 x 256 f32 0.46 ms (5.9 TB/s); 80 000 x 256 bf16 forward 16 us
+// (5.1, from the cache), backward 24 us (5.1) and 4 us for the second launch; 30 011 x 509 f16, rows at any address, 20 and
+// 27 us (3.0, 3.3) alone.
 #include "typed.h"
 
 namespace vsn {
 
-template <typename T, int VEC>
+// Columns at ... at + VEC of a row, zeros behind its end.  ODD (16-bit rows of at least one vector that end within one): a lane
+// at the row's end loads the row's last whole vector and shifts its columns down, as nobody waits then for one that goes
+// element by element (30 011 x 509 f16: forward 17.4 -> 13.7 us, backward 35.9 -> 24.0; float32 rows, at most three such
+// elements, gain nothing, and rows of whole vectors would lose: 80 000 x 256 bf16 15.6 -> 16.6, 1 310 720 x 256 f32 454 -> 634).
+template <typename T, int VEC, bool ODD>
 __device__ __forceinline__ void load_row(const T* __restrict__ p, int at, int width, float (&v)[VEC]) {
-  if (at + VEC <= width) {
+  if constexpr (ODD) {
+    static_assert(sizeof(T) * VEC == 16, "one 16-byte vector");
+    const int from = __builtin_elementwise_min(at, width - VEC), skip = at - from;
+    unsigned __int128 bits;
+    __builtin_memcpy(&bits, p + from, sizeof(bits));
+    if (skip) bits = skip < VEC ? bits >> (skip * (int)sizeof(T) * 8) : 0;
+    T tmp[VEC];
+    __builtin_memcpy(tmp, &bits, sizeof(tmp));
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v[i] = (float)tmp[i];
+  } else if (at + VEC <= width) {
     T tmp[VEC];
     __builtin_memcpy(tmp, p + at, sizeof(tmp));
 #pragma unroll
@@ -46,15 +60,15 @@ __device__ __forceinline__ void store_row(T* __restrict__ p, int at, int width, 
 }
 // weight / bias columns of one lane: the rows' type or float32; absent = `fill`.  Whole vectors, as the rows are: a load per
 // element made up almost half of the forward pass (80 000 x 256 bf16 27 us, so 15 us; 5000 x 1024 bf16 13.4 us, so 6.0 us).
-template <typename T, int VEC>
+template <typename T, int VEC, bool ODD>
 __device__ __forceinline__ void load_param(const void* p, int is_f32, int at, int width, float fill, float (&v)[VEC]) {
   if (!p) {
 #pragma unroll
     for (int i = 0; i < VEC; ++i) v[i] = at + i < width ? fill : 0.f;
   } else if (is_f32) {
-    load_row<float, VEC>((const float*)p, at, width, v);
+    load_row<float, VEC, false>((const float*)p, at, width, v);
   } else {
-    load_row<T, VEC>((const T*)p, at, width, v);
+    load_row<T, VEC, ODD>((const T*)p, at, width, v);
   }
 }
 template <int LPR>
@@ -65,7 +79,7 @@ __device__ __forceinline__ float row_sum(float v) {
 }
 
 // (y may be x: a wave holds its rows before it stores them, and no other wave reads them)
-template <typename T, int VEC, int LPR, int NV>
+template <typename T, int VEC, int LPR, int NV, bool ODD>
 __global__ __launch_bounds__(256) void k_layernorm(const T* x, int64_t ldx, const void* __restrict__ w,
                                                    const void* __restrict__ b, int param_f32, int64_t rows, int width,
                                                    float inv_width, float eps, T* y, int64_t ldy,
@@ -75,15 +89,15 @@ __global__ __launch_bounds__(256) void k_layernorm(const T* x, int64_t ldx, cons
   float wv[NV][VEC], bv[NV][VEC];
 #pragma unroll
   for (int n = 0; n < NV; ++n) {
-    load_param<T, VEC>(w, param_f32, (n * LPR + lane) * VEC, width, 1.f, wv[n]);
-    load_param<T, VEC>(b, param_f32, (n * LPR + lane) * VEC, width, 0.f, bv[n]);
+    load_param<T, VEC, ODD>(w, param_f32, (n * LPR + lane) * VEC, width, 1.f, wv[n]);
+    load_param<T, VEC, ODD>(b, param_f32, (n * LPR + lane) * VEC, width, 0.f, bv[n]);
   }
   for (int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / LPR; row < rows; row += (int64_t)gridDim.x * RPB) {
     float v[NV][VEC];
     float s = 0.f;
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
-      load_row<T, VEC>(x + row * ldx, (n * LPR + lane) * VEC, width, v[n]);
+      load_row<T, VEC, ODD>(x + row * ldx, (n * LPR + lane) * VEC, width, v[n]);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) s += v[n][i];
     }
@@ -108,7 +122,7 @@ __global__ __launch_bounds__(256) void k_layernorm(const T* x, int64_t ldx, cons
 }
 
 // partial: [gridDim.x][2][width] column sums of dy h and dy
-template <typename T, int VEC, int LPR, int NV>
+template <typename T, int VEC, int LPR, int NV, bool ODD>
 __global__ __launch_bounds__(256) void k_layernorm_bwd(const T* __restrict__ dy, int64_t lddy, const T* __restrict__ x,
                                                        int64_t ldx, const float2* __restrict__ stats,
                                                        const void* __restrict__ w, int param_f32, int64_t rows,
@@ -119,7 +133,7 @@ __global__ __launch_bounds__(256) void k_layernorm_bwd(const T* __restrict__ dy,
   float wv[NV][VEC], aw[NV][VEC], ab[NV][VEC];
 #pragma unroll
   for (int n = 0; n < NV; ++n) {
-    load_param<T, VEC>(w, param_f32, (n * LPR + lane) * VEC, width, 1.f, wv[n]);
+    load_param<T, VEC, ODD>(w, param_f32, (n * LPR + lane) * VEC, width, 1.f, wv[n]);
 #pragma unroll
     for (int i = 0; i < VEC; ++i) aw[n][i] = ab[n][i] = 0.f;
   }
@@ -129,8 +143,8 @@ __global__ __launch_bounds__(256) void k_layernorm_bwd(const T* __restrict__ dy,
     float sg = 0.f, sgh = 0.f;
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
-      load_row<T, VEC>(x + row * ldx, (n * LPR + lane) * VEC, width, h[n]);
-      load_row<T, VEC>(dy + row * lddy, (n * LPR + lane) * VEC, width, g[n]);
+      load_row<T, VEC, ODD>(x + row * ldx, (n * LPR + lane) * VEC, width, h[n]);
+      load_row<T, VEC, ODD>(dy + row * lddy, (n * LPR + lane) * VEC, width, g[n]);
     }
 #pragma unroll
     for (int n = 0; n < NV; ++n)
@@ -237,14 +251,14 @@ struct NormArgs {
   bool backward;
 };
 
-template <typename T, int VEC, int LPR, int NV>
+template <typename T, int VEC, int LPR, int NV, bool ODD>
 static void norm_launch(const NormArgs& a, hipStream_t st) {
   const float inv = 1.0f / (float)a.width;
   const int rpb = 256 / LPR;
   if (!a.backward) {
     if (!a.rows) return;
     const int groups = norm_groups(a.rows, rpb, norm_forward_cap<T>(a.rows, a.width));
-    hipLaunchKernelGGL((k_layernorm<T, VEC, LPR, NV>), dim3(groups), dim3(256), 0, st,
+    hipLaunchKernelGGL((k_layernorm<T, VEC, LPR, NV, ODD>), dim3(groups), dim3(256), 0, st,
                        (const T*)a.x, a.ldx, a.w, a.b, a.param_f32, a.rows, a.width, inv, a.eps, (T*)a.y, a.ldy,
                        (float2*)a.stats);
     return;
@@ -252,7 +266,7 @@ static void norm_launch(const NormArgs& a, hipStream_t st) {
   const int groups = norm_groups(a.rows, rpb, kNormGroups);
   float* partial = a.dw || a.db ? a.partial : nullptr;
   if (groups)
-    hipLaunchKernelGGL((k_layernorm_bwd<T, VEC, LPR, NV>), dim3(groups), dim3(256), 0, st, (const T*)a.dy, a.lddy,
+    hipLaunchKernelGGL((k_layernorm_bwd<T, VEC, LPR, NV, ODD>), dim3(groups), dim3(256), 0, st, (const T*)a.dy, a.lddy,
                        (const T*)a.x, a.ldx, (const float2*)a.stats, a.w, a.param_f32, a.rows, a.width, inv, (T*)a.dx,
                        a.lddx, partial);
   if (partial || (!groups && (a.dw || a.db)))
@@ -260,24 +274,32 @@ static void norm_launch(const NormArgs& a, hipStream_t st) {
                        a.width, a.dw, a.db, a.param_f32);
 }
 
-template <typename T, int VEC>
+template <typename T, int VEC, bool ODD>
 static void norm_pick(const NormArgs& a, hipStream_t st) {
   const int n = a.width;
-  if (n <= 8 * VEC) return norm_launch<T, VEC, 8, 1>(a, st);
-  if (n <= 16 * VEC) return norm_launch<T, VEC, 16, 1>(a, st);
-  if (n <= 32 * VEC) return norm_launch<T, VEC, 32, 1>(a, st);
-  if (n <= 64 * VEC) return norm_launch<T, VEC, 64, 1>(a, st);
-  if (n <= 128 * VEC) return norm_launch<T, VEC, 64, 2>(a, st);
-  if (n <= 256 * VEC) return norm_launch<T, VEC, 64, 4>(a, st);
-  if (n <= 512 * VEC) return norm_launch<T, VEC, 64, 8>(a, st);
-  if constexpr (VEC == 4) return norm_launch<T, VEC, 64, 16>(a, st);
+  if (n <= 8 * VEC) return norm_launch<T, VEC, 8, 1, ODD>(a, st);
+  if (n <= 16 * VEC) return norm_launch<T, VEC, 16, 1, ODD>(a, st);
+  if (n <= 32 * VEC) return norm_launch<T, VEC, 32, 1, ODD>(a, st);
+  if (n <= 64 * VEC) return norm_launch<T, VEC, 64, 1, ODD>(a, st);
+  if (n <= 128 * VEC) return norm_launch<T, VEC, 64, 2, ODD>(a, st);
+  if (n <= 256 * VEC) return norm_launch<T, VEC, 64, 4, ODD>(a, st);
+  if (n <= 512 * VEC) return norm_launch<T, VEC, 64, 8, ODD>(a, st);
+  if constexpr (VEC == 4) return norm_launch<T, VEC, 64, 16, ODD>(a, st);
+}
+
+template <typename T>
+static void norm_pick_16bit(const NormArgs& a, hipStream_t st) {
+  if (a.width % 8 && a.width > 8)
+    norm_pick<T, 8, true>(a, st);
+  else
+    norm_pick<T, 8, false>(a, st);
 }
 
 static int norm_dispatch(int dtype, const NormArgs& a, hipStream_t st) {
   switch (dtype) {
-    case VSN_F32: norm_pick<float, 4>(a, st); break;
-    case VSN_BF16: norm_pick<__bf16, 8>(a, st); break;
-    default: norm_pick<_Float16, 8>(a, st); break;
+    case VSN_F32: norm_pick<float, 4, false>(a, st); break;
+    case VSN_BF16: norm_pick_16bit<__bf16>(a, st); break;
+    default: norm_pick_16bit<_Float16>(a, st); break;
   }
   return hipGetLastError() == hipSuccess ? 0 : -5;
 }

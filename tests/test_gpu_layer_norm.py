@@ -189,3 +189,34 @@ def test_refusals():
         layer_norm(x, w.requires_grad_(), b)
     with torch.no_grad():
         layer_norm(x, w, b)
+
+
+@pytest.mark.parametrize("T", TYPES, ids=str)
+@pytest.mark.parametrize("width", [5, 8, 9, 15, 17, 31, 63, 129, 255, 511, 1023, 4095])
+@pytest.mark.parametrize("own_params", [True, False])
+def test_rows_that_end_within_a_vector(T, width, own_params):
+    """a row between poisoned columns: what is loaded next to it must not count, and what is next to it stays"""
+    from ai2bmd_amd.norm import layer_norm, layer_norm_backward
+    x, w, b, dy = make(37, width, T, width, param=T if own_params else torch.float32)
+    inside = [torch.full((37, width + 5), float("nan"), dtype=T, device="cuda") for _ in range(2)]
+    for wide, rows in zip(inside, (x, dy)):
+        wide[:, 2:2 + width] = rows
+    xs, dys = (wide[:, 2:2 + width] for wide in inside)
+    params = torch.full((2, width + 2), float("nan"), dtype=w.dtype, device="cuda")
+    params[0, 1:-1], params[1, 1:-1] = w, b
+    ws, bs = params[0, 1:-1], params[1, 1:-1]
+    out = torch.full((39, width), 7.0, dtype=T, device="cuda")
+    y, stats = layer_norm(xs, ws, bs, out=out[1:38])
+    check(x, w, b, dy, y, layer_norm_backward(dys, xs, stats, ws, bs))
+    assert (out[0] == 7).all() and (out[38] == 7).all()
+    again = x.clone()
+    assert torch.equal(layer_norm(again, w, b, out=again)[0], y)
+
+
+@pytest.mark.parametrize("rows,width", [(140_001, 256), (33_001, 1024), (530_001, 64), (33_001, 1025)])
+def test_float32_rows_beyond_the_cache(rows, width):
+    from ai2bmd_amd.norm import layer_norm, layer_norm_backward
+    x, w, b, dy = make(rows, width, torch.float32, 11)
+    y, stats = layer_norm(x, w, b)
+    check(x, w, b, dy, y, layer_norm_backward(dy, x, stats, w, b))
+    assert torch.equal(layer_norm(x[-7:], w, b)[0], y[-7:])
