@@ -230,8 +230,8 @@ static int norm_groups(int64_t rows, int rows_per_group, int cap) {
 }
 
 // Workgroups of the forward pass.  As many as the chip holds at once, each walking its share of the rows, so that weight and
-// bias are read once for many rows: 80 000 x 256 bf16 15.2 us, with one turn each 17.4; 30 011 x 509 f16 17.5 and 22.8;
-// 1 310 720 x 80 bf16 83 and 155; 700 000 x 509 f16 399 and 588; 150 000 x 4096 f32 985 and 1111.  Float32 rows of ordinary
+// bias are read once for many rows: 80 000 x 256 bf16 15.6 us, with one turn each 18.9; 30 011 x 509 f16 13.8 and 16.7;
+// 1 310 720 x 80 bf16 83 and 155; 700 000 x 509 f16 382 and 396; 150 000 x 4096 f32 973 and 1111.  Float32 rows of ordinary
 // width that do not fit the 256 MB cache go the other way, as fresh waves keep more loads in flight than a wave's next turn:
 // 1 310 720 x 256 f32 552 us walking, 449 with one turn each; 200 000 x 256 78 and 72; 2 600 000 x 64 274 and 222;
 // 600 000 x 1024 984 and 853.
