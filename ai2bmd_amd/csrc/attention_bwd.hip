@@ -44,7 +44,7 @@ __global__ __launch_bounds__(256, (backward_waves<T, DP>())) void k_attn_bwd_q(A
   const int col = lane & 31, hi = lane >> 5;
   const int tid = COOP ? threadIdx.x : lane;
   constexpr int THREADS = COOP ? 64 * kCoopWaves : 64;
-  constexpr bool HALF = sizeof(T) == 2 && !__is_same(T, __bf16);
+  constexpr bool HALF = is_half<T>();
   const uint32_t id = COOP ? blockIdx.x : blockIdx.x * (blockDim.x >> 6) + wave;
   if (id >= (uint32_t)p.workers * p.heads) return;
   const int head = uniform(id % p.heads), worker = uniform(id / p.heads);
@@ -314,7 +314,7 @@ __global__ __launch_bounds__(256, (backward_waves<T, DP>())) void k_attn_bwd_k(A
   const int col = lane & 31, hi = lane >> 5;
   const int tid = COOP ? threadIdx.x : lane;
   constexpr int THREADS = COOP ? 64 * kCoopWaves : 64;
-  constexpr bool HALF = sizeof(T) == 2 && !__is_same(T, __bf16);
+  constexpr bool HALF = is_half<T>();
   const uint32_t id = COOP ? blockIdx.x : blockIdx.x * (blockDim.x >> 6) + wave;
   if (id >= (uint32_t)p.count * p.kv_heads) return;
   const int kv = uniform(id % p.kv_heads), share = uniform(p.heads / p.kv_heads);

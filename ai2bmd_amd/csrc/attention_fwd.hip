@@ -52,8 +52,8 @@ __global__ __launch_bounds__(256, (forward_waves<T, DP>())) void k_attn_fwd(Attn
   f32x16 o[DP / 32];
 #pragma unroll
   for (int d = 0; d < DP / 32; ++d) o[d] = acc_zero();
-  float m = -INFINITY;
-  LongSum l;  // this half's share
+  float m = -INFINITY;  // the reference of the exponentials: that of the largest score so far
+  LongSum l;            // this half's share
 
   TilePair<T, DP, THREADS> tiles;
   constexpr bool AHEAD = TilePair<T, DP, THREADS>::N <= 8;
@@ -109,7 +109,7 @@ __global__ __launch_bounds__(256, (forward_waves<T, DP>())) void k_attn_fwd(Attn
     float top = s[0];
 #pragma unroll
     for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
-    top = fmaxf(m, fmaxf(top, other_half(top)));
+    top = fmaxf(m, exp_ref<T>(fmaxf(top, other_half(top))));
     // a row whose scores are all -inf so far keeps the maximum -inf and adds nothing
     const float ref = top == -INFINITY ? 0.f : top;
     const float fade = __builtin_amdgcn_exp2f(m - ref);
@@ -147,7 +147,7 @@ __global__ __launch_bounds__(256, (forward_waves<T, DP>())) void k_attn_fwd(Attn
     return;
   }
   const float inv = total == 0.f ? 0.f : 1.f / total;
-  if (hi == 0 && p.stats) p.stats[head * p.rows_q + row] = make_float2(m, total);
+  if (hi == 0 && p.stats) p.stats[head * p.rows_q + row] = attn_stats<T>(m, total);
   T* op = (T*)p.out + row * p.out_row + head * p.out_head;
 #pragma unroll
   for (int d = 0; d < DP / 32; ++d)
@@ -159,8 +159,8 @@ __global__ __launch_bounds__(256, (forward_waves<T, DP>())) void k_attn_fwd(Attn
     }
 }
 
-// Joins the pieces' outputs, each weighted by 2^(m_s - max m).  A few pieces: one workgroup per (block of columns, head),
-// a thread per four elements of a column, which finds the weights itself.
+// Joins the pieces' outputs, each weighted by 2^(m_s - max m), m the references of their exponentials.  A few pieces: one
+// workgroup per (block of columns, head), a thread per four elements of a column, which finds the weights itself.
 template <typename T>
 __global__ __launch_bounds__(256) void k_attn_join(AttnParams p) {
   const AttnJoin j = p.join[blockIdx.x];
@@ -185,7 +185,7 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnParams p) {
     const float inv = l == 0.f ? 0.f : 1.f / l;
     const int64_t row = (int64_t)j.col0 + col;
     store4<T>((T*)p.out + row * p.out_row + head * p.out_head + d, a.x * inv, a.y * inv, a.z * inv, a.w * inv);
-    if (d == 0 && p.stats) p.stats[head * p.rows_q + row] = make_float2(m, l);
+    if (d == 0 && p.stats) p.stats[head * p.rows_q + row] = attn_stats<T>(m, l);
   }
 }
 
@@ -236,7 +236,7 @@ __global__ __launch_bounds__(256) void k_attn_join_many(AttnParams p) {
     }
     store4<T>((T*)p.out + row * p.out_row + head * p.out_head + d, a.x * inv, a.y * inv, a.z * inv, a.w * inv);
   }
-  if (tid == 0 && p.stats) p.stats[head * p.rows_q + row] = make_float2(m, l);
+  if (tid == 0 && p.stats) p.stats[head * p.rows_q + row] = attn_stats<T>(m, l);
 }
 
 template <typename T, int DP>

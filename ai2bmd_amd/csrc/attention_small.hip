@@ -155,12 +155,13 @@ __device__ __forceinline__ void small_scores(const AttnParams& p, SmallGeometry&
   for (int r = 0; r < 16; ++r) s[r] = acc_row(r, hi) < limit ? s[r] : -INFINITY;
 }
 
-// s -> exponentials; returns the maximum
+// s -> exponentials relative to exp_ref of their maximum; returns that
+template <typename T>
 __device__ __forceinline__ float small_exp(float* s) {
   float top = s[0];
 #pragma unroll
   for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
-  top = fmaxf(top, other_half(top));
+  top = exp_ref<T>(fmaxf(top, other_half(top)));
   const float ref = top == -INFINITY ? 0.f : top;
 #pragma unroll
   for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(s[r] - ref);
@@ -216,12 +217,12 @@ __global__ __launch_bounds__(256) void k_attn_small_fwd(AttnParams p, size_t per
     if (head + 1 < h0 + each) load(head + 1);  // in flight while this head is computed
     float s[16];
     small_scores<T>(p, g, acc, scale, slopes[head] * kLog2e, tab + head * n_rel, live ? nk : 0, hi, s);
-    const float top = small_exp(s);
+    const float ref = small_exp<T>(s);
     float l = tile_sum(s);
     l += other_half(l);
     const float inv = l == 0.f ? 0.f : 1.f / l;
     const typename vec8<T>::type p0 = pack8<T>(s), p1 = pack8<T>(s + 8);
-    if (live && hi == 0 && p.stats) p.stats[head * p.rows_q + q_row] = make_float2(top, l);
+    if (live && hi == 0 && p.stats) p.stats[head * p.rows_q + q_row] = attn_stats<T>(ref, l);
     T* op = (T*)p.out + w.col0 * p.out_row + head * p.out_head;
     const uint32_t o_at = col * (uint32_t)p.out_row;
 #pragma unroll
@@ -244,7 +245,7 @@ __global__ __launch_bounds__(256) void k_attn_small_fwd(AttnParams p, size_t per
 template <typename T, int DP, bool SHARE>
 __global__ __launch_bounds__(256, (small_waves<T, DP>())) void k_attn_small_bwd(AttnParams p, size_t per_wave, int groups) {
   extern __shared__ __attribute__((aligned(16))) char lds_raw[];
-  constexpr bool HALF = sizeof(T) == 2 && !__is_same(T, __bf16);
+  constexpr bool HALF = is_half<T>();
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane_of_wave = threadIdx.x & 63;
   float* tab = (float*)lds_raw;
   const int n_rel = p.table ? p.n_rel : 0;
@@ -312,7 +313,7 @@ __global__ __launch_bounds__(256, (small_waves<T, DP>())) void k_attn_small_bwd(
       const float slope = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, slopes[head])));
       float s[16], t[16];
       small_scores<T>(p, g, acc, scale, slope * kLog2e, tab + head * n_rel, live ? nk : 0, hi, s);
-      small_exp(s);
+      small_exp<T>(s);
 #pragma unroll
       for (int r = 0; r < 16; ++r) t[r] = s[r] * dp[r];
       float l = tile_sum(s), delta = tile_sum(t);
@@ -508,7 +509,7 @@ struct PairLds {
 template <typename T, int DP>
 __global__ __launch_bounds__(256, (sizeof(T) == 4 ? 1 : 2)) void k_attn_pair_bwd(AttnParams p, size_t per_wave) {
   extern __shared__ __attribute__((aligned(16))) char lds_raw[];
-  constexpr bool HALF = sizeof(T) == 2 && !__is_same(T, __bf16);
+  constexpr bool HALF = is_half<T>();
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane_of_wave = threadIdx.x & 63;
   const uint32_t id = blockIdx.x * (blockDim.x >> 6) + wave;
   if (id >= (uint32_t)p.workers * p.heads) return;
