@@ -243,12 +243,35 @@ __device__ __forceinline__ typename vec8<T>::type load_col(const T* row, int at,
   return f;
 }
 
+// Eight weights (P, dS) as B operands of a product.  16-bit rows take them in two parts, hi + lo: one rounding to the rows'
+// type would put an error as large as the result's own rounding into every term, which the caller of 16-bit rows did not
+// ask for; two leave 2^-18 (bf16) and 2^-24 (f16) of a term.  The second product costs little, as the matrix units wait for
+// the vector ones; what it costs is the split, 6 instructions per pair of weights (bf16).  17 882 atoms bf16, dim 32: forward
+// 1.35 -> 1.62 ms, both directions 9.2 -> 10.2 ms; 6007 atoms f16, dim 64, both 1.48 -> 1.65 ms; fragments gain nothing by
+// less (4096 of them bf16, both 0.332 and 0.338 ms).
 template <typename T>
-__device__ __forceinline__ typename vec8<T>::type pack8(const float* p) {
-  typename vec8<T>::type f;
+struct Weights {
+  typename vec8<T>::type hi, lo;
+};
+template <>
+struct Weights<float> {
+  f32x8 hi;
+};
+template <typename T>
+__device__ __forceinline__ Weights<T> split8(const float* p) {
+  Weights<T> w;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = (T)p[i];
-  return f;
+  for (int i = 0; i < 8; ++i) {
+    w.hi[i] = (T)p[i];
+    if constexpr (sizeof(T) == 2) w.lo[i] = (T)(p[i] - (float)w.hi[i]);
+  }
+  return w;
+}
+template <typename T>
+__device__ __forceinline__ f32x16 mma(typename vec8<T>::type a, const Weights<T>& b, f32x16 c) {
+  c = Mma<T>::run(a, b.hi, c);
+  if constexpr (sizeof(T) == 2) c = Mma<T>::run(a, b.lo, c);
+  return c;
 }
 
 // four consecutive elements of an output row
@@ -316,17 +339,16 @@ __device__ __forceinline__ void expand_table(float* tab, const float* table, con
 
 // c += a * b over one tile of 32 rows
 template <typename T>
-__device__ __forceinline__ void tile_mma(f32x16& c, typename vec8<T>::type a0, typename vec8<T>::type b0,
-                                         typename vec8<T>::type a1, typename vec8<T>::type b1) {
+__device__ __forceinline__ void tile_mma(f32x16& c, typename vec8<T>::type a0, const Weights<T>& b0,
+                                         typename vec8<T>::type a1, const Weights<T>& b1) {
   if constexpr (sizeof(T) == 4) {
-    f32x16 t = acc_zero();
-    t = Mma<T>::run(a0, b0, t);
-    t = Mma<T>::run(a1, b1, t);
+    f32x16 t = mma<T>(a0, b0, acc_zero());
+    t = mma<T>(a1, b1, t);
 #pragma unroll
     for (int r = 0; r < 16; ++r) c[r] += t[r];
   } else {
-    c = Mma<T>::run(a0, b0, c);
-    c = Mma<T>::run(a1, b1, c);
+    c = mma<T>(a0, b0, c);
+    c = mma<T>(a1, b1, c);
   }
 }
 

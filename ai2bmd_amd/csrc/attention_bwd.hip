@@ -9,11 +9,11 @@
 // lanes for dq, D, the slopes, the table and the queries' share of the positions; keys in lanes for dk, dv and the keys'
 // share.  Seven products instead of five, against a pass that would have to add dq (or dk, dv) across workgroups in an
 // order of its own.  The maximum and the sum are kept apart (not as one logarithm), so P keeps its precision however
-// large the scores are.  D is summed from the scores before anything is rounded (do_i.o_i would carry the rounding of P
-// in the forward product into every float32 gradient): a pass of its own ahead of the dq pass, except where one tile
+// large the scores are.  D is summed from the scores before anything is rounded (do_i.o_i would carry the rounding of the
+// output into every float32 gradient): a pass of its own ahead of the dq pass, except where one tile
 // holds all keys of a fragment and everything is still in registers.
 // Long runs of rows are split into pieces of equal length (make_lists); a piece leaves float32 sums that a join adds up.
-// P and dS are rounded to the rows' type where they enter a product.  float16 has few exponents for that: P goes in
+// P and dS enter a product in two parts of 16-bit rows' type (split8).  float16 has few exponents for that: P goes in
 // times 2^14, and dS times a power of two per column that follows the largest one seen so far.
 // All sums are in a fixed order; the table's are kept per wave in LDS.
 // Bound by vector instructions: 17 882 atoms, 8 heads of 32, bf16, distances and table: D 1.5 ms, dq 2.9 ms, dk / dv 3.3 ms;
@@ -241,7 +241,7 @@ __global__ __launch_bounds__(256, (backward_waves<T, DP>())) void k_attn_bwd_q(A
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] *= cs.f;
       }
-      const typename vec8<T>::type s0 = pack8<T>(s), s1 = pack8<T>(s + 8);
+      const Weights<T> s0 = split8<T>(s), s1 = split8<T>(s + 8);
 #pragma unroll
       for (int d = 0; d < DP / 32; ++d) {
         if (d * 32 >= p.dim) continue;
@@ -455,7 +455,7 @@ __global__ __launch_bounds__(256, (backward_waves<T, DP>())) void k_attn_bwd_k(A
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] *= cs.f;
       }
-      const typename vec8<T>::type s0 = pack8<T>(s), s1 = pack8<T>(s + 8), p0 = pack8<T>(pr), p1 = pack8<T>(pr + 8);
+      const Weights<T> s0 = split8<T>(s), s1 = split8<T>(s + 8), p0 = split8<T>(pr), p1 = split8<T>(pr + 8);
 #pragma unroll
       for (int d = 0; d < DP / 32; ++d) {
         if (d * 32 >= p.dim) continue;

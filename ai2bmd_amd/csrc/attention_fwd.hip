@@ -1,8 +1,8 @@
 // Fragment attention, forward: one pass over the keys with a running maximum and sum (attention.h has the tile).
 //
 // S^T = K Q^T puts keys in rows and queries in lanes; the softmax of a query is then 16 registers and one exchange with
-// the other half of the wave, and O^T += V^T P^T takes P from the same registers.  P is rounded to the rows' type for
-// that product (float32 rows: not at all); maximum, sum and output stay in float32.
+// the other half of the wave, and O^T += V^T P^T takes P from the same registers.  16-bit rows take P
+// in two parts (split8); maximum, sum and output stay in float32.
 // Bound by vector instructions: 17 882 atoms, 8 heads of 32, bf16, with distances 1.34 ms (244 TFLOP/s of the two products;
 // some 320 instructions per tile, half of them distances); 6007 atoms, 8 heads of 64, f16, with a table 0.20 ms (368 TFLOP/s).
 #include "attention.h"
@@ -124,7 +124,7 @@ __global__ __launch_bounds__(256, (forward_waves<T, DP>())) void k_attn_fwd(Attn
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[d][r] *= fade;
     }
-    const typename vec8<T>::type p0 = pack8<T>(s), p1 = pack8<T>(s + 8);
+    const Weights<T> p0 = split8<T>(s), p1 = split8<T>(s + 8);
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d) {
       if (d * 32 >= p.dim) continue;

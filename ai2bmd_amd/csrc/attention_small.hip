@@ -3,8 +3,8 @@
 //
 // What does not depend on the head - distances, residue offsets, positions' directions - is computed once per fragment
 // and stays in registers; a head's scores are computed once for all of its gradients.  With queries in lanes, dq takes dS
-// from the registers; dk and dv contract over the lanes, so dS and P pass through LDS (rounded to the rows' type, as any
-// product's operand) and are read back transposed.  The positions' gradient needs only sum_heads slope dS: one pass per
+// from the registers; dk and dv contract over the lanes, so dS and P pass through LDS (in two parts of 16-bit rows' type, as
+// any product's weights) and are read back transposed.  The positions' gradient needs only sum_heads slope dS: one pass per
 // fragment.  Rows are loaded straight into matrix operands (a lane has its row's 16-byte pieces) and written to LDS from
 // there for the products that need them transposed; nothing is read twice.
 // Softmax statistics are recomputed: they cost less than reading them.
@@ -25,9 +25,39 @@ constexpr int small_waves() {
 
 constexpr int kPullLd = 33;  // floats per row of the transposed pulls: column reads fall on different banks
 
+// The lane's 16 weights as its row of [column][row], 16-bit rows' second parts in a tile behind the first; and a product's
+// operand of rows 16 c ... + 15, read back transposed.
+template <typename T>
+struct WeightTile {
+  static constexpr int AT = TileShape<T, 32>::LD * kTile;  // of the second parts
+  static constexpr size_t BYTES = (sizeof(T) == 2 ? 2 : 1) * TileShape<T, 32>::BYTES;
+  static __device__ __forceinline__ void put(T* tile, const Weights<T>& a, const Weights<T>& b, int col, int hi) {
+    T* row = tile + col * TileShape<T, 32>::LD + 4 * hi;
+    put8(row, a.hi);
+    put8(row + 16, b.hi);
+    if constexpr (sizeof(T) == 2) {
+      put8(row + AT, a.lo);
+      put8(row + AT + 16, b.lo);
+    }
+  }
+  static __device__ __forceinline__ Weights<T> get(const T* tile, int c, int lane, int hi) {
+    Weights<T> w;
+    w.hi = load_t<T, 32>(tile, c, 0, lane, hi);
+    if constexpr (sizeof(T) == 2) w.lo = load_t<T, 32>(tile + AT, c, 0, lane, hi);
+    return w;
+  }
+
+ private:
+  static __device__ __forceinline__ void put8(T* row, const typename vec8<T>::type& v) {
+    typedef T half4 __attribute__((ext_vector_type(4)));
+    *(half4*)row = __builtin_shufflevector(v, v, 0, 1, 2, 3);
+    *(half4*)(row + 8) = __builtin_shufflevector(v, v, 4, 5, 6, 7);
+  }
+};
+
 template <typename T, int DP>
 struct SmallLds {
-  static constexpr size_t A = TileShape<T, DP>::BYTES, B = TileShape<T, 32>::BYTES;
+  static constexpr size_t A = TileShape<T, DP>::BYTES, B = WeightTile<T>::BYTES;
   static constexpr size_t PULL = sizeof(float) * kTile * kPullLd;
   T *dout, *q, *k;  // rows to be read transposed (the forward pass has v in `dout`)
   T* score;         // [query][key]: P, then dS
@@ -82,14 +112,6 @@ __device__ __forceinline__ void keep_rows(typename vec8<T>::type (&f)[DP / 16], 
     f[c] = live && c * 16 + hi * 8 < dim ? f[c] : zero;
   }
 }
-// the lane's 16 values as its row of [column][row]
-template <typename T>
-__device__ __forceinline__ void put_scores(T* tile, const float* v, int col, int hi) {
-#pragma unroll
-  for (int g = 0; g < 4; ++g)
-    store4<T>(tile + col * TileShape<T, 32>::LD + 8 * g + 4 * hi, v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
-}
-
 // distances and table indices of the lane's 16 pairs
 struct SmallGeometry {
   float far[16];
@@ -221,7 +243,7 @@ __global__ __launch_bounds__(256) void k_attn_small_fwd(AttnParams p, size_t per
     float l = tile_sum(s);
     l += other_half(l);
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    const typename vec8<T>::type p0 = pack8<T>(s), p1 = pack8<T>(s + 8);
+    const Weights<T> p0 = split8<T>(s), p1 = split8<T>(s + 8);
     if (live && hi == 0 && p.stats) p.stats[head * p.rows_q + q_row] = attn_stats<T>(ref, l);
     T* op = (T*)p.out + w.col0 * p.out_row + head * p.out_head;
     const uint32_t o_at = col * (uint32_t)p.out_row;
@@ -229,8 +251,8 @@ __global__ __launch_bounds__(256) void k_attn_small_fwd(AttnParams p, size_t per
     for (int d = 0; d < DP / 32; ++d) {
       if (d * 32 >= p.dim) continue;
       f32x16 o = acc_zero();
-      o = Mma<T>::run(load_t<T, DP>(lds.dout, 0, d * 32, lane, hi), p0, o);
-      if (nk > 16) o = Mma<T>::run(load_t<T, DP>(lds.dout, 1, d * 32, lane, hi), p1, o);
+      o = mma<T>(load_t<T, DP>(lds.dout, 0, d * 32, lane, hi), p0, o);
+      if (nk > 16) o = mma<T>(load_t<T, DP>(lds.dout, 1, d * 32, lane, hi), p1, o);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const int e = d * 32 + 8 * k + 4 * hi;
@@ -364,29 +386,29 @@ __global__ __launch_bounds__(256, (small_waves<T, DP>())) void k_attn_small_bwd(
 #pragma unroll
         for (int r = 0; r < 16; ++r) t[r] *= up, s[r] *= PUP;
       }
-      put_scores<T>(lds.score, s, col, hi);
+      WeightTile<T>::put(lds.score, split8<T>(s), split8<T>(s + 8), col, hi);
       tile_sync<false>();
 #pragma unroll
       for (int d = 0; d < DP / 32; ++d)
         if (d * 32 < p.dim) {
           if (!SHARE) dv[d] = acc_zero();
-          dv[d] = Mma<T>::run(load_t<T, DP>(lds.dout, 0, d * 32, lane, hi), load_t<T, 32>(lds.score, 0, 0, lane, hi), dv[d]);
+          dv[d] = mma<T>(load_t<T, DP>(lds.dout, 0, d * 32, lane, hi), WeightTile<T>::get(lds.score, 0, lane, hi), dv[d]);
           if (nq > 16)  // (the other half of the contraction is all zeros)
-            dv[d] = Mma<T>::run(load_t<T, DP>(lds.dout, 1, d * 32, lane, hi), load_t<T, 32>(lds.score, 1, 0, lane, hi), dv[d]);
+            dv[d] = mma<T>(load_t<T, DP>(lds.dout, 1, d * 32, lane, hi), WeightTile<T>::get(lds.score, 1, lane, hi), dv[d]);
         }
       tile_sync<false>();
-      put_scores<T>(lds.score, t, col, hi);
+      const Weights<T> t0 = split8<T>(t), t1 = split8<T>(t + 8);
+      WeightTile<T>::put(lds.score, t0, t1, col, hi);
       tile_sync<false>();
 #pragma unroll
       for (int d = 0; d < DP / 32; ++d) {
         if (d * 32 >= p.dim) continue;
         f32x16 x = acc_zero();
-        x = Mma<T>::run(load_t<T, DP>(lds.q, 0, d * 32, lane, hi), load_t<T, 32>(lds.score, 0, 0, lane, hi), x);
-        if (nq > 16) x = Mma<T>::run(load_t<T, DP>(lds.q, 1, d * 32, lane, hi), load_t<T, 32>(lds.score, 1, 0, lane, hi), x);
+        x = mma<T>(load_t<T, DP>(lds.q, 0, d * 32, lane, hi), WeightTile<T>::get(lds.score, 0, lane, hi), x);
+        if (nq > 16) x = mma<T>(load_t<T, DP>(lds.q, 1, d * 32, lane, hi), WeightTile<T>::get(lds.score, 1, lane, hi), x);
 #pragma unroll
         for (int r = 0; r < 16; ++r) dk[d][r] = SHARE ? dk[d][r] + x[r] * down : x[r] * down;
       }
-      const typename vec8<T>::type t0 = pack8<T>(t), t1 = pack8<T>(t + 8);
       const float f = p.scale * down;
       T* oq = (T*)p.dq + ((int64_t)w.col0 * p.heads + head) * p.dim;
       const uint32_t oq_at = (uint32_t)(col * p.heads) * p.dim;
@@ -394,8 +416,8 @@ __global__ __launch_bounds__(256, (small_waves<T, DP>())) void k_attn_small_bwd(
       for (int d = 0; d < DP / 32; ++d) {
         if (d * 32 >= p.dim) continue;
         f32x16 x = acc_zero();
-        x = Mma<T>::run(load_t<T, DP>(lds.k, 0, d * 32, lane, hi), t0, x);
-        if (nk > 16) x = Mma<T>::run(load_t<T, DP>(lds.k, 1, d * 32, lane, hi), t1, x);
+        x = mma<T>(load_t<T, DP>(lds.k, 0, d * 32, lane, hi), t0, x);
+        if (nk > 16) x = mma<T>(load_t<T, DP>(lds.k, 1, d * 32, lane, hi), t1, x);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const int e = d * 32 + 8 * k + 4 * hi;
@@ -480,7 +502,7 @@ __global__ __launch_bounds__(256, (small_waves<T, DP>())) void k_attn_small_bwd(
 // two waves per SIMD and still beat one wave (127 us); float32 rows do not.
 template <typename T, int DP>
 struct PairLds {
-  static constexpr size_t A = TileShape<T, DP>::BYTES, B = TileShape<T, 32>::BYTES;
+  static constexpr size_t A = TileShape<T, DP>::BYTES, B = WeightTile<T>::BYTES;
   static constexpr size_t PULL = sizeof(float) * kTile * kPullLd;
   static constexpr size_t S = B > PULL ? B : PULL;
   T *k, *q, *dout, *score;  // k: two tiles; score: P, dS, and the pulls of one tile
@@ -702,29 +724,29 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 ? 1 : 2)) void k_attn_pair_bwd
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[j][r] *= PUP, u[r] = t[j][r] * up;
         tile_sync<false>();
-        put_scores<T>(lds.score, s[j], col, hi);
+        WeightTile<T>::put(lds.score, split8<T>(s[j]), split8<T>(s[j] + 8), col, hi);
         tile_sync<false>();
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d)
           if (d * 32 < p.dim) {
-            dv[j][d] = Mma<T>::run(load_t<T, DP>(lds.dout, 0, d * 32, lane, hi), load_t<T, 32>(lds.score, 0, 0, lane, hi), dv[j][d]);
+            dv[j][d] = mma<T>(load_t<T, DP>(lds.dout, 0, d * 32, lane, hi), WeightTile<T>::get(lds.score, 0, lane, hi), dv[j][d]);
             if (n_i > 16)
-              dv[j][d] = Mma<T>::run(load_t<T, DP>(lds.dout, 1, d * 32, lane, hi), load_t<T, 32>(lds.score, 1, 0, lane, hi), dv[j][d]);
+              dv[j][d] = mma<T>(load_t<T, DP>(lds.dout, 1, d * 32, lane, hi), WeightTile<T>::get(lds.score, 1, lane, hi), dv[j][d]);
           }
         tile_sync<false>();
-        put_scores<T>(lds.score, u, col, hi);
+        const Weights<T> u0 = split8<T>(u), u1 = split8<T>(u + 8);
+        WeightTile<T>::put(lds.score, u0, u1, col, hi);
         tile_sync<false>();
-        const typename vec8<T>::type u0 = pack8<T>(u), u1 = pack8<T>(u + 8);
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d) {
           if (d * 32 >= p.dim) continue;
           f32x16 x = acc_zero();
-          x = Mma<T>::run(load_t<T, DP>(lds.q, 0, d * 32, lane, hi), load_t<T, 32>(lds.score, 0, 0, lane, hi), x);
-          if (n_i > 16) x = Mma<T>::run(load_t<T, DP>(lds.q, 1, d * 32, lane, hi), load_t<T, 32>(lds.score, 1, 0, lane, hi), x);
+          x = mma<T>(load_t<T, DP>(lds.q, 0, d * 32, lane, hi), WeightTile<T>::get(lds.score, 0, lane, hi), x);
+          if (n_i > 16) x = mma<T>(load_t<T, DP>(lds.q, 1, d * 32, lane, hi), WeightTile<T>::get(lds.score, 1, lane, hi), x);
 #pragma unroll
           for (int r = 0; r < 16; ++r) dk[j][d][r] += x[r] * down;
-          dq[d] = Mma<T>::run(load_t<T, DP>(kt, 0, d * 32, lane, hi), u0, dq[d]);
-          if (n_j > 16) dq[d] = Mma<T>::run(load_t<T, DP>(kt, 1, d * 32, lane, hi), u1, dq[d]);
+          dq[d] = mma<T>(load_t<T, DP>(kt, 0, d * 32, lane, hi), u0, dq[d]);
+          if (n_j > 16) dq[d] = mma<T>(load_t<T, DP>(kt, 1, d * 32, lane, hi), u1, dq[d]);
         }
       }
       if (live) store_column<T, DP>((T*)p.dq + (q_row * p.heads + head) * p.dim, dq, p.scale * down, p.dim, hi);

@@ -51,3 +51,32 @@ def test_float16_scores_of_any_height(sizes, queries, height):
     mean = case.v[:sizes[0]].double().mean(0)
     assert ((got["out"].double() - mean).abs() <= 2 * unit(torch.float16) * case.v.double().abs().mean(0) + 2.0 ** -25).all()
     assert all(torch.isfinite(x).all() for x in got.values())
+
+
+KINDS = {"one tile": dict(sizes=[22, 12, 32, 1] * 3), "one tile, shared heads": dict(sizes=[19, 3, 32] * 3, kv=2, heads=4),
+         "many of one tile": dict(sizes=[1 + (7 * i) % 32 for i in range(520)], heads=2, dim=16), "two tiles": dict(sizes=[44, 33, 64, 50]),
+         "two tiles, dim 64": dict(sizes=[44, 64], dim=64), "a wave each": dict(sizes=[70, 300, 97], kv=4), "shared tiles": dict(sizes=[150, 130, 65, 260] * 4),
+         "pieces": dict(sizes=[1700, 513, 700], queries=[1, 2, 35], kv=2, dim=64), "wide": dict(sizes=[20, 75, 200], heads=4, kv=1, dim=128)}
+
+
+@pytest.mark.parametrize("T", TYPES[1:], ids=str)
+@pytest.mark.parametrize("kind", KINDS)
+def test_results_are_rounded_once(T, kind):
+    """P and dS reach the products in two parts of T each: hi is off by u of a term, lo by u of that.
+    Bound: u |result|, u^2 of the sums' terms (u times what one rounding of P and dS would have been) and the bound of the
+    float32 arithmetic alone.  float16: the parts' absolute step is 2^-39 of P and of the largest dS, at most 2 D max|do|
+    max|v|, for each of n terms; a result under 2^-14 is a multiple of 2^-24."""
+    case = Case(T=T, lut=CLIP, **KINDS[kind])
+    got, once = case.results(), case.reference()
+    case.T = torch.float32
+    bare = case.reference()
+    u, extra = unit(T), 0.0
+    if T == torch.float16:
+        top = lambda x: float(x.double().abs().max())
+        n = int(max(np.max(case.end - case.start), np.max(case.q_end - case.q_start))) * case.heads // case.kv
+        extra = 2.0 ** -25 + 2.0 ** -38 * n * max(top(case.q), top(case.k), top(case.dout), 1.0) * (1 + 2 * case.dim ** 0.5 * top(case.dout) * top(case.v))
+    for name, (value, bound) in bare.items():
+        own = got[name].dtype == T
+        limit = 1.1 * (1 + u) * bound + (u * value.abs() + 1.1 * u * (once[name][1] - bound) + extra if own else 1e-30)
+        off = (got[name].double() - value).abs()
+        assert (off <= limit).all(), (name, int((off > limit).sum()), float((off / limit).max()))
