@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import hashlib
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -46,11 +47,22 @@ def _hipcc() -> str:
     raise RuntimeError("hipcc not found (expected /opt/rocm/bin/hipcc)")
 
 
-def _digest() -> str:
+# the layer operators beside the engine: no kernel of the engine depends on these files
+LAYER_FILES = ["norm.hip", "attention.hip", "attention_fwd.hip", "attention_bwd.hip", "attention_small.hip", "typed.h", "attention.h", "attention_host.h"]
+
+
+def _digest(engine_only: bool = False) -> str:
+    """of all sources and flags; `engine_only`: without the layer operators and their section of vsn.h, which is what a
+    profile of the engine's kernels is measured on"""
     h = hashlib.sha256()
     for f in SOURCES + HEADERS:
+        if engine_only and f in LAYER_FILES:
+            continue
         with open(os.path.join(CSRC, f), "rb") as fh:
-            h.update(fh.read())
+            text = fh.read()
+        if engine_only and os.path.basename(f) == "vsn.h":  # its sections begin with "/* ---- "
+            text = re.sub(rb"(?s)/\* ---- layer operators.*?(?=/\* ---- )", b"", text)
+        h.update(text)
     h.update(" ".join(FLAGS).encode())
     h.update(repr(sorted(PER_FILE_FLAGS.items())).encode())
     return h.hexdigest()

@@ -278,7 +278,7 @@ def parity_check(what, E, F, E64, F64, tol_f=1e-4, tol_e=1e-5, collective=True):
 def traffic_from_profile(workload, kernel):
     """HBM traffic per launch of `kernel`: PMC counters need their own rocprofv3 passes, so the per-launch average
     of the committed run of THIS command is read back from profiles/.  -> (bytes | None, note).  The file carries the
-    digest of the kernel sources it was measured on (ai2bmd_amd.build._digest): when the library has changed since,
+    digest of the engine's sources it was measured on (ai2bmd_amd.build._digest): when the engine has changed since,
     the figure is NOT reported (it would be another build's traffic)."""
     try:
         with open(os.path.join(ROOT, TRAFFIC_PROFILE)) as fh:
@@ -288,7 +288,7 @@ def traffic_from_profile(workload, kernel):
     try:
         from ai2bmd_amd.build import _digest
 
-        dig = _digest()
+        dig = _digest(engine_only=True)
     except Exception:
         dig = None
     if d.get("build_digest") != dig:
@@ -370,7 +370,7 @@ def rocprof_from_profile(workload, kernel):
             d = json.load(fh)
         from ai2bmd_amd.build import _digest
 
-        if d.get("build_digest") != _digest():
+        if d.get("build_digest") != _digest(engine_only=True):
             return None
         return d.get("kernel_ns", {}).get(workload, {}).get(kernel)
     except Exception:

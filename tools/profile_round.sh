@@ -71,12 +71,12 @@ for wl, (tag, pats) in want.items():
             kn.setdefault(wl, {})[key] = dict(calls=calls, avg_ns=sum(int(r["total_ns"]) for r in hit) / calls,
                                               min_ns=min(int(r["min_ns"]) for r in hit))
 res["kernel_ns"] = kn
-res["build_digest"] = _digest()
+res["build_digest"] = _digest(engine_only=True)
 res["_note"] = ("HBM bytes per launch = 2*FETCH_SIZE + WRITE_SIZE (KB*1024) averaged over all launches of the kernel in "
                 "the <tag>_pmc.csv of this directory (rocprofv3 --pmc FETCH_SIZE and --pmc WRITE_SIZE, separate passes, "
                 "tools/profile_round.sh; FETCH_SIZE doubled per MI355X_MICROARCH.md HBM section); build_digest = "
-                "ai2bmd_amd.build._digest() of the kernel sources measured: bench.py reports these figures only while "
-                "the library it runs is that build")
+                "ai2bmd_amd.build._digest(engine_only=True) of the sources measured: bench.py reports these figures only "
+                "while the engine it runs is that build")
 json.dump(res, open(f"{out}/pmc_traffic.json", "w"), indent=1)
 print(res)
 PY
