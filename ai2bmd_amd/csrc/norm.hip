@@ -121,12 +121,12 @@ __global__ __launch_bounds__(256) void k_layernorm(const T* x, int64_t ldx, cons
   }
 }
 
-// partial: [gridDim.x][2][width] column sums of dy h and dy
+// partial: [gridDim.x][2][width] column sums of dy h and dy.  (dx may be dy, as y may be x above: no restrict on either.)
 template <typename T, int VEC, int LPR, int NV, bool ODD>
-__global__ __launch_bounds__(256) void k_layernorm_bwd(const T* __restrict__ dy, int64_t lddy, const T* __restrict__ x,
+__global__ __launch_bounds__(256) void k_layernorm_bwd(const T* dy, int64_t lddy, const T* __restrict__ x,
                                                        int64_t ldx, const float2* __restrict__ stats,
                                                        const void* __restrict__ w, int param_f32, int64_t rows,
-                                                       int width, float inv_width, T* __restrict__ dx, int64_t lddx,
+                                                       int width, float inv_width, T* dx, int64_t lddx,
                                                        float* __restrict__ partial) {
   constexpr int RPB = 256 / LPR;
   const int lane = threadIdx.x % LPR;

@@ -1,0 +1,30 @@
+"""GPU: calls of the layer norm that its header or docstring allows: in place, many rows, parameters on either side."""
+import pytest
+import torch
+
+from test_gpu_layer_norm import TYPES, check, make
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("T", TYPES, ids=str)
+@pytest.mark.parametrize("rows,width,ld", [(37, 256, 256), (3001, 256, 261), (37, 509, 509), (9001, 67, 70), (5, 4095, 4095), (700, 12, 12)])
+def test_the_rows_gradient_may_take_the_place_of_dy(T, rows, width, ld):
+    """vsn_layernorm_backward with dx = dy gives the bits of a call with an array of its own, and leaves what lies between
+    the rows"""
+    from ai2bmd_amd import capi
+    from ai2bmd_amd.norm import DTYPE, layer_norm, layer_norm_backward
+    x, w, b, dy = make(rows, width, T, rows + width)
+    _, stats = layer_norm(x, w, b)
+    dx, dw, db = layer_norm_backward(dy, x, stats, w, b)
+    wide = torch.full((rows, ld), 7.0, dtype=T, device="cuda")
+    wide[:, :width] = dy
+    gw, gb = torch.empty_like(w), torch.empty_like(b)
+    lib = capi.lib()
+    size = lib.vsn_layernorm_workspace(rows, width)
+    work = torch.empty(size // 4, device="cuda")
+    code = DTYPE[T]
+    assert lib.vsn_layernorm_backward(0, code, code, wide.data_ptr(), ld, x.data_ptr(), width, stats.data_ptr(), w.data_ptr(), rows,
+                                      width, wide.data_ptr(), ld, gw.data_ptr(), gb.data_ptr(), work.data_ptr(), size,
+                                      torch.cuda.current_stream().cuda_stream) == 0
+    assert torch.equal(wide[:, :width], dx) and torch.equal(gw, dw) and torch.equal(gb, db) and (wide[:, width:] == 7).all()
