@@ -18,6 +18,7 @@ struct vsn_attn {
   };
   int device = 0, heads = 0, kv_heads = 0, dim = 0, reach = 0, n_rel = 0, n_buckets = 0;
   int64_t used_q = 0, used_k = 0;
+  bool same_rows = true;  // a fragment's queries are its keys' rows
   Side fwd, by_query, by_key;
   int* lut = nullptr;
   char* lists = nullptr;  // what all of these point into
@@ -291,6 +292,7 @@ extern "C" int vsn_attn_create(vsn_attn_handle* out, int device_id, int64_t n, c
     a = new vsn_attn();
     a->device = device_id, a->heads = heads, a->kv_heads = kv_heads, a->dim = head_dim;
     a->used_q = qe[n - 1], a->used_k = host_end[n - 1];
+    a->same_rows = std::equal(qe, qe + n, host_end);
     std::vector<int> lut;
     if (n_buckets) {
       a->reach = reach, a->n_rel = 2 * reach + 1, a->n_buckets = n_buckets;
@@ -368,7 +370,8 @@ extern "C" int vsn_attn_backward(vsn_attn_handle a, const vsn_attn_io* io, const
   if ((uintptr_t)g->dq % 16 || (uintptr_t)g->dk % 16 || (uintptr_t)g->dv % 16) return -22;
   if ((g->dpos || g->dquery_pos || g->dslope) && !io->slope) return -22;
   if (g->dquery_pos && !g->dpos) return -22;
-  if (g->dpos && !g->dquery_pos && (a->used_q != a->used_k || io->rows_q != io->rows_k)) return -22;
+  // one gradient for both ends of a pair: they have to be the same atoms
+  if (g->dpos && !g->dquery_pos && (!a->same_rows || io->rows_q != io->rows_k || io->q_pos != io->k_pos)) return -22;
   if (g->dtable && !io->table) return -22;
   const BackwardSpace s = backward_space(*a, io->rows_q, io->rows_k);
   if (s.size && (!dev_workspace || (uintptr_t)dev_workspace % 16 || workspace_bytes < s.size)) return -22;

@@ -332,7 +332,8 @@ int vsn_layernorm_backward(int device_id, int dtype, int param_dtype, const void
  *     forward call: not wanted); `out` is not read by a backward call
  *     and overlaps none of the inputs.
  *   vsn_attn_grads   dout as out; dq, dk, dv dense.  dpos f32 [rows_k][3]: of both ends of a pair where dquery_pos is
- *     NULL (queries = keys), else of the keys' positions, and dquery_pos f32 [rows_q][3] of the queries'.  dpos, dslope
+ *     NULL (only where the queries are the keys' rows: the same ranges, rows_q = rows_k and q_pos = k_pos), else of the
+ *     keys' positions, and dquery_pos f32 [rows_q][3] of the queries'.  dpos, dslope
  *     f32 [heads], dtable f32 [heads][n_buckets] are overwritten and may be NULL.  Fixed summation order.
  * Asynchronous on `stream`; the workspace (vsn_attn_workspace bytes, 16-byte aligned) belongs to the call until the
  * stream has passed it. */

@@ -1,0 +1,57 @@
+"""GPU: calls of fragment attention that its header allows or refuses, at the C boundary, and launch shapes of large batches."""
+import ctypes as C
+
+import pytest
+import torch
+
+from test_gpu_attention import CLIP, COARSE, TYPES, Case
+
+pytestmark = pytest.mark.gpu
+
+
+def backward(case, plan, flags=1, less=0, **change):
+    """vsn_attn_backward with every gradient of the case, `change`d -> (code, gradients, bytes of workspace)"""
+    from ai2bmd_amd import capi
+    lib = capi.lib()
+    out, stats = plan.forward(case.q, case.k, case.v, save=True, **case.terms)
+    t = case.terms
+    io, held = plan._io(case.q, case.k, case.v, t.get("pos"), t.get("slope"), t.get("residue"), t.get("table"), t.get("query_pos"),
+                        t.get("query_residue"), None)
+    io.stats = stats.data_ptr()
+    f32 = dict(device="cuda")
+    made = dict(dq=torch.empty_like(case.q), dk=torch.empty_like(case.k), dv=torch.empty_like(case.v),
+                dpos=torch.empty(case.k.shape[0], 3, **f32), dquery_pos=torch.empty(case.q.shape[0], 3, **f32),
+                dslope=torch.empty(case.heads, **f32), dtable=torch.empty(case.heads, max(plan.num_buckets, 1), **f32))
+    if not case.apart:
+        made["dquery_pos"] = None
+    for name, value in change.items():
+        if name in made:
+            made[name] = value
+        else:
+            setattr(io, name, value)
+    g = capi.VsnAttnGrads(case.dout.data_ptr(), case.dout.stride(0), case.dout.stride(1),
+                          *(0 if made[n] is None else made[n].data_ptr() for n in ("dq", "dk", "dv", "dpos", "dquery_pos", "dslope", "dtable")))
+    size = lib.vsn_attn_workspace(plan._h, case.q.shape[0], case.k.shape[0], flags)
+    assert size >= 0
+    work = torch.empty(max(size, 16), dtype=torch.uint8, device="cuda")
+    rc = lib.vsn_attn_backward(plan._h, C.byref(io), C.byref(g), work.data_ptr(), size - less, torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    return rc, made, size
+
+
+def test_one_gradient_for_both_ends_only_where_the_rows_are_the_same():
+    # ranges of their own, of the same total: dpos alone is refused, dpos with dquery_pos is not
+    for queries, code in (([5, 3], -22), ([3, 5], -22)):
+        case = Case([3, 5], torch.float32, heads=2, dim=16, lut=CLIP, queries=queries)
+        plan = case.plan()
+        assert backward(case, plan, dquery_pos=None)[0] == code
+        rc, made, _ = backward(case, plan)
+        want = case.results(plan)
+        assert rc == 0 and all(torch.equal(made[n], want[n]) for n in ("dq", "dk", "dv", "dpos", "dquery_pos", "dslope", "dtable"))
+    # the same ranges and the same positions, given twice
+    both = Case([3, 5], torch.float32, heads=2, dim=16, lut=CLIP)
+    apart = Case([3, 5], torch.float32, heads=2, dim=16, lut=CLIP, queries=[3, 5])
+    apart.q, apart.k, apart.v, apart.dout = both.q, both.k, both.v, both.dout
+    apart.terms = {**both.terms, "query_pos": both.terms["pos"], "query_residue": both.terms["residue"]}
+    rc, made, _ = backward(apart, apart.plan(), dquery_pos=None)
+    assert rc == 0 and torch.equal(made["dpos"], both.results()["dpos"])
