@@ -164,11 +164,20 @@ int workers(int items, int heads, int n_rel, int most) {
 
 constexpr int64_t kMaxRowStep = (int64_t)1 << 25;
 
-// launches count their waves in 32 bits
+// A launch has fewer than 2^32 threads along an axis: whole workgroups of four waves here.  (Joins have fewer: there are
+// none from kPieceWaves waves on; the backward passes' workers are bounded by workers().)
+constexpr int64_t kMostGroups = ((int64_t)1 << 24) - 1;
 bool countable(const Lists& l, int heads) {
-  const int64_t most = ((int64_t)1 << 31) / heads;
-  return (int64_t)l.small.size() < most && (int64_t)l.pair.size() < most && (int64_t)l.lone.size() < most &&
-         (int64_t)l.coop.size() < most && (int64_t)l.join.size() < ((int64_t)1 << 26);
+  const int64_t waves = std::max(l.small.size(), std::max(l.pair.size(), l.lone.size())) * (int64_t)heads;
+  return (waves + 3) / 4 <= kMostGroups && (int64_t)l.coop.size() * heads <= kMostGroups;
+}
+// workgroups of the backward pass's last launch (join_launch): positions by block and fragment, slopes, table
+bool joinable(const vsn_attn& a, const vsn_attn_grads& g) {
+  int64_t n = g.dslope ? a.heads : 0;
+  if (g.dtable) n += (int64_t)a.heads * a.n_buckets;
+  if (g.dpos) n += (int64_t)a.by_key.blocks + a.by_query.pair + a.by_query.small;
+  if (g.dquery_pos) n += (int64_t)a.by_query.blocks + a.by_query.pair + a.by_query.small;
+  return n <= kMostGroups;
 }
 
 struct Workspace {
@@ -282,8 +291,6 @@ extern "C" int vsn_attn_create(vsn_attn_handle* out, int device_id, int64_t n, c
   if (n_buckets)
     for (int i = 0; i < 2 * reach + 1; ++i)
       if (host_buckets[i] < 0 || host_buckets[i] >= n_buckets) return -22;
-  DeviceScope scope(device_id);
-  if (!scope.ok) return -19;
   const int64_t* qs = host_query_start ? host_query_start : host_start;
   const int64_t* qe = host_query_start ? host_query_end : host_end;
   vsn_attn* a = nullptr;
@@ -311,6 +318,11 @@ extern "C" int vsn_attn_create(vsn_attn_handle* out, int device_id, int64_t n, c
     if (!countable(fwd, heads) || !countable(by_query, heads) || !countable(by_key, kv_heads)) {
       delete a;
       return -22;
+    }
+    DeviceScope scope(device_id);
+    if (!scope.ok) {
+      delete a;
+      return -19;
     }
     Packed all;
     all.add(fwd, a->fwd);
@@ -373,6 +385,7 @@ extern "C" int vsn_attn_backward(vsn_attn_handle a, const vsn_attn_io* io, const
   // one gradient for both ends of a pair: they have to be the same atoms
   if (g->dpos && !g->dquery_pos && (!a->same_rows || io->rows_q != io->rows_k || io->q_pos != io->k_pos)) return -22;
   if (g->dtable && !io->table) return -22;
+  if (!joinable(*a, *g)) return -22;
   const BackwardSpace s = backward_space(*a, io->rows_q, io->rows_k);
   if (s.size && (!dev_workspace || (uintptr_t)dev_workspace % 16 || workspace_bytes < s.size)) return -22;
   DeviceScope scope(a->device);

@@ -322,7 +322,8 @@ int vsn_layernorm_backward(int device_id, int dtype, int param_dtype, const void
  *     queries the same rows, or those of host_query_start / host_query_end (both NULL: the same), e.g. one read-out row
  *     per fragment.  Ranges contiguous and ascending from 0, as in vsn_forces; empty ones are allowed.  head_dim: a
  *     multiple of 8, 8 ... 128; kv_heads divides heads.  n_buckets > 0: host_buckets[2 reach + 1] gives the bucket of
- *     each difference clipped to -reach ... reach (reach <= 1023).  A plan holds no results and may be used from any
+ *     each difference clipped to -reach ... reach (reach <= 1023).  heads <= 1024, and together fewer than 2^26
+ *     waves of 32 rows x head (-22 where a launch could not count them).  A plan holds no results and may be used from any
  *     stream, by several calls at once; make it outside of a stream capture.
  *   vsn_attn_io   `q` [rows_q][heads][head_dim], `k`, `v` [rows_k][kv_heads][head_dim], `out` as q: last axis dense, the
  *     strides (elements) of rows (at most 2^25) and heads multiples of 16 bytes, addresses too.  rows_* may exceed the plan's: rows

@@ -112,3 +112,25 @@ def test_relative_buckets():
     for bad in ((31, 128), (2, 128), (0, 4), (32, 1024), (32, -1)):
         with pytest.raises(ValueError):
             relative_buckets(*bad)
+
+
+def test_plans_that_no_launch_could_count_are_refused(lib_built):
+    """2^32 threads along an axis: 2^26 waves of 64.  Fragments of one row with 1024 heads (too many heads for the kernel of
+    one-tile fragments): a wave per fragment and head."""
+    import numpy as np
+
+    from ai2bmd_amd import capi
+    L = capi.lib()
+
+    def create(n, heads, rows=1):
+        end = np.arange(1, n + 1, dtype=np.int64) * rows
+        h = C.c_void_p()
+        rc = L.vsn_attn_create(C.byref(h), 0, n, capi.i64_ptr(end - rows), capi.i64_ptr(end), None, None, heads, heads, 8, 0, None, 0)
+        if rc == 0:
+            L.vsn_attn_destroy(h)
+        return rc
+
+    fits = 0 if torch.cuda.is_available() else -19
+    assert create(65535, 1024) == fits and create(65536, 1024) == -22
+    # workgroups of four waves that share the tiles of 128 rows: 2^24 of them
+    assert create(16383, 1024, 65) == fits and create(16384, 1024, 65) == -22
