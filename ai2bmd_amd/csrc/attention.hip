@@ -334,6 +334,7 @@ extern "C" int vsn_attn_create(vsn_attn_handle* out, int device_id, int64_t n, c
     ok = false;
   }
   if (!ok) {
+    (void)hipGetLastError();
     vsn_attn_destroy(a);
     return -12;
   }

@@ -32,8 +32,10 @@ inline int lone_waves(int64_t total, size_t bytes) {
 }
 
 inline bool allow_lds(const void* kernel, size_t bytes) {
-  return bytes <= 64 * 1024 ||
-         hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) == hipSuccess;
+  if (bytes <= 64 * 1024 || hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) == hipSuccess)
+    return true;
+  (void)hipGetLastError();
+  return false;
 }
 
 // Waves per small fragment: one that walks all heads, so distances are computed once and positions' gradients need no

@@ -26,13 +26,15 @@ struct vec8<_Float16> {
   typedef f16x8 type;
 };
 
-// Makes a device current for the length of a call and puts the caller's back.
+// Makes a device current for the length of a call and puts the caller's back.  (A failure is the return code's to report:
+// left behind, the runtime's last error would be taken for one of the next call's, here or in torch.)
 struct DeviceScope {
   int before = -1;
   bool ok = false;
   explicit DeviceScope(int device) {
     if (hipGetDevice(&before) != hipSuccess) before = -1;
     ok = before == device || hipSetDevice(device) == hipSuccess;
+    if (!ok) (void)hipGetLastError();
     if (before == device) before = -1;
   }
   ~DeviceScope() {

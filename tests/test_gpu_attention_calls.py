@@ -55,3 +55,16 @@ def test_one_gradient_for_both_ends_only_where_the_rows_are_the_same():
     apart.terms = {**both.terms, "query_pos": both.terms["pos"], "query_residue": both.terms["residue"]}
     rc, made, _ = backward(apart, apart.plan(), dquery_pos=None)
     assert rc == 0 and torch.equal(made["dpos"], both.results()["dpos"])
+
+
+def test_a_refused_device_leaves_no_error_behind():
+    from ai2bmd_amd.attention import FragmentAttention
+    from ai2bmd_amd import capi
+    from ai2bmd_amd.norm import layer_norm
+    x = torch.randn(4, 64, device="cuda")
+    for _ in range(2):
+        with pytest.raises(RuntimeError, match="-19"):
+            FragmentAttention([0], [4], 2, 8, device="cuda:99")
+        layer_norm(x)
+        assert capi.lib().vsn_layernorm(99, 0, 0, x.data_ptr(), 64, None, None, 4, 64, 1e-5, x.data_ptr(), 64, None, None) == -19
+        assert (x + 1).isfinite().all()
