@@ -218,7 +218,7 @@ class FragmentAttention:
         dslope [heads], dtable [heads, buckets]; None where the term is absent.  `stats`: what forward returned."""
         io, held = self._io(q, k, v, pos, slope, residue, table, query_pos, query_residue, scale)
         q, k = held[0], held[1]
-        no_graph(dout)
+        no_graph(dout, stats)
         dout = self._rows(dout, "dout", self.num_heads, self.rows_q, q.dtype, exact=q.shape[0])
         stats = self._small(stats, "stats", (self.num_heads, q.shape[0], 2), torch.float32)
         io.stats = stats.data_ptr()

@@ -7,6 +7,7 @@ Like everything here it is differentiated by hand: the two functions are called 
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import capi
 
@@ -29,7 +30,11 @@ def on_device(t: torch.Tensor, name: str, device=None) -> None:
 
 
 def no_graph(*tensors) -> None:
-    """The operators build no autograd graph; a result that silently cut one would train nothing."""
+    """The operators build no autograd graph and carry no tangent; a result that silently cut one would train nothing."""
+    if forward_ad._current_level >= 0:  # (within forward_ad.dual_level: the tensors have to be looked at)
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError("no tangent is computed: forward-mode differentiation is not supported")
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
@@ -92,7 +97,7 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, out=None):
     `weight`, `bias` [width] of x's type or float32 (None: 1 and 0).  `out`: contiguous, of x's shape and type; it may be x.
     `stats` float32 [rows, 2] (mean, 1 / sqrt(var + eps)) goes to layer_norm_backward.  On the current stream of x's device."""
     width, code, param_code = _check(x, weight, bias)
-    no_graph(x, weight, bias)
+    no_graph(x, weight, bias, out)
     if not eps >= 0:
         raise ValueError("eps: a number >= 0 expected")
     if out is not None:
@@ -114,7 +119,7 @@ def layer_norm_backward(dy, x, stats, weight=None, bias=None):
 
     dweight / dbias have the parameters' type and are None where the parameter is.  Sums run in a fixed order."""
     width, code, param_code = _check(x, weight, bias)
-    no_graph(dy, x, weight, bias)
+    no_graph(dy, x, stats, weight, bias)
     on_device(dy, "dy", x.device)
     on_device(stats, "stats", x.device)
     if dy.shape != x.shape or dy.dtype != x.dtype:

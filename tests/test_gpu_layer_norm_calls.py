@@ -28,3 +28,37 @@ def test_the_rows_gradient_may_take_the_place_of_dy(T, rows, width, ld):
                                       width, wide.data_ptr(), ld, gw.data_ptr(), gb.data_ptr(), work.data_ptr(), size,
                                       torch.cuda.current_stream().cuda_stream) == 0
     assert torch.equal(wide[:, :width], dx) and torch.equal(gw, dw) and torch.equal(gb, db) and (wide[:, width:] == 7).all()
+
+
+@pytest.mark.parametrize("T", TYPES[1:], ids=str)
+@pytest.mark.parametrize("rows,width", [(40_001, 256), (20_011, 509), (70_003, 33), (300_007, 8), (9_001, 4096)])
+def test_16_bit_rows_that_are_walked_in_several_turns(T, rows, width):
+    """more rows than 2048 (forward) and 1024 (backward) workgroups take in one turn"""
+    from ai2bmd_amd.norm import layer_norm, layer_norm_backward
+    x, w, b, dy = make(rows, width, T, 17)
+    y, stats = layer_norm(x, w, b)
+    check(x, w, b, dy, y, layer_norm_backward(dy, x, stats, w, b))
+    for at in (0, rows // 2, rows - 9):
+        assert torch.equal(layer_norm(x[at:at + 9], w, b)[0], y[at:at + 9])
+
+
+def test_outputs_and_tangents_of_a_graph_are_refused():
+    from torch.autograd import forward_ad
+
+    from ai2bmd_amd.attention import FragmentAttention
+    from ai2bmd_amd.norm import layer_norm, layer_norm_backward
+    x, w, b, dy = make(8, 64, torch.float32, 2)
+    _, stats = layer_norm(x, w, b)
+    leaf = torch.zeros(8, 64, device="cuda", requires_grad=True)
+    with pytest.raises(RuntimeError, match="autograd"):
+        layer_norm(x, w, b, out=leaf)
+    with torch.no_grad():
+        assert layer_norm(x, w, b, out=leaf)[0] is leaf
+    plan = FragmentAttention([0], [8], 2, 32)
+    rows = x.view(8, 2, 32)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: layer_norm(dual, w, b), lambda: layer_norm(x, forward_ad.make_dual(w, w), b), lambda: layer_norm_backward(dual, x, stats, w, b),
+                     lambda: plan.forward(rows, dual.view(8, 2, 32), rows)):
+            with torch.no_grad(), pytest.raises(RuntimeError, match="tangent"):
+                call()
