@@ -64,6 +64,12 @@ def _rows(t: torch.Tensor, width: int):
     return t.contiguous(), rows, width
 
 
+def _span(t: torch.Tensor):
+    """first address of a tensor and the one behind its last element"""
+    first = t.data_ptr()
+    return first, first + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size() if t.numel() else first
+
+
 def _param(p, x, name: str) -> None:
     if not p.is_cuda or p.device != x.device:
         on_device(p, name, x.device)
@@ -94,7 +100,7 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, out=None):
     """y = (x - mean) / sqrt(var + eps) * weight + bias over the last axis -> (y, stats).
 
     `x` [..., width], float32 / bfloat16 / float16; evenly spaced rows are read in place, other layouts are copied.
-    `weight`, `bias` [width] of x's type or float32 (None: 1 and 0).  `out`: contiguous, of x's shape and type; it may be x.
+    `weight`, `bias` [width] of x's type or float32 (None: 1 and 0).  `out`: contiguous, of x's shape and type; x itself, or apart from all inputs.
     `stats` float32 [rows, 2] (mean, 1 / sqrt(var + eps)) goes to layer_norm_backward.  On the current stream of x's device."""
     width, code, param_code = _check(x, weight, bias)
     no_graph(x, weight, bias, out)
@@ -106,6 +112,10 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, out=None):
             raise ValueError("out: contiguous, with x's shape and type expected")
     y = x.new_empty(x.shape) if out is None else out
     src, rows, ld = _rows(x, width)
+    if out is not None:
+        (o0, o1), (x0, x1) = _span(out), _span(src)
+        if o0 < x1 and x0 < o1 and not (o0 == x0 and ld == width):
+            raise ValueError("out: x itself or memory apart from it expected (their rows overlap)")
     stats = torch.empty(rows, 2, dtype=torch.float32, device=x.device)
     rc = capi.lib().vsn_layernorm(x.device.index, code, param_code, src.data_ptr(), ld, ptr(weight), ptr(bias), rows,
                                   width, eps, y.data_ptr(), width, stats.data_ptr(), stream_of(x))

@@ -62,3 +62,20 @@ def test_outputs_and_tangents_of_a_graph_are_refused():
                      lambda: plan.forward(rows, dual.view(8, 2, 32), rows)):
             with torch.no_grad(), pytest.raises(RuntimeError, match="tangent"):
                 call()
+
+
+def test_an_output_that_overlaps_its_rows_is_refused():
+    from ai2bmd_amd.norm import layer_norm
+    wide = torch.randn(12, 64, device="cuda")
+    flat = wide.view(-1)
+    part = wide[:10, :32]  # rows 64 apart: an output of rows 32 apart at the same address would meet rows not read yet
+    for x, out in ((part, flat[:320].view(10, 32)), (wide[:10], flat[64:704].view(10, 64)), (wide[2:12], flat[64:704].view(10, 64)),
+                   (part, flat[5:325].view(10, 32))):
+        with pytest.raises(ValueError, match="overlap"):
+            layer_norm(x, out=out)
+    want = layer_norm(wide[:5])[0]
+    assert torch.equal(layer_norm(wide[:5], out=wide[5:10])[0], want)       # side by side
+    assert torch.equal(layer_norm(wide[:5], out=flat[:320].view(5, 64))[0], want) and torch.equal(wide[:5], want)
+    columns = torch.randn(32, 10, device="cuda")                             # copied first: may be written over
+    want = layer_norm(columns.t())[0]
+    assert torch.equal(layer_norm(columns.t(), out=columns.view(10, 32))[0], want)
