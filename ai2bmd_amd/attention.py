@@ -21,7 +21,7 @@ import torch
 from . import capi
 from .norm import dtype_code, no_graph, on_device, ptr, stream_of
 
-MAX_REACH, MAX_BUCKETS, MAX_ROW_STEP = 1023, 4096, 1 << 25
+MAX_REACH, MAX_BUCKETS, MAX_ROW_STEP, MAX_ROWS, MAX_HEADS = 1023, 4096, 1 << 25, 1 << 30, 1024
 AttentionGrads = namedtuple("AttentionGrads", "dq dk dv dpos dquery_pos dslope dtable")
 
 
@@ -50,11 +50,16 @@ def relative_buckets(num_buckets: int, reach: int) -> np.ndarray:
     return (np.asarray(bucket)[np.abs(offset)] + np.where(offset > 0, half, 0)).astype(np.int32)
 
 
-def _range(a, name: str) -> np.ndarray:
-    a = np.ascontiguousarray(a, dtype=np.int64)
-    if a.ndim != 1:
-        raise ValueError(f"{name}: one-dimensional array expected")
-    return a
+def _whole(a, name: str, dtype) -> np.ndarray:
+    """one-dimensional array of whole numbers in `dtype`; a conversion that would change a value is refused"""
+    a = np.asarray(a)
+    if a.ndim != 1 or a.dtype.kind not in "iuf":
+        raise ValueError(f"{name}: one-dimensional array of whole numbers expected")
+    with np.errstate(invalid="ignore"):
+        to = np.ascontiguousarray(a, dtype=dtype)
+    if (to != a).any():
+        raise ValueError(f"{name}: whole numbers in the range of {np.dtype(dtype).name} expected")
+    return to
 
 
 class FragmentAttention:
@@ -74,25 +79,30 @@ class FragmentAttention:
         self.device = torch.device("cuda", torch.device(device).index or 0)
         self.num_heads, self.head_dim = int(num_heads), int(head_dim)
         self.num_kv_heads = self.num_heads if num_kv_heads is None else int(num_kv_heads)
-        k0, k1 = _range(start, "start"), _range(end, "end")
+        k0, k1 = _whole(start, "start", np.int64), _whole(end, "end", np.int64)
         if (query_start is None) != (query_end is None):
             raise ValueError("query_start and query_end come together")
         self.own_queries = query_start is not None
-        q0, q1 = (_range(query_start, "query_start"), _range(query_end, "query_end")) if self.own_queries else (k0, k1)
+        q0, q1 = (k0, k1) if not self.own_queries else (_whole(query_start, "query_start", np.int64),
+                                                        _whole(query_end, "query_end", np.int64))
         for lo, hi, name in ((k0, k1, "start / end"), (q0, q1, "query_start / query_end")):
             if len(lo) == 0 or len(lo) != len(k0) or len(hi) != len(k0) or lo[0] != 0 or (lo[1:] != hi[:-1]).any() \
                     or (hi < lo).any():
                 raise ValueError(f"{name}: contiguous ascending ranges from 0, one per fragment, expected")
+            if hi[-1] > MAX_ROWS:
+                raise ValueError(f"{name}: at most 2^30 rows expected")
         if self.num_heads < 1 or self.num_kv_heads < 1 or self.num_heads % self.num_kv_heads:
             raise ValueError("num_kv_heads has to divide num_heads")
+        if self.num_heads > MAX_HEADS:
+            raise ValueError(f"num_heads: at most {MAX_HEADS} expected")
         if not 8 <= self.head_dim <= 128 or self.head_dim % 8:
             raise ValueError("head_dim: a multiple of 8 from 8 to 128 expected")
         self.rows_k, self.rows_q = int(k1[-1]), int(q1[-1])
         self.num_buckets, reach, lut = 0, 0, None
         if buckets is not None:
-            lut = np.ascontiguousarray(buckets, dtype=np.int32)
+            lut = _whole(buckets, "buckets", np.int32)
             reach = len(lut) // 2
-            if lut.ndim != 1 or len(lut) % 2 == 0 or reach > MAX_REACH or lut.min() < 0:
+            if len(lut) % 2 == 0 or reach > MAX_REACH or lut.min() < 0:
                 raise ValueError(f"buckets: [2 reach + 1] bucket numbers, reach <= {MAX_REACH}, expected")
             self.num_buckets = int(lut.max()) + 1 if num_buckets is None else int(num_buckets)
             if not lut.max() < self.num_buckets <= MAX_BUCKETS:
