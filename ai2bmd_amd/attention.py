@@ -211,7 +211,8 @@ class FragmentAttention:
         io.out, io.out_row, io.out_head = out.data_ptr(), out.stride(0), out.stride(1)
         stats = None
         if save:
-            stats = torch.empty(self.num_heads, rows, 2, dtype=torch.float32, device=self.device)
+            make = torch.empty if rows == self.rows_q else torch.zeros
+            stats = make(self.num_heads, rows, 2, dtype=torch.float32, device=self.device)
             io.stats = stats.data_ptr()
         work, size = self._space(rows, held[1].shape[0], False)
         rc = self._L.vsn_attn_forward(self._h, C.byref(io), ptr(work), size, stream_of(held[0]))

@@ -68,3 +68,12 @@ def test_a_refused_device_leaves_no_error_behind():
         layer_norm(x)
         assert capi.lib().vsn_layernorm(99, 0, 0, x.data_ptr(), 64, None, None, 4, 64, 1e-5, x.data_ptr(), 64, None, None) == -19
         assert (x + 1).isfinite().all()
+
+
+def test_statistics_of_rows_behind_the_last_fragment_are_zeros():
+    case = Case([20, 45], torch.float32, extra=5)
+    plan = case.plan()
+    for _ in range(3):
+        torch.full((8, 70, 2), 7.0, device="cuda")  # memory that the next allocation takes over
+        _, stats = plan.forward(case.q, case.k, case.v, save=True, **case.terms)
+        assert not stats[:, 65:].any() and (stats[:, :65, 1] > 0).all()
