@@ -22,6 +22,7 @@ from . import capi
 from .norm import dtype_code, no_graph, on_device, ptr, stream_of
 
 MAX_REACH, MAX_BUCKETS, MAX_ROW_STEP, MAX_ROWS, MAX_HEADS = 1023, 4096, 1 << 25, 1 << 30, 1024
+BACKWARD, NO_POS, NO_TABLE = 1, 2, 4  # VSN_ATTN_* (include/vsn.h)
 AttentionGrads = namedtuple("AttentionGrads", "dq dk dv dpos dquery_pos dslope dtable")
 
 
@@ -186,8 +187,8 @@ class FragmentAttention:
         make = torch.empty if shape[0] == used else torch.zeros
         return make(shape, dtype=dtype, device=self.device)
 
-    def _space(self, rows_q: int, rows_k: int, backward: bool):
-        size = self._L.vsn_attn_workspace(self._h, rows_q, rows_k, int(backward))
+    def _space(self, rows_q: int, rows_k: int, backward: int):
+        size = self._L.vsn_attn_workspace(self._h, rows_q, rows_k, backward)
         return torch.empty(size, dtype=torch.uint8, device=self.device) if size else None, size
 
     # -- calls -------------------------------------------------------------------------------------------------------
@@ -214,7 +215,7 @@ class FragmentAttention:
             make = torch.empty if rows == self.rows_q else torch.zeros
             stats = make(self.num_heads, rows, 2, dtype=torch.float32, device=self.device)
             io.stats = stats.data_ptr()
-        work, size = self._space(rows, held[1].shape[0], False)
+        work, size = self._space(rows, held[1].shape[0], 0)
         rc = self._L.vsn_attn_forward(self._h, C.byref(io), ptr(work), size, stream_of(held[0]))
         if rc:
             raise RuntimeError(f"vsn_attn_forward failed ({rc})")
@@ -247,7 +248,7 @@ class FragmentAttention:
         address = lambda t: 0 if t is None else t.data_ptr()
         grads = capi.VsnAttnGrads(dout.data_ptr(), dout.stride(0), dout.stride(1), dq.data_ptr(), dk.data_ptr(),
                                   dv.data_ptr(), address(dpos), address(dquery_pos), address(dslope), address(dtable))
-        work, size = self._space(q.shape[0], k.shape[0], True)
+        work, size = self._space(q.shape[0], k.shape[0], BACKWARD | (NO_POS if pos is None else 0) | (NO_TABLE if table is None else 0))
         rc = self._L.vsn_attn_backward(self._h, C.byref(io), C.byref(grads), ptr(work), size, stream_of(q))
         if rc:
             raise RuntimeError(f"vsn_attn_backward failed ({rc})")

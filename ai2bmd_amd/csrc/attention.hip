@@ -195,7 +195,7 @@ struct BackwardSpace {
   int parts;
 };
 
-BackwardSpace backward_space(const vsn_attn& a, int64_t rows_q, int64_t rows_k) {
+BackwardSpace backward_space(const vsn_attn& a, int64_t rows_q, int64_t rows_k, bool pos, bool table) {
   BackwardSpace s;
   s.workers.lone = workers(a.by_query.lone, a.heads, a.n_rel, a.n_rel ? 2048 : 4096);
   s.workers.coop = workers(a.by_query.coop, a.heads, a.n_rel, 2048);
@@ -204,16 +204,16 @@ BackwardSpace backward_space(const vsn_attn& a, int64_t rows_q, int64_t rows_k) 
   s.parts = s.workers.lone + s.workers.coop + s.workers.small + s.workers.pair;
   Workspace w;
   s.delta = w.take(rows_q * a.heads * 8);
-  s.pos_q = w.take(rows_q * a.heads * 12);
-  s.pos_k = w.take(rows_k * a.kv_heads * 12);
+  s.pos_q = w.take(pos ? rows_q * a.heads * 12 : 0);
+  s.pos_k = w.take(pos ? rows_k * a.kv_heads * 12 : 0);
   s.slope = w.take((int64_t)s.parts * a.heads * kCoopWaves * 4);
-  s.hist = w.take((int64_t)s.parts * a.heads * a.n_rel * 4);
+  s.hist = w.take(table ? (int64_t)s.parts * a.heads * a.n_rel * 4 : 0);
   // pieces: the dq pass and the dk / dv pass use the same space one after the other
   const int64_t q_cols = (int64_t)a.by_query.slots * a.heads * kTile, k_cols = (int64_t)a.by_key.slots * a.kv_heads * kTile;
   s.ml = w.take(q_cols * 8);
   s.o = w.take(std::max(q_cols, k_cols) * a.dim * 4);
   s.o2 = w.take(k_cols * a.dim * 4);
-  s.g = w.take(std::max(q_cols, k_cols) * 16);
+  s.g = w.take(pos ? std::max(q_cols, k_cols) * 16 : 0);
   s.size = w.size;
   return s;
 }
@@ -350,8 +350,9 @@ extern "C" void vsn_attn_destroy(vsn_attn_handle a) {
 }
 
 extern "C" int64_t vsn_attn_workspace(vsn_attn_handle a, int64_t rows_q, int64_t rows_k, int backward) {
-  if (!a || rows_q < a->used_q || rows_k < a->used_k) return -22;
-  return backward ? vsn::backward_space(*a, rows_q, rows_k).size : vsn::forward_space(*a, nullptr);
+  if (!a || rows_q < a->used_q || rows_k < a->used_k || backward < 0 || backward > 7) return -22;
+  if (!(backward & VSN_ATTN_BACKWARD)) return vsn::forward_space(*a, nullptr);
+  return vsn::backward_space(*a, rows_q, rows_k, !(backward & VSN_ATTN_NO_POS), !(backward & VSN_ATTN_NO_TABLE)).size;
 }
 
 extern "C" int vsn_attn_forward(vsn_attn_handle a, const vsn_attn_io* io, void* dev_workspace, int64_t workspace_bytes,
@@ -387,7 +388,7 @@ extern "C" int vsn_attn_backward(vsn_attn_handle a, const vsn_attn_io* io, const
   if (g->dpos && !g->dquery_pos && (!a->same_rows || io->rows_q != io->rows_k || io->q_pos != io->k_pos)) return -22;
   if (g->dtable && !io->table) return -22;
   if (!joinable(*a, *g)) return -22;
-  const BackwardSpace s = backward_space(*a, io->rows_q, io->rows_k);
+  const BackwardSpace s = backward_space(*a, io->rows_q, io->rows_k, g->dpos != nullptr, g->dtable != nullptr);
   if (s.size && (!dev_workspace || (uintptr_t)dev_workspace % 16 || workspace_bytes < s.size)) return -22;
   DeviceScope scope(a->device);
   if (!scope.ok) return -19;

@@ -362,6 +362,8 @@ int vsn_attn_create(vsn_attn_handle* out, int device_id, int64_t n_fragments, co
                     const int64_t* host_end, const int64_t* host_query_start, const int64_t* host_query_end, int heads,
                     int kv_heads, int head_dim, int reach, const int32_t* host_buckets, int n_buckets);
 void vsn_attn_destroy(vsn_attn_handle a);
+/* backward: 0, or VSN_ATTN_BACKWARD and what the call does without (the table's sums reach 100 MB) */
+enum { VSN_ATTN_BACKWARD = 1, VSN_ATTN_NO_POS = 2 /* dpos is NULL */, VSN_ATTN_NO_TABLE = 4 /* dtable is NULL */ };
 int64_t vsn_attn_workspace(vsn_attn_handle a, int64_t rows_q, int64_t rows_k, int backward);
 int vsn_attn_forward(vsn_attn_handle a, const vsn_attn_io* io, void* dev_workspace, int64_t workspace_bytes,
                      void* stream);

@@ -77,3 +77,21 @@ def test_statistics_of_rows_behind_the_last_fragment_are_zeros():
         torch.full((8, 70, 2), 7.0, device="cuda")  # memory that the next allocation takes over
         _, stats = plan.forward(case.q, case.k, case.v, save=True, **case.terms)
         assert not stats[:, 65:].any() and (stats[:, :65, 1] > 0).all()
+
+
+def test_workspace_is_for_the_terms_that_a_call_has():
+    case = Case([150, 12, 60, 400], torch.float32, heads=4, dim=16, lut=list(range(257)))
+    plan = case.plan()
+    every = ("dq", "dk", "dv", "dpos", "dslope", "dtable")
+    rc, want, full = backward(case, plan)
+    assert rc == 0 and backward(case, plan, less=1)[0] == -22
+    partial = {2: dict(dpos=None), 4: dict(dtable=None), 6: dict(dpos=None, dtable=None)}
+    sizes = {}
+    for flags, without in partial.items():
+        rc, made, sizes[flags] = backward(case, plan, flags=1 | flags, **without)
+        assert rc == 0 and all(torch.equal(made[n], want[n]) for n in every if made[n] is not None)
+        assert backward(case, plan, flags=1 | flags, less=1, **without)[0] == -22
+    assert sizes[6] < sizes[2] < full and sizes[6] < sizes[4] < full
+    assert full - sizes[4] >= 4 * 257 * 4 and full - sizes[2] >= 622 * 4 * 24   # the table's sums; the positions' of both sides
+    assert backward(case, plan, flags=3)[0] == backward(case, plan, flags=5)[0] == -22     # too small for what is asked
+    assert plan._L.vsn_attn_workspace(plan._h, 622, 622, 8) == plan._L.vsn_attn_workspace(plan._h, 622, 622, -1) == -22
