@@ -95,3 +95,30 @@ def test_workspace_is_for_the_terms_that_a_call_has():
     assert full - sizes[4] >= 4 * 257 * 4 and full - sizes[2] >= 622 * 4 * 24   # the table's sums; the positions' of both sides
     assert backward(case, plan, flags=3)[0] == backward(case, plan, flags=5)[0] == -22     # too small for what is asked
     assert plan._L.vsn_attn_workspace(plan._h, 622, 622, 8) == plan._L.vsn_attn_workspace(plan._h, 622, 622, -1) == -22
+
+
+# Launch shapes of large batches: a worker of the backward passes takes a second item (from 4096 one-tile fragments, 4096 / heads
+# two-tile ones, 4096 / heads runs of 32 rows, 2048 / heads with a table or of 128 shared rows), and workgroups hold several
+# waves with LDS of their own (from 1024 waves of one-tile fragments, 16 384 of the others).
+
+@pytest.mark.parametrize("T", TYPES, ids=str)
+def test_more_one_tile_fragments_than_workers(T):
+    Case([1 + (7 * i) % 32 for i in range(4500)], T, heads=2, dim=8, lut=COARSE).check()
+
+
+@pytest.mark.parametrize("T", TYPES, ids=str)
+@pytest.mark.parametrize("lut", [None, COARSE], ids=["slope", "table"])
+def test_more_two_tile_fragments_than_workers(T, lut):
+    Case([33 + i % 12 for i in range(700)], T, dim=16, lut=lut).check()
+
+
+@pytest.mark.parametrize("T", TYPES, ids=str)
+@pytest.mark.parametrize("kv,dim", [(8, 72), (2, 24)])
+def test_more_runs_of_32_rows_than_workers_and_several_waves_a_workgroup(T, kv, dim):
+    Case([33 + (5 * i) % 32 for i in range(1100)], T, kv=kv, dim=dim, lut=COARSE).check()
+
+
+@pytest.mark.parametrize("T", TYPES, ids=str)
+@pytest.mark.parametrize("dim", [16, 64])
+def test_more_shared_tiles_than_workers(T, dim):
+    Case([65 + (11 * i) % 90 for i in range(300)], T, dim=dim, lut=COARSE).check()
