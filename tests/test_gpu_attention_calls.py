@@ -122,3 +122,23 @@ def test_more_runs_of_32_rows_than_workers_and_several_waves_a_workgroup(T, kv, 
 @pytest.mark.parametrize("dim", [16, 64])
 def test_more_shared_tiles_than_workers(T, dim):
     Case([65 + (11 * i) % 90 for i in range(300)], T, dim=dim, lut=COARSE).check()
+
+
+@pytest.mark.parametrize("T", TYPES, ids=str)
+def test_thousands_of_keys(T):
+    Case([9001, 700], T, heads=2, dim=16, lut=COARSE).check()
+
+
+@pytest.mark.parametrize("sizes,step", [([64], 1 << 25), ([30, 34], 1 << 25), ([4101], 1 << 20), ([300, 3801], 1 << 20)])
+def test_offsets_beyond_32_bits(sizes, step):
+    """rows up to 2^25 elements apart: a tile's offsets pass 2^31 elements, an array's 2^32"""
+    case = Case(sizes, torch.bfloat16, heads=2, dim=16, lut=CLIP)
+    plan = case.plan()
+    want = case.results(plan)
+    for name in ("q", "k", "v", "dout"):
+        rows = getattr(case, name)
+        wide = torch.empty((rows.shape[0] - 1) * step + 32, dtype=torch.bfloat16, device="cuda").as_strided((rows.shape[0], 2, 16), (step, 16, 1))
+        setattr(case, name, wide.copy_(rows))
+        assert plan._rows(wide, name, 2, 0, torch.bfloat16) is wide  # read in place
+    got = case.results(plan)
+    assert all(torch.equal(got[n], want[n]) for n in want)

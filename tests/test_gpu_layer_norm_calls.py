@@ -79,3 +79,24 @@ def test_an_output_that_overlaps_its_rows_is_refused():
     columns = torch.randn(32, 10, device="cuda")                             # copied first: may be written over
     want = layer_norm(columns.t())[0]
     assert torch.equal(layer_norm(columns.t(), out=columns.view(10, 32))[0], want)
+
+
+def test_offsets_beyond_32_bits():
+    """2^31 elements and more, by many rows and by rows far apart"""
+    from ai2bmd_amd.norm import layer_norm, layer_norm_backward
+    for rows, width, step in ((8_400_001, 256, 256), (2_101, 300, 1 << 20)):
+        few = 2_000
+        x, w, b, dy = make(few, width, torch.bfloat16, 5)
+        y, stats = layer_norm(x, w, b)
+        dx = layer_norm_backward(dy, x, stats, w, b)[0]
+        xs, dys = (torch.empty((rows - 1) * step + width, dtype=torch.bfloat16, device="cuda").as_strided((rows, width), (step, 1)) for _ in range(2))
+        for wide, part in ((xs, x), (dys, dy)):
+            if step == width:
+                wide.zero_()
+            else:
+                wide[:rows - few] = part[:rows - few]
+            wide[-few:] = part
+        out, st = layer_norm(xs, w, b)
+        grads = layer_norm_backward(dys, xs, st, w, b)
+        assert torch.equal(out[-few:], y) and torch.equal(st[-few:], stats) and torch.equal(grads[0][-few:], dx)
+        del xs, dys, out, grads
