@@ -21,8 +21,9 @@ namespace vsn {
 
 // Columns at ... at + VEC of a row, zeros behind its end.  ODD (16-bit rows of at least one vector that end within one): a lane
 // at the row's end loads the row's last whole vector and shifts its columns down, as nobody waits then for one that goes
-// element by element (30 011 x 509 f16: forward 17.4 -> 13.7 us, backward 35.9 -> 24.0; float32 rows, at most three such
-// elements, gain nothing, and rows of whole vectors would lose: 80 000 x 256 bf16 15.6 -> 16.6, 1 310 720 x 256 f32 454 -> 634).
+// element by element (30 011 x 509 f16: forward 17.5 -> 14.5 us, both directions 52.9 -> 37.1).  Rows of whole vectors keep the
+// branch: 80 000 rows bf16 forward, width 256 15.6 us and 16.5 this way, 192 13.4 and 14.2, 320 21.2 and 22.3; only the
+// backward pass gains at 320 (both directions 58.0 and 54.4).  So do float32 rows: 1 310 720 x 256 forward 454 us, 634 this way.
 template <typename T, int VEC, bool ODD>
 __device__ __forceinline__ void load_row(const T* __restrict__ p, int at, int width, float (&v)[VEC]) {
   if constexpr (ODD) {
@@ -234,11 +235,15 @@ static int norm_groups(int64_t rows, int rows_per_group, int cap) {
 // 1 310 720 x 80 bf16 83 and 155; 700 000 x 509 f16 382 and 396; 150 000 x 4096 f32 973 and 1111.  Float32 rows of ordinary
 // width that do not fit the 256 MB cache go the other way, as fresh waves keep more loads in flight than a wave's next turn:
 // 1 310 720 x 256 f32 552 us walking, 449 with one turn each; 200 000 x 256 78 and 72; 2 600 000 x 64 274 and 222;
-// 600 000 x 1024 984 and 853.
+// 600 000 x 1024 984 and 853.  But not where lanes of a row's only vector lie behind its end, or half of the lanes have no
+// second one: each load then waits for the one before (load_row), which a fresh wave pays for weight, bias and row alike.
+// 96 10^6 elements f32, walking and one turn each: width 96 147 and 215 us, 192 145 and 217, 240 150 and 177, 288 156 and 183,
+// 320 154 and 167, 352 155 and 155; 384 154 and 147, 448 151 and 136, 640 151 and 140; 64, 128 and 256 149 and 132.
 template <typename T>
 static int norm_forward_cap(int64_t rows, int width) {
   const bool beyond_cache = rows * width * 2 * (int64_t)sizeof(T) > (int64_t)256 << 20;
-  return sizeof(T) == 4 && width >= 64 && width <= 1024 && beyond_cache ? 1 << 20 : 2048;
+  const bool lanes_full = width <= 256 ? (width & (width - 1)) == 0 : width >= 384;
+  return sizeof(T) == 4 && width >= 64 && width <= 1024 && lanes_full && beyond_cache ? 1 << 20 : 2048;
 }
 
 struct NormArgs {

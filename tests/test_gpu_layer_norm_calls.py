@@ -100,3 +100,13 @@ def test_offsets_beyond_32_bits():
         grads = layer_norm_backward(dys, xs, st, w, b)
         assert torch.equal(out[-few:], y) and torch.equal(st[-few:], stats) and torch.equal(grads[0][-few:], dx)
         del xs, dys, out, grads
+
+
+@pytest.mark.parametrize("rows,width", [(180_001, 192), (110_001, 320), (360_001, 96), (270_001, 128), (90_001, 384)])
+def test_float32_rows_beyond_the_cache_of_any_width(rows, width):
+    """widths on both sides of the launch rule: lanes of a row all full, and not"""
+    from ai2bmd_amd.norm import layer_norm, layer_norm_backward
+    x, w, b, dy = make(rows, width, torch.float32, 11)
+    y, stats = layer_norm(x, w, b)
+    check(x, w, b, dy, y, layer_norm_backward(dy, x, stats, w, b))
+    assert torch.equal(layer_norm(x[-7:], w, b)[0], y[-7:])
