@@ -28,14 +28,17 @@ namespace vsn {
 namespace {
 
 // A workgroup of four waves reads each tile of rows once for 128 columns, a lone wave once for 32.  Sharing pays from a few
-// workgroups on, which pieces multiply, but narrow heads sooner: forward + backward of 3000 atoms bf16, dim 32, 192 workgroups
-// 353 us shared, 402 us alone; 1786 atoms f32, dim 64, 112 workgroups 615 us shared (its registers spill), 558 us alone.
+// workgroups on, which pieces multiply, and narrow heads sooner.  Forward + backward with a table, 8 heads, shared and alone:
+//   dim 32    104 workgroups (1600 atoms) bf16 224 and 242 us, f32 362 and 342; 192 (3000 atoms) bf16 401 and 455, f32 equal
+//   dim 64    104 workgroups bf16 345 and 325 us, f16 345 and 331, f32 622 and 601; 152 (2400 atoms) bf16 467 and 463, f16 479
+//             and 482, f32 equal; 192 bf16 587 and 615, f16 609 and 640, f32 1395 and 1474
+//   dim 128   104 workgroups bf16 721 and 696 us, f32 1273 and 1226; 192 bf16 1221 and 1245, f32 2849 and 3034
 constexpr int kCoopCols = kTile * kCoopWaves;
-inline int64_t coop_min(int dim) { return dim <= 32 ? 64 : 256; }
+inline int64_t coop_min(int dim) { return dim <= 32 ? 64 : 160; }
 // A run of rows is split into pieces where the items alone are too few waves for the 1024 SIMDs to be filled evenly
-// (12 rounds of one wave each); a piece keeps at least 2 tiles.  One protein of 175
-// atoms, forward: whole runs 19.6 us, pieces of 2 tiles 14.3 us with the join, of 1 tile 12.4 us; four proteins of up to 746
-// atoms, backward: of 4 tiles 185 us, of 2 tiles 190 us, of 1 tile 252 us.
+// (12 rounds of one wave each); a piece keeps at least 2 tiles.  Whole calls with pieces of 1, 2 and 4 tiles: one protein of
+// 175 atoms f32, forward, 18.1, 17.9 and 18.1 us; four proteins of up to 746 atoms f32, forward, 38.3 and 34.4 us, both
+// directions 229, 185 and 204 us; 8 read-out rows over up to 17 882 atoms bf16, forward, 42.6, 34.7 and 32.4 us.
 constexpr int64_t kPieceWaves = 12288;
 constexpr int kPieceTiles = 2;
 
