@@ -606,7 +606,7 @@ static int q_launch(const AttnPlanView& by_query, AttnParams p, int lone_workers
   if (by_query.lone) {
     p.work = by_query.lone_work, p.count = by_query.lone, p.workers = DELTA ? by_query.lone : lone_workers, p.part0 = 0;
     const int64_t total = (int64_t)p.workers * p.heads;
-    const int waves = lone_waves(total, lone_bytes);
+    const int waves = lone_waves(lone_bytes);
     if (!allow_lds((const void*)k_attn_bwd_q<T, DP, false, DELTA>, waves * lone_bytes)) return -5;
     hipLaunchKernelGGL((k_attn_bwd_q<T, DP, false, DELTA>), dim3((unsigned)((total + waves - 1) / waves)),
                        dim3(64 * waves), waves * lone_bytes, st, p, lone_bytes);
@@ -642,7 +642,7 @@ static int bwd_launch(const AttnPlanView& by_query, const AttnPlanView& by_key, 
   if (by_key.lone) {
     p.work = by_key.lone_work, p.count = by_key.lone;
     const int64_t total = (int64_t)by_key.lone * p.kv_heads;
-    const int waves = lone_waves(total, tab);
+    const int waves = lone_waves(tab);
     if (!allow_lds((const void*)k_attn_bwd_k<T, DP, false>, waves * tab)) return -5;
     hipLaunchKernelGGL((k_attn_bwd_k<T, DP, false>), dim3((unsigned)((total + waves - 1) / waves)), dim3(64 * waves),
                        waves * tab, st, p, tab);

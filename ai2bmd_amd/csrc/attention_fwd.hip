@@ -245,7 +245,7 @@ static int fwd_launch(const AttnPlanView& plan, AttnParams p, hipStream_t st) {
   if (plan.lone) {
     p.work = plan.lone_work, p.count = plan.lone;
     const int64_t total = (int64_t)plan.lone * p.heads;
-    const int waves = lone_waves(total, bytes);
+    const int waves = lone_waves(bytes);
     if (!allow_lds((const void*)k_attn_fwd<T, DP, false>, waves * bytes)) return -5;
     hipLaunchKernelGGL((k_attn_fwd<T, DP, false>), dim3((unsigned)((total + waves - 1) / waves)), dim3(64 * waves),
                        waves * bytes, st, p, bytes);

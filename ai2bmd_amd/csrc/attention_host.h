@@ -23,10 +23,12 @@ struct AttnPlanView {
   int joins, few;  // the first `few` of them have at most kFewSlots pieces
 };
 
-// Waves per workgroup where every wave has its own tiles: one while the items are few rounds of the chip, so that they
-// spread evenly (8136 tiles of four proteins, backward: 172 -> 160 us), else four (as far as LDS allows).
-inline int lone_waves(int64_t total, size_t bytes) {
-  int waves = total <= 16384 ? 1 : 4;
+// Waves per workgroup where every wave has its own tiles: four, as far as LDS allows.  One each instead: 8 read-out rows over
+// up to 17 882 atoms bf16 34.9 us (four: 28.4), 4096 fragments of 33 ... 64 rows bf16, dim 32, forward 157 us (144), four
+// proteins f32 and one of 746 atoms bf16 equal; only at dim 128, where LDS holds few, one is better (the 4096 fragments f32,
+// forward 1202 and 1278 us, bf16 466 and 476).
+inline int lone_waves(size_t bytes) {
+  int waves = 4;
   while (waves > 1 && waves * bytes > kLdsPerCu / 2) waves /= 2;
   return waves;
 }

@@ -787,7 +787,7 @@ template <typename T, int DP>
 static int pair_launch(const AttnParams& p, hipStream_t st) {
   const size_t bytes = PairLds<T, DP>::bytes(p.table ? p.n_rel : 0);
   const int64_t total = (int64_t)p.workers * p.heads;
-  const int waves = lone_waves(total, bytes);
+  const int waves = lone_waves(bytes);
   if (!allow_lds((const void*)k_attn_pair_bwd<T, DP>, waves * bytes)) return -5;
   hipLaunchKernelGGL((k_attn_pair_bwd<T, DP>), dim3((unsigned)((total + waves - 1) / waves)), dim3(64 * waves),
                      waves * bytes, st, p, bytes);

@@ -99,7 +99,7 @@ def test_workspace_is_for_the_terms_that_a_call_has():
 
 # Launch shapes of large batches: a worker of the backward passes takes a second item (from 4096 one-tile fragments, 4096 / heads
 # two-tile ones, 4096 / heads runs of 32 rows, 2048 / heads with a table or of 128 shared rows), and workgroups hold several
-# waves with LDS of their own (from 1024 waves of one-tile fragments, 16 384 of the others).
+# waves with LDS of their own (one-tile fragments from 1024 waves on, the others always).
 
 @pytest.mark.parametrize("T", TYPES, ids=str)
 def test_more_one_tile_fragments_than_workers(T):
