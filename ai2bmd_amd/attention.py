@@ -121,7 +121,7 @@ class FragmentAttention:
     # -- arguments ---------------------------------------------------------------------------------------------------
     def _rows(self, t, name: str, heads: int, least: int, dtype, exact=None):
         """The tensor as it is where the kernels can address it (dense last axis, 16-byte steps), else a copy."""
-        if not t.is_cuda or t.device != self.device:
+        if not t.is_cuda or t.device != self.device or t.is_neg():
             on_device(t, name, self.device)
         if t.dtype != dtype:
             raise ValueError(f"{name}: {dtype} expected, not {t.dtype}")
@@ -140,7 +140,7 @@ class FragmentAttention:
         return t
 
     def _small(self, t, name: str, shape, dtype):
-        if not t.is_cuda or t.device != self.device:
+        if not t.is_cuda or t.device != self.device or t.is_neg():
             on_device(t, name, self.device)
         if t.dtype != dtype or t.shape != shape:
             raise ValueError(f"{name}: {dtype} {tuple(shape)} expected, got {t.dtype} {tuple(t.shape)}")

@@ -27,6 +27,8 @@ def on_device(t: torch.Tensor, name: str, device=None) -> None:
         raise ValueError(f"{name}: this package is the MI355X path ('cuda:<k>' tensors only), got one on {t.device}")
     if device is not None and t.device != device:
         raise ValueError(f"{name} is on {t.device}, expected {device}")
+    if t.is_neg():  # its memory holds the negated values, and the kernels read memory
+        raise ValueError(f"{name}: a lazily negated view; call resolve_neg() first")
 
 
 def no_graph(*tensors) -> None:
@@ -71,7 +73,7 @@ def _span(t: torch.Tensor):
 
 
 def _param(p, x, name: str) -> None:
-    if not p.is_cuda or p.device != x.device:
+    if not p.is_cuda or p.device != x.device or p.is_neg():
         on_device(p, name, x.device)
     if p.shape != x.shape[-1:] or not p.is_contiguous():
         raise ValueError(f"{name}: contiguous [{x.shape[-1]}] expected, got {tuple(p.shape)}")

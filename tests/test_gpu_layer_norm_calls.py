@@ -110,3 +110,21 @@ def test_float32_rows_beyond_the_cache_of_any_width(rows, width):
     y, stats = layer_norm(x, w, b)
     check(x, w, b, dy, y, layer_norm_backward(dy, x, stats, w, b))
     assert torch.equal(layer_norm(x[-7:], w, b)[0], y[-7:])
+
+
+def test_lazily_negated_views_are_refused():
+    """their memory holds the values before the negation"""
+    from ai2bmd_amd.attention import FragmentAttention
+    from ai2bmd_amd.norm import layer_norm, layer_norm_backward
+    x, w, b, dy = make(8, 64, torch.float32, 2)
+    _, stats = layer_norm(x, w, b)
+    neg = torch._neg_view
+    plan = FragmentAttention([0], [8], 2, 32)
+    rows, pos, slope = x.view(8, 2, 32), x[:, :3].contiguous(), w[:2].contiguous()
+    for call in (lambda: layer_norm(neg(x), w, b), lambda: layer_norm(x, neg(w), b), lambda: layer_norm(x, w, neg(b)), lambda: layer_norm(x, out=neg(dy)),
+                 lambda: layer_norm_backward(neg(dy), x, stats, w, b), lambda: layer_norm_backward(dy, x, neg(stats), w, b),
+                 lambda: plan.forward(neg(rows), rows, rows), lambda: plan.forward(rows, neg(rows), rows), lambda: plan.forward(rows, rows, neg(rows)),
+                 lambda: plan.forward(rows, rows, rows, pos=neg(pos), slope=slope), lambda: plan.forward(rows, rows, rows, pos=pos, slope=neg(slope))):
+        with pytest.raises(ValueError, match="negated"):
+            call()
+    assert torch.equal(layer_norm(neg(x).resolve_neg(), w, b)[0], layer_norm(-x, w, b)[0])
