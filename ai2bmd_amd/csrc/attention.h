@@ -398,9 +398,9 @@ struct LongSum {
 };
 
 // Waves per SIMD that the tile kernels are compiled for: as many as fit without spilling, left alone the compiler hoists
-// its loads into twice the registers.  Three against one or two at 17 882 atoms bf16, dim 32: dq pass 10.2 -> 8.1 ms, dk / dv
-// pass 5.6 -> 4.3 ms (four spill and lose it again); two against one at 6007 atoms f16, dim 64: dq pass 1003 -> 607 us,
-// dk / dv pass 867 -> 530 us, forward 324 -> 226 us.
+// its loads into twice the registers.  17 882 atoms bf16, dim 32, both directions at two, three and four: 11.5, 10.5 and 17.2 ms
+// (the forward pass alone 1.7 ms at each); 6007 atoms f16, dim 64, at one and two: both directions 2.67 and 1.66 ms, forward
+// 343 and 256 us.
 template <typename T, int DP>
 constexpr int forward_waves() {
   return DP <= 32 ? 3 : DP > 64 && sizeof(T) == 4 ? 1 : 2;

@@ -16,8 +16,9 @@
 // P and dS enter a product in two parts of 16-bit rows' type (split8).  float16 has few exponents for that: P goes in
 // times 2^14, and dS times a power of two per column that follows the largest one seen so far.
 // All sums are in a fixed order; the table's are kept per wave in LDS.
-// Bound by vector instructions: 17 882 atoms, 8 heads of 32, bf16, distances and table: D 1.5 ms, dq 2.9 ms, dk / dv 3.3 ms;
-// 6007 atoms, 8 heads of 64, f16, table: 0.19, 0.59 and 0.49 ms.
+// 17 882 atoms, 8 heads of 32, bf16, distances and table: D 1.5 ms, dq 3.1 ms, dk / dv 3.7 ms, bound by vector instructions
+// (the units busy 95, 91 and 85 % by the counters); 6007 atoms, 8 heads of 64, f16, table: 0.18, 0.60 and 0.48 ms (69, 39 and
+// 54 %: the two waves per SIMD that registers allow wait for LDS and for one another).
 #include "attention.h"
 #include "attention_host.h"
 

@@ -1,10 +1,11 @@
 // Fragment attention, forward: one pass over the keys with a running maximum and sum (attention.h has the tile).
 //
 // S^T = K Q^T puts keys in rows and queries in lanes; the softmax of a query is then 16 registers and one exchange with
-// the other half of the wave, and O^T += V^T P^T takes P from the same registers.  16-bit rows take P
-// in two parts (split8); maximum, sum and output stay in float32.
-// Bound by vector instructions: 17 882 atoms, 8 heads of 32, bf16, with distances 1.34 ms (244 TFLOP/s of the two products;
-// some 320 instructions per tile, half of them distances); 6007 atoms, 8 heads of 64, f16, with a table 0.20 ms (368 TFLOP/s).
+// the other half of the wave, and O^T += V^T P^T takes P from the same registers.  16-bit rows take P in two parts (split8);
+// maximum, sum and output stay in float32.
+// Bound by vector instructions: 17 882 atoms, 8 heads of 32, bf16, with distances 1.62 ms (202 TFLOP/s of the two products; 347
+// instructions per tile by the counters, the vector units busy throughout, the matrix units 13 %); 6007 atoms, 8 heads of 64,
+// f16, with a table 0.24 ms (313 TFLOP/s; vector units busy 76 %) and 35 us of joining.
 #include "attention.h"
 #include "attention_host.h"
 

@@ -41,7 +41,9 @@ inline bool allow_lds(const void* kernel, size_t bytes) {
 }
 
 // Waves per small fragment: one that walks all heads, so distances are computed once and positions' gradients need no
-// joining - or, where the fragments alone would leave half of the 1024 SIMDs idle, one per key head.
+// joining - or, where the fragments alone would leave half of the 1024 SIMDs idle, one per key head.  8 heads of 32, both
+// directions, one wave and one per key head: 512 fragments f32 115 and 94 us, bf16 90 and 78; 1024 fragments f32 equal, bf16 99
+// and 103 (forward alone 25 and 23).
 inline int small_groups(int items, int kv_heads) { return items >= 512 ? 1 : kv_heads; }
 
 // workers of the backward passes that add up slope and table gradients, per list

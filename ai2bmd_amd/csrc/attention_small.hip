@@ -16,8 +16,8 @@
 
 namespace vsn {
 
-// Waves per SIMD that the backward kernel is compiled for (registers are what limits them: bf16 rows of 32 at one wave
-// 186 us, at two 121 us, at three, spilling, 417 us).
+// Waves per SIMD that the backward kernel is compiled for; registers are what limits them.  4096 fragments, heads of 32, both
+// directions at one, two and three (spilling): float32 440, 407 and 688 us, bf16 with the table 323, 323 and 409 us.
 template <typename T, int DP>
 constexpr int small_waves() {
   return DP > 64 || (DP > 32 && sizeof(T) == 4) ? 1 : 2;
@@ -498,8 +498,9 @@ __global__ __launch_bounds__(256, (small_waves<T, DP>())) void k_attn_small_bwd(
 // ---- fragments of two tiles: up to 64 queries and 64 keys ----
 // A wave takes a fragment and one key head.  All keys of a query are in registers (two tiles side by side), so here too
 // every score is computed once: 4 tiles instead of the 12 that the passes of attention_bwd.hip visit.  492 of 4096 fragments
-// (33 ... 44 rows), 8 heads: f32 127 us (the three passes 195), bf16 109 us (166).  Bound by latency: 16-bit rows spill at
-// two waves per SIMD and still beat one wave (127 us); float32 rows do not.
+// (33 ... 44 rows), 8 heads: f32 126 us (the three passes 63 more), bf16 105 us (47 more).  Bound by latency: 16-bit rows spill
+// at two waves per SIMD and still beat one wave (all fragments, both directions, 323 and 345 us); float32 rows do not (430 us
+// at two, 407 at one).
 template <typename T, int DP>
 struct PairLds {
   static constexpr size_t A = TileShape<T, DP>::BYTES, B = WeightTile<T>::BYTES;
@@ -710,7 +711,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 ? 1 : 2)) void k_attn_pair_bwd
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
               // rows beyond the last query pull by 0; 16-bit rows skip them, which keeps the loads from being hoisted into
-              // registers that spill (bf16 138 us without the branch, 109 us with it)
+              // registers that spill (bf16, all fragments, both directions: 347 us without the branch, 323 us with it)
               const int row = acc_row(r, hi);
               if (sizeof(T) == 4 || row < n_i) {
                 const float4 o = lds.qpos[i0 + row];

@@ -12,9 +12,9 @@
 // second launch, both in a fixed order (no atomics: equal inputs give equal bits).  All sums are float32.
 // Vector loads need only element alignment (gfx950 takes global addresses of any alignment); the row's last, partial
 // vector is stored element by element.
-// One MI355X (a large copy runs at 4.73 TB/s): forward 1 310 720 x 256 f32 0.46 ms (5.9 TB/s); 80 000 x 256 bf16 forward 16 us
-// (5.1, from the cache), backward 24 us (5.1) and 4 us for the second launch; 30 011 x 509 f16, rows at any address, 20 and
-// 27 us (3.0, 3.3) alone.
+// One MI355X (a large copy runs at 4.73 TB/s): forward 1 310 720 x 256 f32 0.45 ms (5.9 TB/s); 80 000 x 256 bf16 forward 16 us
+// (5.2, from the cache), backward 24 us (5.1) and 4 us for the second launch; 30 011 x 509 f16, rows at any address, 15 and
+// 21 us (4.1, 4.4) and 4 us.
 #include "typed.h"
 
 namespace vsn {

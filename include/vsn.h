@@ -316,7 +316,8 @@ int vsn_layernorm_backward(int device_id, int dtype, int param_dtype, const void
  * ViSNet/model/visnet_block.py:276-312, runs over <= 32 neighbours and has no softmax), its scores biased by distance and
  * by residue offset.  For query row i and key row j of one fragment, head a, key head a / (heads / kv_heads):
  *   s_ij = scale q_i.k_j - slope[a] |x_i - x_j| + table[a][bucket(res_j - res_i)],  P = softmax_j(s),  o_i = sum_j P_ij v_j
- * A row whose fragment has no keys, or whose scores are all -inf, gives 0 and no gradient.
+ * A row whose fragment has no keys, or whose scores are all -inf, gives 0 and no gradient.  A finite table entry beyond
+ * +-2.35e38 (a mask of the type's lowest value) counts as that value.
  *
  *   vsn_attn_create   the plan of a batch layout: fragment f's keys are rows host_start[f] ... host_end[f] - 1, its
  *     queries the same rows, or those of host_query_start / host_query_end (both NULL: the same), e.g. one read-out row
