@@ -170,16 +170,18 @@ constexpr int64_t kMaxRowStep = (int64_t)1 << 25;
 // A launch has fewer than 2^32 threads along an axis: whole workgroups of four waves here.  (Joins have fewer: there are
 // none from kPieceWaves waves on; the backward passes' workers are bounded by workers().)
 constexpr int64_t kMostGroups = ((int64_t)1 << 24) - 1;
-bool countable(const Lists& l, int heads) {
-  const int64_t waves = std::max(l.small.size(), std::max(l.pair.size(), l.lone.size())) * (int64_t)heads;
-  return (waves + 3) / 4 <= kMostGroups && (int64_t)l.coop.size() * heads <= kMostGroups;
+bool countable(const Lists& l, int heads, int kv_heads) {
+  const int64_t small = l.small.size(), lone = l.lone.size(), coop = l.coop.size();
+  const int64_t waves = std::max(lone * heads, small * small_groups((int)small, kv_heads));
+  return (waves + 3) / 4 <= kMostGroups && coop * heads <= kMostGroups;
 }
 // workgroups of the backward pass's last launch (join_launch): positions by block and fragment, slopes, table
 bool joinable(const vsn_attn& a, const vsn_attn_grads& g) {
   int64_t n = g.dslope ? a.heads : 0;
   if (g.dtable) n += (int64_t)a.heads * a.n_buckets;
-  if (g.dpos) n += (int64_t)a.by_key.blocks + a.by_query.pair + a.by_query.small;
-  if (g.dquery_pos) n += (int64_t)a.by_query.blocks + a.by_query.pair + a.by_query.small;
+  const int64_t small = small_groups(a.by_query.small, a.kv_heads) > 1 ? a.by_query.small : 0;
+  if (g.dpos) n += a.by_key.blocks + a.by_query.pair + small;
+  if (g.dquery_pos) n += a.by_query.blocks + a.by_query.pair + small;
   return n <= kMostGroups;
 }
 
@@ -320,7 +322,7 @@ extern "C" int vsn_attn_create(vsn_attn_handle* out, int device_id, int64_t n, c
     const Lists fwd = make_lists(n, qs, qe, host_start, host_end, heads, head_dim, small, false);
     const Lists by_query = make_lists(n, qs, qe, host_start, host_end, heads, head_dim, small, pair);
     const Lists by_key = make_lists(n, host_start, host_end, qs, qe, kv_heads, head_dim, small, pair);
-    if (!countable(fwd, heads) || !countable(by_query, heads) || !countable(by_key, kv_heads)) {
+    if (!countable(fwd, heads, kv_heads) || !countable(by_query, heads, kv_heads) || !countable(by_key, kv_heads, kv_heads)) {
       delete a;
       return -22;
     }

@@ -134,3 +134,5 @@ def test_plans_that_no_launch_could_count_are_refused(lib_built):
     assert create(65535, 1024) == fits and create(65536, 1024) == -22
     # workgroups of four waves that share the tiles of 128 rows: 2^24 of them
     assert create(16383, 1024, 65) == fits and create(16384, 1024, 65) == -22
+    # one-tile fragments by the million: one wave walks all heads
+    assert create(8_500_000, 8) == fits
