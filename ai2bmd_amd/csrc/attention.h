@@ -246,7 +246,7 @@ __device__ __forceinline__ typename vec8<T>::type load_col(const T* row, int at,
 // Eight weights (P, dS) as B operands of a product.  16-bit rows take them in two parts, hi + lo: one rounding to the rows'
 // type would put an error as large as the result's own rounding into every term, which the caller of 16-bit rows did not
 // ask for; two leave 2^-18 (bf16) and 2^-24 (f16) of a term.  The second product costs little, as the matrix units wait for
-// the vector ones; what it costs is the split, 6 instructions per pair of weights (bf16).  17 882 atoms bf16, dim 32: forward
+// the vector ones; what it costs is the split, 7 instructions per pair of weights (bf16).  17 882 atoms bf16, dim 32: forward
 // 1.35 -> 1.62 ms, both directions 9.2 -> 10.2 ms; 6007 atoms f16, dim 64, both 1.48 -> 1.65 ms; fragments gain nothing by
 // less (4096 of them bf16, both 0.332 and 0.338 ms).
 template <typename T>
