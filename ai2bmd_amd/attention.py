@@ -248,7 +248,8 @@ class FragmentAttention:
         address = lambda t: 0 if t is None else t.data_ptr()
         grads = capi.VsnAttnGrads(dout.data_ptr(), dout.stride(0), dout.stride(1), dq.data_ptr(), dk.data_ptr(),
                                   dv.data_ptr(), address(dpos), address(dquery_pos), address(dslope), address(dtable))
-        work, size = self._space(q.shape[0], k.shape[0], BACKWARD | (NO_POS if pos is None else 0) | (NO_TABLE if table is None else 0))
+        absent = (NO_POS if pos is None else 0) | (NO_TABLE if table is None else 0)
+        work, size = self._space(q.shape[0], k.shape[0], BACKWARD | absent)
         rc = self._L.vsn_attn_backward(self._h, C.byref(io), C.byref(grads), ptr(work), size, stream_of(q))
         if rc:
             raise RuntimeError(f"vsn_attn_backward failed ({rc})")

@@ -69,7 +69,9 @@ def _rows(t: torch.Tensor, width: int):
 def _span(t: torch.Tensor):
     """first address of a tensor and the one behind its last element"""
     first = t.data_ptr()
-    return first, first + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size() if t.numel() else first
+    if not t.numel():
+        return first, first
+    return first, first + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size()
 
 
 def _param(p, x, name: str) -> None:
@@ -102,7 +104,8 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, out=None):
     """y = (x - mean) / sqrt(var + eps) * weight + bias over the last axis -> (y, stats).
 
     `x` [..., width], float32 / bfloat16 / float16; evenly spaced rows are read in place, other layouts are copied.
-    `weight`, `bias` [width] of x's type or float32 (None: 1 and 0).  `out`: contiguous, of x's shape and type; x itself, or apart from all inputs.
+    `weight`, `bias` [width] of x's type or float32 (None: 1 and 0).  `out`: contiguous, of x's shape and type; x itself,
+    or apart from all inputs.
     `stats` float32 [rows, 2] (mean, 1 / sqrt(var + eps)) goes to layer_norm_backward.  On the current stream of x's device."""
     width, code, param_code = _check(x, weight, bias)
     no_graph(x, weight, bias, out)
