@@ -99,9 +99,9 @@ template <typename T>
 constexpr bool is_half() {
   return __is_same(T, _Float16);
 }
-// The reference that a maximum stands for in the exponentials.  (Where 14 is no exact step of the maximum, float32 could
-// round it to 16, and 2^16 is no float16 any more: such scores keep their maximum, next to it they are whole numbers.)
-constexpr float kExact = 0x1p20f;
+// The reference that a maximum stands for in the exponentials.  (From 2^25 on float32 could round the difference of 14 to 16,
+// and 2^16 is no float16 any more; below 2^24, where scores still tell one unit from the next, it is at most 15.)
+constexpr float kExact = 0x1p24f;
 template <typename T>
 __device__ __forceinline__ float exp_ref(float top) {
   return is_half<T>() && fabsf(top) < kExact ? top - 14.f : top;

@@ -40,10 +40,10 @@ def test_many_small_terms_under_one_large_one(T, n, queries):
 
 
 @pytest.mark.parametrize("sizes,queries", [([20], None), ([60], None), ([300], None), ([1700], [1])])
-@pytest.mark.parametrize("height", [2.0 ** 19.9, 2.0 ** 20.1, 1e8, 1.5e8, 3e9, -1e8, -1.5e8])
+@pytest.mark.parametrize("height", [2.0 ** 19.9, 1.162e7, -1.162e7, 1.163e7, -1.163e7, 2.3e7, -2.33e7, 1e8, 1.5e8, 3e9, -1e8, -1.5e8])
 def test_float16_scores_of_any_height(sizes, queries, height):
-    """equal scores, of a height at which float32 no longer tells 14 from 16: the mean over the keys (P to float16, the
-    result to float16), and gradients that are finite"""
+    """equal scores, up to a height at which float32 no longer tells 14 from 16 (2^24 in units of log 2 is 1.1629e7): the mean
+    over the keys (P to float16, the result to float16), and gradients that are finite"""
     case = Case(sizes, torch.float16, heads=2, dim=16, slope=False, lut=[0], queries=queries)
     case.q.zero_()
     case.terms["table"][:] = height
